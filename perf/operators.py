@@ -1,0 +1,383 @@
+"""What the set-transformer operators of ``hit_adv_amd.ops`` are measured on: differential attention, the root-mean-square norm (with a
+residual, with an 8-bit output) and dropout from a counter-based generator.  Every case runs in two ways on the same inputs: the plain form
+below (elementary torch operations in 32 bits) or, with ``own`` set, the framework's operators."""
+import math
+
+import torch
+
+own = False
+
+TYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+BYTES = {"fp32": 4, "bf16": 2, "fp16": 2}
+E4M3_MAX = 448.0
+EPS = 1e-6
+
+
+def _attn(name, B, Nq, Nk, H, Hkv, D, t, causal, ragged, train):
+    return {"name": name, "op": "attention", "B": B, "Nq": Nq, "Nk": Nk, "H": H, "Hkv": Hkv, "D": D, "type": t, "causal": causal,
+            "ragged": ragged, "train": train}
+
+
+def _norm(name, rows, cols, t, residual, mode):
+    return {"name": name, "op": "norm", "rows": rows, "cols": cols, "type": t, "residual": residual, "mode": mode}
+
+
+def _drop(name, rows, cols, t, residual, p):
+    return {"name": name, "op": "dropout", "rows": rows, "cols": cols, "type": t, "residual": residual, "p": p}
+
+
+def listed():
+    return [
+        # one attention layer of a point transformer over 32 clouds of 256 sampled points, 256 channels: the victim's forward pass ...
+        _attn("attn_cloud_fwd", 32, 256, 256, 4, 4, 32, "fp32", False, False, False),
+        # ... and with the gradients that an attack or a training step takes
+        _attn("attn_cloud_grad", 32, 256, 256, 4, 4, 32, "fp32", False, False, True),
+        # a training step over long ordered sequences
+        _attn("attn_long_grad", 2, 4096, 4096, 8, 8, 64, "bf16", True, False, True),
+        # clouds of unlike sizes padded to the largest, shared key/value heads, a head size that is no power of two
+        _attn("attn_ragged_fwd", 8, 1000, 1000, 8, 2, 48, "fp16", False, True, False),
+        # one new token for each of 16 sequences over a cache of up to 8192 keys
+        _attn("attn_token_cache", 16, 1, 8192, 16, 4, 64, "bf16", True, True, False),
+        # one token over a short cache: what a single call costs
+        _attn("attn_token_small", 1, 1, 200, 8, 8, 32, "bf16", True, False, False),
+        # the norm in front of that point transformer's layer with its gradients
+        _norm("norm_cloud_grad", 8192, 256, "fp32", False, "train"),
+        # a wide block's norm behind its residual, training
+        _norm("norm_wide_grad", 16384, 4096, "bf16", True, "train"),
+        # the same block's serving form: 8-bit rows with their scales for the products that follow
+        _norm("norm_wide_8bit", 16384, 4096, "bf16", True, "quant"),
+        # one token of it
+        _norm("norm_token_8bit", 1, 4096, "bf16", True, "quant"),
+        # the dropout behind that block's projection, added to the residual, training
+        _drop("dropout_wide_grad", 16384, 4096, "bf16", True, 0.1),
+        # the classifier heads' dropout: 32 clouds, 512 features
+        _drop("dropout_head_grad", 32, 512, "fp32", False, 0.2),
+    ]
+
+
+def _log(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    kind = rng.choice(["attention", "attention", "attention", "norm", "norm", "dropout"])
+    t = rng.choice(["fp32", "bf16", "fp16"])
+    if kind == "attention":
+        Hkv = rng.choice([1, 2, 3, 4, 8])
+        H = Hkv * rng.choice([1, 1, 2, 4, 7])
+        D = rng.choice([8, 16, 24, 32, 40, 48, 56, 64])
+        train = rng.random() < 0.5
+        B = _log(rng, 1, 32)
+        if not train and rng.random() < 0.4:  # a few new tokens over a cache
+            Nq, Nk = rng.choice([1, 1, 1, 2, 5]), _log(rng, 2, 16384)
+            Nq = min(Nq, Nk)
+        else:
+            Nq = _log(rng, 2, 4096)
+            Nk = Nq if rng.random() < 0.7 else max(2, min(4096, Nq + rng.randint(-Nq // 2, Nq)))
+        most = 6.0e9 * (1.0 if train else 3.0)  # no dearer than the long training step
+        while B > 1 and B * H * Nq * Nk * D > most:
+            B = max(1, B // 2)
+        while B * H * Nq * Nk * D > most:
+            Nq, Nk = max(2, Nq // 2), max(2, Nk // 2)
+        c = _attn("", B, Nq, Nk, H, Hkv, D, t, rng.random() < 0.5, rng.random() < 0.4, train)
+    elif kind == "norm":
+        rows, cols = _log(rng, 1, 32768), _log(rng, 8, 8192)
+        rows = max(1, min(rows, 16384 * 4096 // cols // (2 if t == "fp32" else 1)))
+        c = _norm("", rows, cols, t, rng.random() < 0.5, rng.choice(["fwd", "train", "quant"]))
+    else:
+        rows, cols = _log(rng, 1, 32768), _log(rng, 8, 8192)
+        rows = max(1, min(rows, 16384 * 4096 // cols // (2 if t == "fp32" else 1)))
+        c = _drop("", rows, cols, t, rng.random() < 0.5, rng.choice([0.0, 0.1, 0.25, 0.5, round(rng.uniform(0.01, 0.9), 3)]))
+    del c["name"]
+    return c
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    t = TYPES[case["type"]]
+
+    def randn(*shape, scale=1.0):
+        return (torch.randn(*shape, generator=g, device="cuda") * scale).to(t)
+
+    if case["op"] == "attention":
+        B, Nq, Nk, H, Hkv, D = (case[k] for k in ("B", "Nq", "Nk", "H", "Hkv", "D"))
+        s = {"q": randn(B, Nq, H, 2, D), "k": randn(B, Nk, Hkv, 2, D), "v": randn(B, Nk, Hkv, 2 * D),
+             # the learned weights start at 0.8 - 0.6 exp(-0.3 layer) and wander
+             "lam": torch.rand(H, generator=g, device="cuda") * 0.6 + 0.2, "lengths": None}
+        if case["ragged"]:
+            s["lengths"] = torch.randint(max(1, Nk // 4), Nk + 1, (B,), generator=g, device="cuda", dtype=torch.int32)
+        if case["train"]:
+            s["grad"] = randn(B, Nq, H, 2 * D)
+            for n in ("q", "k", "v", "lam"):
+                s[n].requires_grad_()
+    elif case["op"] == "norm":
+        r, c = case["rows"], case["cols"]
+        s = {"x": randn(r, c), "residual": randn(r, c, scale=2.0) if case["residual"] else None,
+             "weight": torch.rand(c, generator=g, device="cuda") + 0.5}
+        if case["mode"] == "train":
+            s["grad"] = randn(r, c)
+            s["grad_sum"] = randn(r, c) if case["residual"] else None
+            for n in ("x", "residual", "weight"):
+                if s[n] is not None:
+                    s[n].requires_grad_()
+    else:
+        r, c = case["rows"], case["cols"]
+        s = {"x": randn(r, c).requires_grad_(), "residual": randn(r, c).requires_grad_() if case["residual"] else None,
+             "grad": randn(r, c), "rng": torch.randint(0, 2 ** 62, (2,), generator=g, device="cuda", dtype=torch.int64)}
+    s["case"] = case
+    return s
+
+
+# ------------------------------------------------------------------ the framework's operators
+def _own(s):
+    from hit_adv_amd import ops
+    c = s["case"]
+    if c["op"] == "attention":
+        out = ops.diff_attention(s["q"], s["k"], s["v"], s["lam"], causal=c["causal"], key_lengths=s["lengths"])
+        if not c["train"]:
+            return {"out": out}
+        dq, dk, dv, dlam = torch.autograd.grad(out, (s["q"], s["k"], s["v"], s["lam"]), s["grad"])
+        return {"out": out, "dq": dq, "dk": dk, "dv": dv, "dlam": dlam}
+    if c["op"] == "norm":
+        if c["mode"] == "quant":
+            q, scale, total = ops.rms_norm_quant(s["x"], s["weight"], eps=EPS, residual=s["residual"])
+            return {"q": q, "scale": scale, "sum": total} if c["residual"] else {"q": q, "scale": scale}
+        if c["residual"]:
+            y, total = ops.rms_norm(s["x"], s["weight"], eps=EPS, residual=s["residual"])
+            if c["mode"] == "fwd":
+                return {"y": y, "sum": total}
+            dx, dr, dw = torch.autograd.grad((y, total), (s["x"], s["residual"], s["weight"]), (s["grad"], s["grad_sum"]))
+            return {"y": y, "sum": total, "dx": dx, "dr": dr, "dw": dw}
+        y = ops.rms_norm(s["x"], s["weight"], eps=EPS)
+        if c["mode"] == "fwd":
+            return {"y": y}
+        dx, dw = torch.autograd.grad(y, (s["x"], s["weight"]), s["grad"])
+        return {"y": y, "dx": dx, "dw": dw}
+    y = ops.dropout(s["x"], c["p"], s["rng"], residual=s["residual"])
+    if c["residual"]:
+        dx, dr = torch.autograd.grad(y, (s["x"], s["residual"]), s["grad"])
+        return {"y": y, "dx": dx, "dr": dr}
+    return {"y": y, "dx": torch.autograd.grad(y, s["x"], s["grad"])[0]}
+
+
+# ------------------------------------------------------------------ the plain forms
+def _hidden(c, lengths, device):
+    """[B or 1, 1, 1, Nq, Nk] truth values: the keys a query does not see."""
+    Nq, Nk = c["Nq"], c["Nk"]
+    j = torch.arange(Nk, device=device)
+    hidden = torch.zeros(1, 1, 1, Nq, Nk, dtype=torch.bool, device=device)
+    if c["causal"]:
+        hidden = hidden | (j[None, :] > torch.arange(Nq, device=device)[:, None] + (Nk - Nq))
+    if lengths is not None:
+        hidden = hidden | (j[None, :] >= lengths[:, None]).view(-1, 1, 1, 1, Nk)
+    return hidden
+
+
+def _plain_attention(s):
+    c = s["case"]
+    t, D, G = s["q"].dtype, c["D"], c["H"] // c["Hkv"]
+    scale = D ** -0.5
+    q = s["q"].detach().float().permute(0, 2, 3, 1, 4).contiguous()                                    # [B,H,2,Nq,D]
+    k = s["k"].detach().float().permute(0, 2, 3, 1, 4).repeat_interleave(G, dim=1)                     # [B,H,2,Nk,D]
+    v = s["v"].detach().float().permute(0, 2, 1, 3).repeat_interleave(G, dim=1)                        # [B,H,Nk,2D]
+    lam = s["lam"].detach().float().view(1, -1, 1, 1)
+    hidden = _hidden(c, s["lengths"], q.device)
+    S = torch.matmul(q, k.transpose(-1, -2)) * scale
+    S = S.masked_fill(hidden, float("-inf"))
+    m = S.amax(dim=-1, keepdim=True)
+    P = torch.exp(S - torch.where(m.isinf(), torch.zeros_like(m), m))
+    del S
+    total = P.sum(dim=-1, keepdim=True)
+    P = P / torch.where(total == 0, torch.ones_like(total), total)
+    A = P[:, :, 0] - lam * P[:, :, 1]                                                                  # [B,H,Nq,Nk]
+    out = torch.matmul(A, v).permute(0, 2, 1, 3).contiguous().to(t)
+    if not c["train"]:
+        return {"out": out}
+    g = s["grad"].float().permute(0, 2, 1, 3).contiguous()                                             # [B,H,Nq,2D]
+    dv = torch.matmul(A.transpose(-1, -2), g)
+    del A
+    dP = torch.matmul(g, v.transpose(-1, -2)).unsqueeze(2)
+    r = (P * dP).sum(dim=-1, keepdim=True)                                                             # [B,H,2,Nq,1]
+    dS = P * (dP - r) * scale
+    del P, dP
+    sign = torch.stack([torch.ones_like(lam), -lam], dim=2)                                            # [1,H,2,1,1]
+    dS = dS * sign
+    dq = torch.matmul(dS, k).permute(0, 3, 1, 2, 4).contiguous().to(t)
+    dk = torch.matmul(dS.transpose(-1, -2), q)
+    B, Hkv, Nk = c["B"], c["Hkv"], c["Nk"]
+    dk = dk.view(B, Hkv, G, 2, Nk, D).sum(dim=2).permute(0, 3, 1, 2, 4).contiguous().to(t)
+    dv = dv.view(B, Hkv, G, Nk, 2 * D).sum(dim=2).permute(0, 2, 1, 3).contiguous().to(t)
+    dlam = -r[:, :, 1].sum(dim=(0, 2, 3))
+    return {"out": out, "dq": dq, "dk": dk, "dv": dv, "dlam": dlam}
+
+
+def _plain_norm(s):
+    c = s["case"]
+    t = s["x"].dtype
+    total = s["x"].detach()
+    if c["residual"]:
+        total = (total.float() + s["residual"].detach().float()).to(t)  # the sum is an output: the norm is that of the stored values
+    f, w = total.float(), s["weight"].detach().float()
+    r = torch.rsqrt((f * f).mean(dim=-1, keepdim=True) + EPS)
+    n = f * r
+    y = n * w
+    if c["mode"] == "quant":
+        scale = y.abs().amax(dim=-1) / E4M3_MAX
+        scale = torch.where(scale == 0, torch.ones_like(scale), scale)
+        q = (y / scale[:, None]).clamp(-E4M3_MAX, E4M3_MAX).to(torch.float8_e4m3fn)
+        return {"q": q, "scale": scale, "sum": total} if c["residual"] else {"q": q, "scale": scale}
+    if c["mode"] == "fwd":
+        return {"y": y.to(t), "sum": total} if c["residual"] else {"y": y.to(t)}
+    dy = s["grad"].float()
+    dw = (dy * n).sum(dim=0)
+    a = dy * w
+    dx = r * (a - n * (a * n).mean(dim=-1, keepdim=True))
+    if c["residual"]:
+        dx = (dx + s["grad_sum"].float()).to(t)
+        return {"y": y.to(t), "sum": total, "dx": dx, "dr": dx.clone(), "dw": dw}
+    return {"y": y.to(t), "dx": dx.to(t), "dw": dw}
+
+
+_LOW = 0xFFFFFFFF
+
+
+def _mul_hi_lo(a, m):
+    """High and low 32 bits of the product of two 32-bit numbers held in int64."""
+    a_hi, a_lo, m_hi, m_lo = a >> 16, a & 0xFFFF, m >> 16, m & 0xFFFF
+    low = a_lo * m_lo
+    mid = a_hi * m_lo + (low >> 16)
+    mid2 = a_lo * m_hi + (mid & 0xFFFF)
+    return a_hi * m_hi + (mid >> 16) + (mid2 >> 16), ((mid2 & 0xFFFF) << 16) | (low & 0xFFFF)
+
+
+def _philox_words(n, rng):
+    """The first n 32-bit words of Philox4x32-10 (Salmon, Moraes, Dror, Shaw 2011): block b of four has the counter
+    (b low, b high, offset low, offset high) and the key (seed low, seed high)."""
+    b = torch.arange((n + 3) // 4, device=rng.device, dtype=torch.int64)
+    seed, offset = rng[0], rng[1]
+    c0, c1 = b & _LOW, b >> 32
+    c2, c3 = (offset & _LOW).expand_as(b), ((offset >> 32) & _LOW).expand_as(b)
+    k0, k1 = seed & _LOW, (seed >> 32) & _LOW
+    for _ in range(10):
+        h0, l0 = _mul_hi_lo(c0, 0xD2511F53)
+        h1, l1 = _mul_hi_lo(c2, 0xCD9E8D57)
+        c0, c1, c2, c3 = h1 ^ c1 ^ k0, l1, h0 ^ c3 ^ k1, l0
+        k0, k1 = (k0 + 0x9E3779B9) & _LOW, (k1 + 0xBB67AE85) & _LOW
+    return torch.stack([c0, c1, c2, c3], dim=1).view(-1)[:n]
+
+
+def _plain_dropout(s):
+    c = s["case"]
+    x = s["x"].detach()
+    keep = (_philox_words(x.numel(), s["rng"]) >= round(c["p"] * 2 ** 32)).view(x.shape)
+    factor = keep.float() * (1.0 / (1.0 - c["p"]))
+    y = x.float() * factor
+    dx = (s["grad"].float() * factor).to(x.dtype)
+    if c["residual"]:
+        return {"y": (y + s["residual"].detach().float()).to(x.dtype), "dx": dx, "dr": s["grad"].clone()}
+    return {"y": y.to(x.dtype), "dx": dx}
+
+
+def run(state):
+    if own:
+        return _own(state)
+    return {"attention": _plain_attention, "norm": _plain_norm, "dropout": _plain_dropout}[state["case"]["op"]](state)
+
+
+# ------------------------------------------------------------------ what a pass cannot do without
+def work(case):
+    e = BYTES[case["type"]]
+    if case["op"] == "attention":
+        B, Nq, Nk, H, Hkv, D = (case[k] for k in ("B", "Nq", "Nk", "H", "Hkv", "D"))
+        share = 0.625 if case["ragged"] else 1.0  # lengths are uniform between a quarter and all of the keys
+        pairs = Nq * Nk * share
+        if case["causal"]:
+            pairs = share * sum(min(max(i + Nk - Nq + 1, 0), Nk) for i in range(Nq))
+        rows, keys = B * Nq * H, B * Nk * Hkv * share
+        if case["train"]:  # q, k, v, the output's gradient in; the output, dq, dk, dv out; three more products of each kind
+            return {"bytes": e * (rows * 8 * D + keys * 8 * D), "flops": 24.0 * D * pairs * B * H}
+        return {"bytes": e * (rows * 4 * D + keys * 4 * D), "flops": 8.0 * D * pairs * B * H}
+    n = case["rows"] * case["cols"]
+    if case["op"] == "norm":
+        r = 1 if case["residual"] else 0
+        if case["mode"] == "quant":
+            return {"bytes": n * (e * (1 + 2 * r) + 1) + 4 * case["rows"] + 4 * case["cols"], "flops": 5.0 * n}
+        if case["mode"] == "fwd":
+            return {"bytes": n * e * (2 + 2 * r) + 4 * case["cols"], "flops": 4.0 * n}
+        return {"bytes": n * e * (2 + 2 * r + 3 + r) + 8 * case["cols"], "flops": 14.0 * n}
+    return {"bytes": n * e * (4 + (1 if case["residual"] else 0)), "flops": 4.0 * n}
+
+
+# ------------------------------------------------------------------ the definitions in 64 bits
+def _exact_attention(c, s):
+    t, D, G = s["q"].dtype, c["D"], c["H"] // c["Hkv"]
+    q, k, v, lam = (s[n].detach().double().requires_grad_(c["train"]) for n in ("q", "k", "v", "lam"))
+    parts, grads = [], {n: torch.zeros_like(x) for n, x in (("q", q), ("k", k), ("v", v), ("lam", lam))}
+    out = torch.empty(c["B"], c["Nq"], c["H"], 2 * D, dtype=torch.float64, device=q.device)
+    for b in range(c["B"]):
+        n = int(s["lengths"][b]) if s["lengths"] is not None else c["Nk"]
+        for h in range(c["H"]):
+            maps = []
+            for i in range(2):
+                e = (q[b, :, h, i] @ k[b, :n, h // G, i].t()) / math.sqrt(D)
+                if c["causal"]:
+                    last = torch.arange(c["Nq"], device=e.device) + (c["Nk"] - c["Nq"])
+                    unseen = torch.arange(n, device=e.device).view(1, -1) > last.view(-1, 1)
+                    empty = unseen.all(dim=1, keepdim=True)
+                    e = e.masked_fill(unseen & ~empty, -math.inf)
+                    maps.append(torch.softmax(e, dim=1).masked_fill(empty, 0.0))
+                else:
+                    maps.append(torch.softmax(e, dim=1))
+            o = maps[0] @ v[b, :n, h // G] - lam[h] * (maps[1] @ v[b, :n, h // G])
+            out[b, :, h] = o.detach()
+            if c["train"]:
+                for name, x in zip(("q", "k", "v", "lam"), torch.autograd.grad(o, (q, k, v, lam), s["grad"][b, :, h].double())):
+                    grads[name] += x
+            del maps, o, e
+    if not c["train"]:
+        return {"out": out}
+    return {"out": out, "dq": grads["q"], "dk": grads["k"], "dv": grads["v"], "dlam": grads["lam"]}
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    if case["op"] == "attention":
+        with torch.enable_grad():
+            # every head's gradient writes the whole leaves: leave the cases out where that takes long
+            size = s["k"].numel() * 2 + s["v"].numel() + s["q"].numel()
+            if case["train"] and case["B"] * case["H"] * size > 3e10:
+                return None
+            return _exact_attention(case, s)
+    if case["op"] == "norm":
+        total = s["x"].detach().double()
+        if case["residual"]:
+            total = (total + s["residual"].detach().double()).to(s["x"].dtype).double()
+        leaf, w = total.requires_grad_(), s["weight"].detach().double().requires_grad_()
+        y = leaf * w / torch.sqrt(leaf.pow(2).mean(dim=1, keepdim=True) + EPS)
+        if case["mode"] == "quant":
+            return {"q": None, "scale": y.detach().abs().max(dim=1)[0] / E4M3_MAX, **({"sum": total.detach()} if case["residual"] else {})}
+        if case["mode"] == "fwd":
+            return {"y": y.detach(), **({"sum": total.detach()} if case["residual"] else {})}
+        dx, dw = torch.autograd.grad(y, (leaf, w), s["grad"].double())
+        if case["residual"]:
+            dx = dx + s["grad_sum"].double()
+            return {"y": y.detach(), "sum": total.detach(), "dx": dx, "dr": dx, "dw": dw}
+        return {"y": y.detach(), "dx": dx, "dw": dw}
+    import numpy as np
+    # the generator once more on the host, in numpy's unsigned arithmetic
+    n = s["x"].numel()
+    seed_, offset = (int(v) for v in s["rng"].tolist())
+    b = np.arange((n + 3) // 4, dtype=np.uint64)
+    low, sh = np.uint64(0xFFFFFFFF), np.uint64(32)
+    c = [b & low, b >> sh, np.full_like(b, offset & 0xFFFFFFFF), np.full_like(b, (offset >> 32) & 0xFFFFFFFF)]
+    k0, k1 = seed_ & 0xFFFFFFFF, (seed_ >> 32) & 0xFFFFFFFF
+    for _ in range(10):
+        p0, p1 = c[0] * np.uint64(0xD2511F53), c[2] * np.uint64(0xCD9E8D57)
+        c = [(p1 >> sh) ^ c[1] ^ np.uint64(k0), p1 & low, (p0 >> sh) ^ c[3] ^ np.uint64(k1), p0 & low]
+        k0, k1 = (k0 + 0x9E3779B9) & 0xFFFFFFFF, (k1 + 0xBB67AE85) & 0xFFFFFFFF
+    words = np.stack(c, axis=1).reshape(-1)[:n]
+    factor = torch.from_numpy((words >= np.uint64(round(case["p"] * 2 ** 32))).astype(np.float64)).cuda().view_as(s["x"]) / (1.0 - case["p"])
+    y, dx = s["x"].detach().double() * factor, s["grad"].double() * factor
+    if case["residual"]:
+        return {"y": y + s["residual"].detach().double(), "dx": dx, "dr": s["grad"].double()}
+    return {"y": y, "dx": dx}
