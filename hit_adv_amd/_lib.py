@@ -120,12 +120,22 @@ PROTOTYPES = {
     "hitadv_lrelu_pool_bwd": [_P, _P, _P, _I, _I, _I, _F, _P, _P],
     "hitadv_fc_layer": [_P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P],
     "hitadv_fc_layer_scratch_floats": [_I, _I, _I],
+    "hitadv_diff_attention_supported": [_I, _L, _L, _L, _L, _L, _L],
+    "hitadv_diff_attention_scratch_floats": [_I] * 6,
+    "hitadv_diff_attention_fwd": [_I, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P, _P, _P, _P],
+    "hitadv_diff_attention_bwd": [_I, _P, _P, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P, _P, _P, _P, _P, _P],
+    "hitadv_rms_norm_fwd": [_I, _I, _P, _P, _P, _L, _I, _F, _P, _P, _P, _P],
+    "hitadv_rms_norm_e4m3": [_I, _I, _P, _P, _P, _L, _I, _F, _P, _P, _P, _P],
+    "hitadv_rms_norm_bwd_scratch_floats": [_L, _I],
+    "hitadv_rms_norm_bwd": [_I, _I, _P, _P, _P, _P, _P, _L, _I, _P, _P, _P, _P],
+    "hitadv_dropout": [_I, _P, _P, _P, _L, _P, _c.c_uint64, _F, _P],
     "hitadv_fc_layer_pre": [_P, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P],
 }
 _RESTYPE = {"hitadv_version": _c.c_char_p, "hitadv_deform_bwd_scratch_floats": _c.c_int64,
             "hitadv_max_over_points_scratch": _c.c_int64, "hitadv_linear_max_fwd_scratch": _c.c_int64, "hitadv_linear_max_fwd_bf16x3_scratch": _c.c_int64, "hitadv_pointnet_rowmlp_tiles": _c.c_int64, "hitadv_pointnet_rowmlp_bwd_tiles": _c.c_int64, "hitadv_fc_layer_scratch_floats": _c.c_int64, "hitadv_regulariser_scratch_floats": _c.c_int64,
             "hitadv_edge_max_bwd_scratch_ints": _c.c_int64, "hitadv_iteration_head_scratch_floats": _c.c_int64, "hitadv_deform_bwd_slabs": _c.c_int64, "hitadv_group_add_relu_bwd_scratch_ints": _c.c_int64,
-            "hitadv_linear_lrelu_pool_scratch": _c.c_int64}
+            "hitadv_linear_lrelu_pool_scratch": _c.c_int64, "hitadv_diff_attention_scratch_floats": _c.c_int64,
+            "hitadv_rms_norm_bwd_scratch_floats": _c.c_int64}
 
 _lib = None
 

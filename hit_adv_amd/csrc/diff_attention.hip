@@ -1,0 +1,943 @@
+// Differential attention: the difference of two softmax maps over shared values, with a learned weight per head.
+//
+//     P_m[i,j] = softmax over the visible j of  scale q[i,m] . k[j,m]   (m = 1, 2)
+//     out[i]   = sum_j (P_1[i,j] - lam P_2[i,j]) v[j]
+//
+// q [B,Nq,H,2,D], k [B,Nk,Hkv,2,D], v [B,Nk,Hkv,2D], out [B,Nq,H,2D]; H / Hkv = G query heads share one key / value head.  A key is
+// visible below its cloud's length and, if causal, at j <= i + Nk - Nq.  A row that sees nothing gives 0 and has no gradient.
+//
+// Arithmetic.  Everything runs on the 16-bit matrix cores with fp32 accumulators.  The products of two inputs (the scores, dO V^T) take
+// bf16 and fp16 inputs as they are: every product is exact.  fp32 inputs enter as three bf16 pieces whose sum is the value (each the
+// truncation of what is left) and six piece products.  The products with a map on one side (P V and those of the backward pass) are
+// always bf16 pieces, also where the inputs are fp16 (two pieces, exact): a bf16 piece has fp32's exponent, so neither a small
+// probability nor a large gradient leaves the range.  The map itself is two pieces (three in fp32) also where the inputs are bf16:
+// rounding P_1 and P_2 to one bf16 each before their difference is taken puts back the noise that the difference is there to cancel,
+// and one-piece dS and A = P_1 - lam P_2 put the gradients at 1.5x the error of their own last rounding (two: 1.0x).  Maxima, sums
+// and accumulators are fp32.  A value that is not finite makes the rows that see it NaN.
+//
+// Layout.  All products are computed transposed so that no map ever leaves the registers: S^T = K Q^T has the query in the lane (column
+// lane & 31) and 16 keys in its registers, which is -- with the keys of a 16-chunk in the order 4h..4h+3, 8+4h..8+4h+3 for lane half h --
+// exactly the B operand of O^T = V^T P^T.  The transposed tiles (V^T here, K^T, Q^T and dO^T in the backward pass) are written to LDS in
+// that key order, so that an A operand is one 16-byte read.  Rows of one key / value head's G query heads are packed (row r = query r / G,
+// head r % G): a tile of 32 rows then shares every key and value it stages, for a single new token too.
+#include "elements.hpp"
+#include "hitadv.h"
+
+namespace hitadv {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int DA_T = 32;          // rows (keys) of a tile = the matrix instruction's width
+constexpr int DA_TS = DA_T + 8;   // row stride of a transposed tile (16-bit elements): 80 bytes, 16 rows on 16 different bank groups
+constexpr float DA_LOG2E = 1.4426950408889634f;
+constexpr float DA_SLACK = 8.0f;  // the running maximum is raised only when it would rise by 2^8: a probability stays below 2^8
+#define DA_INF __builtin_inff()
+
+struct DaP {
+  const void *q, *k, *v, *dout;
+  const float *lam;
+  const int *lengths;
+  void *out;             // forward: out; backward: unused
+  void *dq, *dk, *dv;
+  float *stats;          // [4][B*H*Nq]: running maximum and log2 of the sum, map 1 then map 2
+  float *r;              // [2][B*H*Nq]: sum_j P_m dP
+  float *part_o, *part_ml;
+  int64_t q_b, q_n, q_h, q_m, k_b, k_n, k_h, k_m, v_b, v_n, v_h;
+  int B, Nq, Nk, H, Hkv, D, G, lam_n, causal, rows, chunk, splits;
+  uint32_t g_magic;      // ceil(2^32 / G), G > 1
+  float scale, scale2;   // scale, scale * log2(e)
+};
+
+__device__ __forceinline__ int da_div_g(const DaP &p, int r) { return p.G == 1 ? r : (int)(((uint64_t)(uint32_t)r * p.g_magic) >> 32); }
+__device__ __forceinline__ float da_lam(const DaP &p, int h) { return p.lam[p.lam_n == 1 ? 0 : h]; }
+__device__ __forceinline__ int da_len(const DaP &p, int b) {
+  return p.lengths ? max(0, min(p.lengths[b], p.Nk)) : p.Nk;
+}
+// the first key that query i does not see
+__device__ __forceinline__ int da_limit(const DaP &p, int i, int len) {
+  return p.causal ? max(0, min(len, i + p.Nk - p.Nq + 1)) : len;
+}
+
+// ---------------------------------------------------------------------------------------------------------------- elements and pieces
+
+template <int NP> struct Raw8 { uint4 a; };
+template <> struct Raw8<3> { float4 a, b; };
+template <int NP> struct Raw4 { uint2 a; };
+template <> struct Raw4<3> { float4 a; };
+
+template <int NP> __device__ __forceinline__ Raw8<NP> da_load8(const void *base, int64_t at, bool ok) {
+  Raw8<NP> r;
+  if constexpr (NP == 3) {
+    r.a = r.b = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (ok) {
+      const float4 *s = (const float4 *)((const float *)base + at);
+      r.a = s[0];
+      r.b = s[1];
+    }
+  } else {
+    r.a = make_uint4(0u, 0u, 0u, 0u);
+    if (ok) r.a = *(const uint4 *)((const uint16_t *)base + at);
+  }
+  return r;
+}
+template <int NP> __device__ __forceinline__ Raw4<NP> da_load4(const void *base, int64_t at, bool ok) {
+  Raw4<NP> r;
+  if constexpr (NP == 3) {
+    r.a = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (ok) r.a = *(const float4 *)((const float *)base + at);
+  } else {
+    r.a = make_uint2(0u, 0u);
+    if (ok) r.a = *(const uint2 *)((const uint16_t *)base + at);
+  }
+  return r;
+}
+
+// the pieces of a value, each a bf16 in the upper half of a word
+template <int NP> __device__ __forceinline__ void da_pieces(float f, uint32_t (&p)[NP]) {
+  p[0] = __float_as_uint(f) & 0xffff0000u;
+  if constexpr (NP >= 2) {
+    const float r1 = f - __uint_as_float(p[0]);
+    p[1] = __float_as_uint(r1) & 0xffff0000u;
+    if constexpr (NP == 3) p[2] = __float_as_uint(r1 - __uint_as_float(p[1]));
+  }
+}
+
+// eight values of a row -> the operand(s) of a product of two inputs: 16-bit elements as they are, fp32 as three pieces
+template <int NP> constexpr int DA_NR = NP == 3 ? 3 : 1;
+template <int NP> __device__ __forceinline__ void da_pieces8(const Raw8<NP> &r, uint4 (&out)[DA_NR<NP>]) {
+  if constexpr (NP != 3) {
+    out[0] = r.a;
+  } else {
+    const float f[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+    uint32_t p[8][3];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) da_pieces<3>(f[i], p[i]);
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+      out[k] = make_uint4(pack_hi(p[0][k], p[1][k]), pack_hi(p[2][k], p[3][k]), pack_hi(p[4][k], p[5][k]), pack_hi(p[6][k], p[7][k]));
+  }
+}
+// four rows of four values -> for each piece and column the four rows' values (a 4 x 4 transposition)
+template <int NP> __device__ __forceinline__ void da_transpose4(const Raw4<NP> (&r)[4], uint2 (&out)[NP][4]) {
+  uint32_t p[4][4][NP];  // [row][column][piece]
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (NP == 3) {
+      da_pieces<NP>(r[i].a.x, p[i][0]);
+      da_pieces<NP>(r[i].a.y, p[i][1]);
+      da_pieces<NP>(r[i].a.z, p[i][2]);
+      da_pieces<NP>(r[i].a.w, p[i][3]);
+    } else if constexpr (NP == 2) {
+      da_pieces<NP>(f16_bits_to_float(r[i].a.x & 0xffffu), p[i][0]);
+      da_pieces<NP>(f16_bits_to_float(r[i].a.x >> 16), p[i][1]);
+      da_pieces<NP>(f16_bits_to_float(r[i].a.y & 0xffffu), p[i][2]);
+      da_pieces<NP>(f16_bits_to_float(r[i].a.y >> 16), p[i][3]);
+    } else {
+      p[i][0][0] = r[i].a.x << 16;
+      p[i][1][0] = r[i].a.x & 0xffff0000u;
+      p[i][2][0] = r[i].a.y << 16;
+      p[i][3][0] = r[i].a.y & 0xffff0000u;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < NP; ++k)
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      out[k][c] = make_uint2(pack_hi(p[0][c][k], p[1][c][k]), pack_hi(p[2][c][k], p[3][c][k]));
+}
+
+// eight probabilities -> NPP pieces, each the B operand of a matrix instruction
+template <int NPP> __device__ __forceinline__ void da_operand(const float *x, bf16x8 (&out)[NPP]) {
+  if constexpr (NPP == 3) {
+    uint32_t p[8][3];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) da_pieces<3>(x[i], p[i]);
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+      out[k] = as_bf16x8(make_uint4(pack_hi(p[0][k], p[1][k]), pack_hi(p[2][k], p[3][k]), pack_hi(p[4][k], p[5][k]), pack_hi(p[6][k], p[7][k])));
+  } else {
+    uint32_t w[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = bf16_pair(x[2 * i], x[2 * i + 1]);
+      if constexpr (NPP == 2)
+        l[i] = bf16_pair(x[2 * i] - __uint_as_float(w[i] << 16), x[2 * i + 1] - __uint_as_float(w[i] & 0xffff0000u));
+    }
+    out[0] = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
+    if constexpr (NPP == 2) out[1] = as_bf16x8(make_uint4(l[0], l[1], l[2], l[3]));
+  }
+}
+
+// c += a b over the pieces that count: weights 2^-8(i + j) with i + j < max(NA, NB)
+template <int NA, int NB> __device__ __forceinline__ f32x16 da_mfma(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB], f32x16 c) {
+  constexpr int CUT = NA > NB ? NA : NB;
+#pragma unroll
+  for (int s = CUT - 1; s >= 0; --s)  // the small products first
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+        if (i + j == s) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[j], c, 0, 0, 0);
+  return c;
+}
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+// c += a b for two inputs' operands
+template <int NP> __device__ __forceinline__ f32x16 da_mfma_in(const bf16x8 (&a)[DA_NR<NP>], const bf16x8 (&b)[DA_NR<NP>], f32x16 c) {
+  if constexpr (NP == 2)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a[0]), __builtin_bit_cast(f16x8, b[0]), c, 0, 0, 0);
+  else
+    return da_mfma<DA_NR<NP>, DA_NR<NP>>(a, b, c);
+}
+
+// ---------------------------------------------------------------------------------------------------------------- LDS tiles
+// a tile of 32 rows: [DA_NR][32][2 DP + 8]; its transpose: [NP][2 DP][DA_TS] with the rows in operand order
+template <int NP, int DP> struct DaTile {
+  static constexpr int W = 2 * DP, RS = W + 8, NR = DA_NR<NP>;
+  static constexpr int ROWS = NR * DA_T * RS, COLS = NP * W * DA_TS;  // 16-bit elements
+  static __device__ __forceinline__ void frag_row(const uint16_t *t, int row, int col, bf16x8 (&f)[NR]) {
+#pragma unroll
+    for (int k = 0; k < NR; ++k) f[k] = as_bf16x8(*(const uint4 *)(t + (k * DA_T + row) * RS + col));
+  }
+  static __device__ __forceinline__ void frag_col(const uint16_t *t, int col, int chunk, int half, bf16x8 (&f)[NP]) {
+#pragma unroll
+    for (int k = 0; k < NP; ++k) f[k] = as_bf16x8(*(const uint4 *)(t + (k * W + col) * DA_TS + 16 * chunk + 8 * half));
+  }
+  static __device__ __forceinline__ void put_row(uint16_t *t, int row, int col, const Raw8<NP> &r) {
+    uint4 p[NR];
+    da_pieces8<NP>(r, p);
+#pragma unroll
+    for (int k = 0; k < NR; ++k) *(uint4 *)(t + (k * DA_T + row) * RS + col) = p[k];
+  }
+  // rows 4 rg .. 4 rg + 3, columns col .. col + 3: key 16 c + 8 y + 4 x + j sits at 16 c + 8 x + 4 y + j
+  static __device__ __forceinline__ void put_col(uint16_t *t, int rg, int col, const Raw4<NP> (&r)[4]) {
+    uint2 o[NP][4];
+    da_transpose4<NP>(r, o);
+    const int at = 16 * (rg >> 2) + 8 * (rg & 1) + 4 * ((rg >> 1) & 1);
+#pragma unroll
+    for (int k = 0; k < NP; ++k)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) *(uint2 *)(t + (k * W + col + c) * DA_TS + at) = o[k][c];
+  }
+};
+
+// where a tile's rows come from: element offset of row `row`'s column `col` of the padded [2][DP] (or [2 DP]) row, or -1 for a zero
+template <int DP> struct DaKeys {  // key rows t .. t + 31 of k (maps of D) or v (2 D in one piece)
+  int64_t base, n, m;
+  int t, end, D;
+  bool maps;
+  __device__ __forceinline__ int64_t at(int row, int col) const {
+    const int key = t + row;
+    if (maps) {
+      const int map = col >= DP, d = col - (map ? DP : 0);
+      return key < end && d < D ? base + key * n + map * m + d : -1;
+    }
+    return key < end && col < 2 * D ? base + key * n + col : -1;
+  }
+};
+template <int DP> struct DaRows {  // packed query rows t .. t + 31 of q (maps) or dout
+  int64_t base, n, h, m;
+  int t, end, D;
+  bool maps;
+  const DaP *p;
+  __device__ __forceinline__ int64_t at(int row, int col) const {
+    const int r = t + row;
+    if (r >= end) return -1;
+    const int i = da_div_g(*p, r), g = r - i * p->G;
+    if (maps) {
+      const int map = col >= DP, d = col - (map ? DP : 0);
+      return d < D ? base + i * n + g * h + map * m + d : -1;
+    }
+    return col < 2 * D ? base + i * n + g * h + col : -1;
+  }
+};
+
+template <int NP, int DP, class SRC> __device__ __forceinline__ void da_stage_rows(uint16_t *t, const void *src, const SRC &s, int tid, int nt) {
+  constexpr int CH = 2 * DP / 8;
+  for (int it = tid; it < DA_T * CH; it += nt) {
+    const int row = it / CH, col = 8 * (it % CH);
+    const int64_t at = s.at(row, col);
+    DaTile<NP, DP>::put_row(t, row, col, da_load8<NP>(src, at, at >= 0));
+  }
+}
+template <int NP, int DP, class SRC> __device__ __forceinline__ void da_stage_cols(uint16_t *t, const void *src, const SRC &s, int tid, int nt) {
+  constexpr int CH = 2 * DP / 4;
+  for (int it = tid; it < 8 * CH; it += nt) {
+    const int rg = it / CH, col = 4 * (it % CH);
+    Raw4<NP> r[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t at = s.at(4 * rg + j, col);
+      r[j] = da_load4<NP>(src, at, at >= 0);
+    }
+    DaTile<NP, DP>::put_col(t, rg, col, r);
+  }
+}
+
+// four consecutive outputs
+template <int NP> __device__ __forceinline__ void da_store4(void *base, int64_t at, float a, float b, float c, float d) {
+  if constexpr (NP == 3) {
+    *(float4 *)((float *)base + at) = make_float4(a, b, c, d);
+  } else if constexpr (NP == 2) {
+    *(uint2 *)((uint16_t *)base + at) = make_uint2(f16_pair(a, b), f16_pair(c, d));
+  } else {
+    *(uint2 *)((uint16_t *)base + at) = make_uint2(bf16_pair(a, b), bf16_pair(c, d));
+  }
+}
+
+__device__ __forceinline__ f32x16 da_zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) z[e] = 0.f;
+  return z;
+}
+__device__ __forceinline__ int da_wave_id() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
+
+// ---------------------------------------------------------------------------------------------------------------- forward
+// One workgroup: NW waves of 32 packed rows each over the keys [split chunk, ...) of one (cloud, key / value head).
+template <int NP, int DP, int NW, bool SPLIT>
+__global__ __launch_bounds__(64 * NW) void diff_attn_fwd_k(DaP p) {
+  using Tile = DaTile<NP, DP>;
+  constexpr int NR = DA_NR<NP>;
+  constexpr int NPP = NP == 3 ? 3 : 2;  // pieces of a probability
+  constexpr int KC = DP / 16, VB = 2 * DP / 32;
+  extern __shared__ __attribute__((aligned(16))) uint16_t da_lds[];
+  uint16_t *Ks = da_lds, *Vt = da_lds + Tile::ROWS;
+  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = da_wave_id(), tid = threadIdx.x;
+  const int b = blockIdx.x / p.Hkv, hk = blockIdx.x % p.Hkv, split = blockIdx.z;
+  const int tile = p.causal ? (int)(gridDim.y - 1 - blockIdx.y) : (int)blockIdx.y;  // causal: the longest rows first
+  const int row0 = (tile * NW + wave) * DA_T, r = row0 + col;
+  const int i = da_div_g(p, r), g = r - i * p.G, h = hk * p.G + g;
+  const bool valid = r < p.rows;
+  const int len = da_len(p, b), lim = da_limit(p, i, len);
+  const int lim_lo = da_limit(p, da_div_g(p, row0), len), lim_hi = da_limit(p, da_div_g(p, row0 + DA_T - 1), len);
+  const int last = da_limit(p, da_div_g(p, min(p.rows, (tile + 1) * NW * DA_T) - 1), len);
+  const int k0 = split * p.chunk, k1 = min(last, k0 + p.chunk);
+
+  bf16x8 qf[2][KC][NR];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      const int d = 16 * c + 8 * half;
+      uint4 w[NR];
+      da_pieces8<NP>(da_load8<NP>(p.q, b * p.q_b + i * p.q_n + h * p.q_h + m * p.q_m + d, valid && d < p.D), w);
+#pragma unroll
+      for (int k = 0; k < NR; ++k) qf[m][c][k] = as_bf16x8(w[k]);
+    }
+
+  f32x16 o[2][VB];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int v = 0; v < VB; ++v) o[m][v] = da_zero16();
+  float mx[2] = {-DA_INF, -DA_INF}, sum[2] = {0.f, 0.f};
+
+  DaKeys<DP> ks{b * p.k_b + hk * p.k_h, p.k_n, p.k_m, 0, len, p.D, true}, vs{b * p.v_b + hk * p.v_h, p.v_n, 0, 0, len, p.D, false};
+  for (int t = k0; t < k1; t += DA_T) {
+    __syncthreads();
+    ks.t = vs.t = t;
+    da_stage_rows<NP, DP>(Ks, p.k, ks, tid, 64 * NW);
+    da_stage_cols<NP, DP>(Vt, p.v, vs, tid, 64 * NW);
+    __syncthreads();
+    if (t >= lim_hi) continue;
+    float pr[2][16];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      f32x16 s = da_zero16();
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        bf16x8 a[NR];
+        Tile::frag_row(Ks, col, m * DP + 16 * c + 8 * half, a);
+        s = da_mfma_in<NP>(a, qf[m][c], s);
+      }
+      float top = -DA_INF;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) pr[m][e] = s[e] * p.scale2;
+      if (t + DA_T > lim_lo) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (t + 8 * (e >> 2) + 4 * half + (e & 3) >= lim) pr[m][e] = -DA_INF;
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, pr[m][e]);
+      top = fmaxf(top, __shfl_xor(top, 32, HITADV_WAVE));
+      if (__ballot(top > mx[m] + DA_SLACK) != 0ull) {  // (-inf + slack = -inf: the first visible key raises it)
+        const float nm = fmaxf(mx[m], top);
+        const float f = nm == -DA_INF ? 1.f : exp2_flush(mx[m] - nm);
+        sum[m] *= f;
+        mx[m] = nm;
+#pragma unroll
+        for (int v = 0; v < VB; ++v)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[m][v][e] *= f;
+      }
+      const float base = mx[m] == -DA_INF ? 0.f : mx[m];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        pr[m][e] = exp2_flush(pr[m][e] - base);
+        sum[m] += pr[m][e];
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      bf16x8 b1[NPP], b2[NPP];
+      da_operand<NPP>(&pr[0][8 * c], b1);
+      da_operand<NPP>(&pr[1][8 * c], b2);
+#pragma unroll
+      for (int v = 0; v < VB; ++v) {
+        bf16x8 a[NP];
+        Tile::frag_col(Vt, 32 * v + col, c, half, a);
+        o[0][v] = da_mfma<NP, NPP>(a, b1, o[0][v]);
+        o[1][v] = da_mfma<NP, NPP>(a, b2, o[1][v]);
+      }
+    }
+  }
+
+#pragma unroll
+  for (int m = 0; m < 2; ++m) sum[m] += __shfl_xor(sum[m], 32, HITADV_WAVE);
+  if (!valid) return;
+  if (SPLIT) {
+    const int64_t row = ((int64_t)split * p.B * p.Hkv + blockIdx.x) * p.rows + r;
+    if (half == 0) *(float4 *)(p.part_ml + 4 * row) = make_float4(mx[0], sum[0], mx[1], sum[1]);
+    float *po = p.part_o + row * 4 * p.D;
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int v = 0; v < VB; ++v)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const int d = 32 * v + 2 * e + 4 * half;
+          if (d < 2 * p.D) *(float4 *)(po + m * 2 * p.D + d) = make_float4(o[m][v][e], o[m][v][e + 1], o[m][v][e + 2], o[m][v][e + 3]);
+        }
+    return;
+  }
+  const float w1 = sum[0] == 0.f ? 0.f : 1.f / sum[0], w2 = sum[1] == 0.f ? 0.f : -da_lam(p, h) / sum[1];
+  const int64_t at = (((int64_t)b * p.Nq + i) * p.H + h) * 2 * p.D;
+#pragma unroll
+  for (int v = 0; v < VB; ++v)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const int d = 32 * v + 2 * e + 4 * half;
+      if (d >= 2 * p.D) continue;
+      float x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = o[0][v][e + j] * w1 + o[1][v][e + j] * w2;
+      da_store4<NP>(p.out, at + d, x[0], x[1], x[2], x[3]);
+    }
+  if (p.stats && half == 0) {
+    const int64_t n = (int64_t)p.B * p.H * p.Nq, row = ((int64_t)b * p.H + h) * p.Nq + i;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      p.stats[(2 * m) * n + row] = sum[m] == 0.f ? 0.f : mx[m];
+      p.stats[(2 * m + 1) * n + row] = sum[m] == 0.f ? DA_INF : log2f(sum[m]);  // an empty row: every probability 2^-inf = 0
+    }
+  }
+}
+
+// joins the splits of a row: thread = value column
+template <int NP>
+__global__ __launch_bounds__(128) void diff_attn_join_k(DaP p) {
+  const int r = blockIdx.x, bh = blockIdx.y, d = threadIdx.x;
+  const int b = bh / p.Hkv, hk = bh % p.Hkv, i = da_div_g(p, r), h = hk * p.G + r - i * p.G;
+  const int64_t step = (int64_t)p.B * p.Hkv * p.rows, row = (int64_t)bh * p.rows + r;
+  float mx[2] = {-DA_INF, -DA_INF};
+  for (int s = 0; s < p.splits; ++s) {
+    const float4 ml = *(const float4 *)(p.part_ml + 4 * (row + s * step));
+    mx[0] = fmaxf(mx[0], ml.x);
+    mx[1] = fmaxf(mx[1], ml.z);
+  }
+  const float b0 = mx[0] == -DA_INF ? 0.f : mx[0], b1 = mx[1] == -DA_INF ? 0.f : mx[1];
+  float sum[2] = {0.f, 0.f}, o[2] = {0.f, 0.f};
+  for (int s = 0; s < p.splits; ++s) {
+    const float4 ml = *(const float4 *)(p.part_ml + 4 * (row + s * step));
+    const float w0 = exp2_flush(ml.x - b0), w1 = exp2_flush(ml.z - b1);  // a split that saw nothing: 2^-inf = 0
+    sum[0] += ml.y * w0;
+    sum[1] += ml.w * w1;
+    if (d < 2 * p.D) {
+      const float *po = p.part_o + (row + s * step) * 4 * p.D;
+      o[0] += po[d] * w0;
+      o[1] += po[2 * p.D + d] * w1;
+    }
+  }
+  if (d < 2 * p.D) {
+    const float w0 = sum[0] == 0.f ? 0.f : 1.f / sum[0], w1 = sum[1] == 0.f ? 0.f : -da_lam(p, h) / sum[1];
+    const float x = o[0] * w0 + o[1] * w1;
+    const int64_t at = (((int64_t)b * p.Nq + i) * p.H + h) * 2 * p.D + d;
+    if constexpr (NP == 3) ((float *)p.out)[at] = x;
+    else if constexpr (NP == 2) ((_Float16 *)p.out)[at] = (_Float16)x;
+    else ((uint16_t *)p.out)[at] = (uint16_t)(bf16_pair(x, 0.f) & 0xffffu);
+  }
+  if (p.stats && d < 2) {
+    const int64_t n = (int64_t)p.B * p.H * p.Nq, srow = ((int64_t)b * p.H + h) * p.Nq + i;
+    p.stats[(2 * d) * n + srow] = sum[d] == 0.f ? 0.f : mx[d];
+    p.stats[(2 * d + 1) * n + srow] = sum[d] == 0.f ? DA_INF : log2f(sum[d]);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- backward
+// dP = dO V^T;  r_m = sum_j P_m dP;  dS_1 = P_1 (dP - r_1), dS_2 = -lam P_2 (dP - r_2).  The r are sums over the very P and dP that the
+// second pass multiplies (not dO . out: out is rounded, and where a row sees one key dS has to vanish exactly).
+//
+// dQ: the forward kernel's layout, two passes over the keys: first r, then dQ_m^T = K_m^T dS_m^T.
+template <int NP, int DP, int NW>
+__global__ __launch_bounds__(64 * NW) void diff_attn_dq_k(DaP p) {
+  using Tile = DaTile<NP, DP>;
+  constexpr int NR = DA_NR<NP>;
+  constexpr int NS = NP == 3 ? 3 : 2;  // pieces of dS
+  constexpr int KC = DP / 16, VC = 2 * DP / 16, DB = DP / 32;
+  extern __shared__ __attribute__((aligned(16))) uint16_t da_lds[];
+  uint16_t *Ks = da_lds, *Vs = da_lds + Tile::ROWS, *Kt = da_lds + 2 * Tile::ROWS;
+  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = da_wave_id(), tid = threadIdx.x;
+  const int b = blockIdx.x / p.Hkv, hk = blockIdx.x % p.Hkv;
+  const int tile = p.causal ? (int)(gridDim.y - 1 - blockIdx.y) : (int)blockIdx.y;
+  const int row0 = (tile * NW + wave) * DA_T, r = row0 + col;
+  const int i = da_div_g(p, r), g = r - i * p.G, h = hk * p.G + g;
+  const bool valid = r < p.rows;
+  const int len = da_len(p, b), lim = da_limit(p, i, len);
+  const int lim_lo = da_limit(p, da_div_g(p, row0), len), lim_hi = da_limit(p, da_div_g(p, row0 + DA_T - 1), len);
+  const int last = da_limit(p, da_div_g(p, min(p.rows, (tile + 1) * NW * DA_T) - 1), len);
+  const int64_t n = (int64_t)p.B * p.H * p.Nq, srow = ((int64_t)b * p.H + h) * p.Nq + i;
+
+  bf16x8 qf[2][KC][NR], gf[VC][NR];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      const int d = 16 * c + 8 * half;
+      uint4 w[NR];
+      da_pieces8<NP>(da_load8<NP>(p.q, b * p.q_b + i * p.q_n + h * p.q_h + m * p.q_m + d, valid && d < p.D), w);
+#pragma unroll
+      for (int k = 0; k < NR; ++k) qf[m][c][k] = as_bf16x8(w[k]);
+    }
+#pragma unroll
+  for (int c = 0; c < VC; ++c) {
+    const int d = 16 * c + 8 * half;
+    uint4 w[NR];
+    da_pieces8<NP>(da_load8<NP>(p.dout, (((int64_t)b * p.Nq + i) * p.H + h) * 2 * p.D + d, valid && d < 2 * p.D), w);
+#pragma unroll
+    for (int k = 0; k < NR; ++k) gf[c][k] = as_bf16x8(w[k]);
+  }
+  float mx[2], ll[2], rs[2] = {0.f, 0.f};
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    mx[m] = valid ? p.stats[(2 * m) * n + srow] : 0.f;
+    ll[m] = valid ? p.stats[(2 * m + 1) * n + srow] : DA_INF;
+  }
+  f32x16 acc[2][DB];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int v = 0; v < DB; ++v) acc[m][v] = da_zero16();
+
+  DaKeys<DP> ks{b * p.k_b + hk * p.k_h, p.k_n, p.k_m, 0, len, p.D, true}, vs{b * p.v_b + hk * p.v_h, p.v_n, 0, 0, len, p.D, false};
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll 1
+    for (int t = 0; t < last; t += DA_T) {
+      __syncthreads();
+      ks.t = vs.t = t;
+      da_stage_rows<NP, DP>(Ks, p.k, ks, tid, 64 * NW);
+      da_stage_rows<NP, DP>(Vs, p.v, vs, tid, 64 * NW);
+      if (pass) da_stage_cols<NP, DP>(Kt, p.k, ks, tid, 64 * NW);
+      __syncthreads();
+      if (t >= lim_hi) continue;
+      f32x16 dp = da_zero16();
+#pragma unroll
+      for (int c = 0; c < VC; ++c) {
+        bf16x8 a[NR];
+        Tile::frag_row(Vs, col, 16 * c + 8 * half, a);
+        dp = da_mfma_in<NP>(a, gf[c], dp);
+      }
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        f32x16 s = da_zero16();
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+          bf16x8 a[NR];
+          Tile::frag_row(Ks, col, m * DP + 16 * c + 8 * half, a);
+          s = da_mfma_in<NP>(a, qf[m][c], s);
+        }
+        float ds[16];
+        const bool edge = t + DA_T > lim_lo;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const bool seen = !edge || t + 8 * (e >> 2) + 4 * half + (e & 3) < lim;
+          ds[e] = seen ? exp2_flush((s[e] * p.scale2 - mx[m]) - ll[m]) : 0.f;
+        }
+        if (pass == 0) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) rs[m] += ds[e] == 0.f ? 0.f : ds[e] * dp[e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) ds[e] = ds[e] == 0.f ? 0.f : ds[e] * (dp[e] - rs[m]);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            bf16x8 bo[NS];
+            da_operand<NS>(&ds[8 * c], bo);
+#pragma unroll
+            for (int v = 0; v < DB; ++v) {
+              bf16x8 a[NP];
+              Tile::frag_col(Kt, m * DP + 32 * v + col, c, half, a);
+              acc[m][v] = da_mfma<NP, NS>(a, bo, acc[m][v]);
+            }
+          }
+        }
+      }
+    }
+    if (pass == 0) {
+#pragma unroll
+      for (int m = 0; m < 2; ++m) rs[m] += __shfl_xor(rs[m], 32, HITADV_WAVE);
+    }
+  }
+  if (!valid) return;
+  if (half == 0) {
+    p.r[srow] = rs[0];
+    p.r[n + srow] = rs[1];
+  }
+  const int64_t at = (((int64_t)b * p.Nq + i) * p.H + h) * 2 * p.D;
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    const float w = m == 0 ? p.scale : -da_lam(p, h) * p.scale;
+#pragma unroll
+    for (int v = 0; v < DB; ++v)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const int d = 32 * v + 2 * e + 4 * half;
+        if (d < p.D) da_store4<NP>(p.dq, at + m * p.D + d, acc[m][v][e] * w, acc[m][v][e + 1] * w, acc[m][v][e + 2] * w, acc[m][v][e + 3] * w);
+      }
+  }
+}
+
+// dK and dV: a wave owns 32 keys (the lane's column) and walks over the packed rows of all G heads, so that the sum over the heads that
+// share a key needs no atomics: dV^T += dO^T A, dK_m^T += Q_m^T dS_m, A = P_1 - lam P_2.
+template <int NP, int DP, int NW>
+__global__ __launch_bounds__(64 * NW) void diff_attn_dkv_k(DaP p) {
+  using Tile = DaTile<NP, DP>;
+  constexpr int NR = DA_NR<NP>;
+  constexpr int NS = NP == 3 ? 3 : 2;
+  constexpr int KC = DP / 16, VC = 2 * DP / 16, DB = DP / 32, VB = 2 * DP / 32;
+  extern __shared__ __attribute__((aligned(16))) uint16_t da_lds[];
+  uint16_t *Qs = da_lds, *Gs = Qs + Tile::ROWS, *Qt = Gs + Tile::ROWS, *Gt = Qt + Tile::COLS;
+  float *st = (float *)(Gt + Tile::COLS);  // [7][32]: max 1, log2 sum 1, max 2, log2 sum 2, r 1, r 2, lam
+  int *lims = (int *)(st + 7 * DA_T);
+  // three pieces at DP = 64 do not fit the register file beside the accumulators: the third piece of V (and of a little of K) is
+  // parked in LDS, read back by the lane that wrote it
+  constexpr bool PARK = NP == 3 && DP == 64;
+  uint4 *parked = (uint4 *)(lims + DA_T) + threadIdx.x;
+  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = da_wave_id(), tid = threadIdx.x;
+  const int b = blockIdx.x / p.Hkv, hk = blockIdx.x % p.Hkv;
+  const int first = blockIdx.y * NW * DA_T, key0 = first + wave * DA_T, key = key0 + col;
+  const int len = da_len(p, b);
+  const int64_t n = (int64_t)p.B * p.H * p.Nq;
+
+  bf16x8 kf[2][KC][NR], vf[VC][NR];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      const int d = 16 * c + 8 * half;
+      uint4 w[NR];
+      da_pieces8<NP>(da_load8<NP>(p.k, b * p.k_b + key * p.k_n + hk * p.k_h + m * p.k_m + d, key < len && d < p.D), w);
+#pragma unroll
+      for (int k = 0; k < NR; ++k) kf[m][c][k] = as_bf16x8(w[k]);
+      if (PARK && m == 0 && c < 2) parked[(VC + c) * 64 * NW] = w[NR - 1];
+    }
+#pragma unroll
+  for (int c = 0; c < VC; ++c) {
+    const int d = 16 * c + 8 * half;
+    uint4 w[NR];
+    da_pieces8<NP>(da_load8<NP>(p.v, b * p.v_b + key * p.v_n + hk * p.v_h + d, key < len && d < 2 * p.D), w);
+#pragma unroll
+    for (int k = 0; k < NR; ++k) vf[c][k] = as_bf16x8(w[k]);
+    if constexpr (PARK) parked[c * 64 * NW] = w[NR - 1];
+  }
+  f32x16 av[VB], ak[2][DB];
+#pragma unroll
+  for (int v = 0; v < VB; ++v) av[v] = da_zero16();
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int v = 0; v < DB; ++v) ak[m][v] = da_zero16();
+
+  // causal: query i sees key j when i >= j - (Nk - Nq): rows before that of the workgroup's first key have nothing here
+  int begin = p.causal ? max(0, first - (p.Nk - p.Nq)) : 0;
+  begin = first >= len ? p.rows : (int)min((int64_t)p.rows, (int64_t)begin * p.G) / DA_T * DA_T;
+  DaRows<DP> qs{b * p.q_b + hk * p.G * p.q_h, p.q_n, p.q_h, p.q_m, 0, p.rows, p.D, true, &p};
+  DaRows<DP> gs{((int64_t)b * p.Nq * p.H + hk * p.G) * 2 * p.D, (int64_t)p.H * 2 * p.D, 2 * p.D, 0, 0, p.rows, p.D, false, &p};
+#pragma unroll 1
+  for (int t = begin; t < p.rows; t += DA_T) {
+    __syncthreads();
+    qs.t = gs.t = t;
+    da_stage_rows<NP, DP>(Qs, p.q, qs, tid, 64 * NW);
+    if (NP == 3) __builtin_amdgcn_sched_barrier(0);
+    da_stage_rows<NP, DP>(Gs, p.dout, gs, tid, 64 * NW);
+    if (NP == 3) __builtin_amdgcn_sched_barrier(0);
+    da_stage_cols<NP, DP>(Qt, p.q, qs, tid, 64 * NW);
+    if (NP == 3) __builtin_amdgcn_sched_barrier(0);
+    da_stage_cols<NP, DP>(Gt, p.dout, gs, tid, 64 * NW);
+    if (tid < DA_T) {
+      const int r = t + tid, i = da_div_g(p, r), h = hk * p.G + r - i * p.G;
+      const bool ok = r < p.rows;
+      const int64_t srow = ((int64_t)b * p.H + h) * p.Nq + i;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) st[k * DA_T + tid] = ok ? p.stats[k * n + srow] : (k & 1) ? DA_INF : 0.f;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) st[(4 + k) * DA_T + tid] = ok ? p.r[k * n + srow] : 0.f;
+      st[6 * DA_T + tid] = ok ? da_lam(p, h) : 0.f;
+      lims[tid] = ok ? da_limit(p, i, len) : 0;
+    }
+    __syncthreads();
+    f32x16 dp = da_zero16();
+#pragma unroll
+    for (int c = 0; c < VC; ++c) {
+      bf16x8 a[NR];
+      Tile::frag_row(Gs, col, 16 * c + 8 * half, a);
+      if constexpr (PARK) {
+        bf16x8 w[NR];
+#pragma unroll
+        for (int k = 0; k < NR; ++k) w[k] = k == NR - 1 ? as_bf16x8(parked[c * 64 * NW]) : vf[c][k];
+        dp = da_mfma_in<NP>(a, w, dp);
+      } else {
+        dp = da_mfma_in<NP>(a, vf[c], dp);
+      }
+      if (NP == 3) __builtin_amdgcn_sched_barrier(0);  // (without it the fragments of several products are fetched ahead and spill)
+    }
+    float A[16];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      f32x16 s = da_zero16();
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        bf16x8 a[NR];
+        Tile::frag_row(Qs, col, m * DP + 16 * c + 8 * half, a);
+        if (PARK && m == 0 && c < 2) {
+          bf16x8 w[NR];
+#pragma unroll
+          for (int k = 0; k < NR; ++k) w[k] = k == NR - 1 ? as_bf16x8(parked[(VC + c) * 64 * NW]) : kf[m][c][k];
+          s = da_mfma_in<NP>(a, w, s);
+        } else {
+          s = da_mfma_in<NP>(a, kf[m][c], s);
+        }
+        if (NP == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+      float ds[16];
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const int row = 2 * e + 4 * half;  // rows row .. row + 3 in registers e .. e + 3
+        const float4 mx = *(const float4 *)(st + (2 * m) * DA_T + row), ll = *(const float4 *)(st + (2 * m + 1) * DA_T + row);
+        const float4 rr = *(const float4 *)(st + (4 + m) * DA_T + row), lam = *(const float4 *)(st + 6 * DA_T + row);
+        const int4 li = *(const int4 *)(lims + row);
+        const float mxs[4] = {mx.x, mx.y, mx.z, mx.w}, lls[4] = {ll.x, ll.y, ll.z, ll.w}, rrs[4] = {rr.x, rr.y, rr.z, rr.w};
+        const float las[4] = {lam.x, lam.y, lam.z, lam.w};
+        const int lis[4] = {li.x, li.y, li.z, li.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float pm = key < lis[j] ? exp2_flush((s[e + j] * p.scale2 - mxs[j]) - lls[j]) : 0.f;
+          const float d = pm == 0.f ? 0.f : pm * (dp[e + j] - rrs[j]);
+          if (m == 0) A[e + j] = pm;
+          else A[e + j] = A[e + j] - las[j] * pm;
+          ds[e + j] = m == 0 ? d : -las[j] * d;
+        }
+        if (NP == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        bf16x8 bo[NS];
+        da_operand<NS>(&ds[8 * c], bo);
+#pragma unroll
+        for (int v = 0; v < DB; ++v) {
+          bf16x8 a[NP];
+          Tile::frag_col(Qt, m * DP + 32 * v + col, c, half, a);
+          ak[m][v] = da_mfma<NP, NS>(a, bo, ak[m][v]);
+          if (NP == 3) __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      bf16x8 bo[NS];
+      da_operand<NS>(&A[8 * c], bo);
+#pragma unroll
+      for (int v = 0; v < VB; ++v) {
+        bf16x8 a[NP];
+        Tile::frag_col(Gt, 32 * v + col, c, half, a);
+        av[v] = da_mfma<NP, NS>(a, bo, av[v]);
+        if (NP == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+  if (key >= p.Nk) return;
+  const int64_t at = (((int64_t)b * p.Nk + key) * p.Hkv + hk) * 2 * p.D;
+#pragma unroll
+  for (int v = 0; v < VB; ++v)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const int d = 32 * v + 2 * e + 4 * half;
+      if (d < 2 * p.D) da_store4<NP>(p.dv, at + d, av[v][e], av[v][e + 1], av[v][e + 2], av[v][e + 3]);
+    }
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int v = 0; v < DB; ++v)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const int d = 32 * v + 2 * e + 4 * half;
+        if (d < p.D)
+          da_store4<NP>(p.dk, at + m * p.D + d, ak[m][v][e] * p.scale, ak[m][v][e + 1] * p.scale, ak[m][v][e + 2] * p.scale,
+                        ak[m][v][e + 3] * p.scale);
+      }
+}
+
+// dlam[h] = -sum over clouds and queries of r_2 (one value for all heads: over the heads too); one workgroup per output, fixed order,
+// sums in double (a long sum of values of both signs)
+__global__ __launch_bounds__(256) void diff_attn_dlam_k(const float *__restrict__ r2, int B, int H, int Nq, int lam_n, float *__restrict__ dlam) {
+  __shared__ double part[4];
+  double s = 0.0;
+  const int h0 = lam_n == 1 ? 0 : blockIdx.x, h1 = lam_n == 1 ? H : h0 + 1;
+  for (int b = 0; b < B; ++b)
+    for (int h = h0; h < h1; ++h)
+      for (int i = threadIdx.x; i < Nq; i += 256) s += (double)r2[((int64_t)b * H + h) * Nq + i];
+  for (int m = 32; m >= 1; m >>= 1) s += __shfl_xor(s, m, HITADV_WAVE);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) dlam[blockIdx.x] = (float)-(((part[0] + part[1]) + part[2]) + part[3]);
+}
+
+// ---------------------------------------------------------------------------------------------------------------- host
+struct DaPlan {
+  int nw, tiles, splits, chunk;
+};
+// Few rows: workgroups of one wave and the keys split over enough of them to fill the chip; else four waves share a tile of keys.
+static DaPlan da_plan(int B, int Nq, int Nk, int H, int Hkv) {
+  DaPlan pl;
+  const int64_t rows = (int64_t)Nq * (H / Hkv), bh = (int64_t)B * Hkv;
+  pl.nw = rows <= 2 * DA_T ? 1 : 4;
+  pl.tiles = (int)((rows + DA_T * pl.nw - 1) / (DA_T * pl.nw));
+  const int64_t waves = bh * pl.tiles * pl.nw, want = (2048 + waves - 1) / waves, most = (Nk + 127) / 128;
+  int64_t s = waves >= 1024 ? 1 : want < most ? want : most;
+  if (s < 1) s = 1;
+  int64_t chunk = ((Nk + s - 1) / s + DA_T - 1) / DA_T * DA_T;
+  if (chunk < DA_T) chunk = DA_T;
+  pl.chunk = (int)chunk;
+  pl.splits = (int)((Nk + chunk - 1) / chunk);
+  if (pl.splits < 1) pl.splits = 1;
+  return pl;
+}
+
+template <int NP, int DP> static int da_launch_fwd(const DaP &p, const DaPlan &pl, hipStream_t s) {
+  const int lds = 2 * (DaTile<NP, DP>::ROWS + DaTile<NP, DP>::COLS);
+  const dim3 grid(p.B * p.Hkv, pl.tiles, pl.splits);
+  if (pl.nw == 1 && pl.splits > 1) {
+    HITADV_RAISE_LDS((diff_attn_fwd_k<NP, DP, 1, true>), lds);
+    diff_attn_fwd_k<NP, DP, 1, true><<<grid, 64, lds, s>>>(p);
+  } else if (pl.nw == 1) {
+    HITADV_RAISE_LDS((diff_attn_fwd_k<NP, DP, 1, false>), lds);
+    diff_attn_fwd_k<NP, DP, 1, false><<<grid, 64, lds, s>>>(p);
+  } else if (pl.splits > 1) {
+    HITADV_RAISE_LDS((diff_attn_fwd_k<NP, DP, 4, true>), lds);
+    diff_attn_fwd_k<NP, DP, 4, true><<<grid, 256, lds, s>>>(p);
+  } else {
+    HITADV_RAISE_LDS((diff_attn_fwd_k<NP, DP, 4, false>), lds);
+    diff_attn_fwd_k<NP, DP, 4, false><<<grid, 256, lds, s>>>(p);
+  }
+  HITADV_LAUNCH_CHECK();
+  if (pl.splits > 1) {
+    diff_attn_join_k<NP><<<dim3(p.rows, p.B * p.Hkv), 128, 0, s>>>(p);
+    HITADV_LAUNCH_CHECK();
+  }
+  return 0;
+}
+template <int NP, int DP> static int da_launch_bwd(const DaP &p, float *dlam, hipStream_t s) {
+  const int lds_q = 2 * (2 * DaTile<NP, DP>::ROWS + DaTile<NP, DP>::COLS);
+  const int lds_kv = 2 * (2 * DaTile<NP, DP>::ROWS + 2 * DaTile<NP, DP>::COLS) + 8 * DA_T * 4 + (NP == 3 && DP == 64 ? (2 * DP / 16 + 2) * 256 * 16 : 0);
+  const int tq = (p.rows + 4 * DA_T - 1) / (4 * DA_T), tk = (p.Nk + 4 * DA_T - 1) / (4 * DA_T);
+  HITADV_RAISE_LDS((diff_attn_dq_k<NP, DP, 4>), lds_q);
+  diff_attn_dq_k<NP, DP, 4><<<dim3(p.B * p.Hkv, tq), 256, lds_q, s>>>(p);
+  HITADV_LAUNCH_CHECK();
+  if (p.dk) {
+    HITADV_RAISE_LDS((diff_attn_dkv_k<NP, DP, 4>), lds_kv);
+    diff_attn_dkv_k<NP, DP, 4><<<dim3(p.B * p.Hkv, tk), 256, lds_kv, s>>>(p);
+    HITADV_LAUNCH_CHECK();
+  }
+  if (dlam) {
+    diff_attn_dlam_k<<<p.lam_n, 256, 0, s>>>(p.r + (int64_t)p.B * p.H * p.Nq, p.B, p.H, p.Nq, p.lam_n, dlam);
+    HITADV_LAUNCH_CHECK();
+  }
+  return 0;
+}
+
+static bool da_shape_ok(int dtype, int64_t B, int64_t Nq, int64_t Nk, int64_t H, int64_t Hkv, int64_t D) {
+  if (dtype < 0 || dtype > 2 || B < 1 || Nq < 1 || Nk < 1 || H < 1 || Hkv < 1 || H % Hkv || D < 8 || D > 64 || D % 8) return false;
+  const int64_t G = H / Hkv, rows = Nq * G;
+  // rows and keys are 32-bit indexes (with room for a tile beyond the end), the division by G is exact below 2^32 / G, and the grid's
+  // second and third extents are 16-bit
+  return rows <= 2000000 && (rows + 256) * G < (1ll << 32) && Nk <= 2000000 && B * Hkv < (1ll << 31) && B * Hkv <= 65535 &&
+         B * H * Nq < (1ll << 40);
+}
+static void da_fill(DaP &p, int B, int Nq, int Nk, int H, int Hkv, int D, int lam_n, int causal, float scale, const int64_t *st) {
+  p.B = B; p.Nq = Nq; p.Nk = Nk; p.H = H; p.Hkv = Hkv; p.D = D; p.G = H / Hkv; p.lam_n = lam_n; p.causal = causal;
+  p.rows = Nq * p.G;
+  p.g_magic = p.G > 1 ? (uint32_t)(((1ull << 32) + p.G - 1) / p.G) : 0u;
+  p.scale = scale;
+  p.scale2 = scale * DA_LOG2E;
+  p.q_b = st[0]; p.q_n = st[1]; p.q_h = st[2]; p.q_m = st[3];
+  p.k_b = st[4]; p.k_n = st[5]; p.k_h = st[6]; p.k_m = st[7];
+  p.v_b = st[8]; p.v_n = st[9]; p.v_h = st[10];
+}
+static bool da_strides_ok(int dtype, const void *q, const void *k, const void *v, const int64_t *st) {
+  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & 15) return false;
+  for (int i = 0; i < 11; ++i)
+    if (st[i] < 0 || st[i] % (dtype == 0 ? 4 : 8)) return false;
+  return true;
+}
+
+}  // namespace hitadv
+
+using namespace hitadv;
+
+extern "C" int hitadv_diff_attention_supported(int dtype, int64_t B, int64_t Nq, int64_t Nk, int64_t H, int64_t Hkv, int64_t D) {
+  return da_shape_ok(dtype, B, Nq, Nk, H, Hkv, D) ? 1 : 0;
+}
+
+extern "C" int64_t hitadv_diff_attention_scratch_floats(int B, int Nq, int Nk, int H, int Hkv, int D) {
+  if (!da_shape_ok(0, B, Nq, Nk, H, Hkv, D)) return 0;
+  const DaPlan pl = da_plan(B, Nq, Nk, H, Hkv);
+  return pl.splits > 1 ? (int64_t)pl.splits * B * H * Nq * (4 * D + 4) : 0;
+}
+
+extern "C" int hitadv_diff_attention_fwd(int dtype, const void *q, const void *k, const void *v, const float *lam, int lam_n, const int32_t *lengths,
+                                         const int64_t *strides, int B, int Nq, int Nk, int H, int Hkv, int D, int causal, float scale, void *out,
+                                         float *stats, float *scratch, void *stream) {
+  if (!q || !k || !v || !lam || !strides || !out || !da_shape_ok(dtype, B, Nq, Nk, H, Hkv, D) || (lam_n != 1 && lam_n != H) ||
+      !da_strides_ok(dtype, q, k, v, strides) || ((uintptr_t)out & 15))
+    return HITADV_E_ARG;
+  DaP p = {};
+  da_fill(p, B, Nq, Nk, H, Hkv, D, lam_n, causal != 0, scale, strides);
+  const DaPlan pl = da_plan(B, Nq, Nk, H, Hkv);
+  if (pl.splits > 1 && (!scratch || ((uintptr_t)scratch & 15))) return HITADV_E_ARG;
+  p.q = q; p.k = k; p.v = v; p.lam = lam; p.lengths = lengths; p.out = out; p.stats = stats;
+  p.chunk = pl.chunk;
+  p.splits = pl.splits;
+  p.part_ml = scratch;
+  p.part_o = scratch ? scratch + (int64_t)pl.splits * B * H * Nq * 4 : nullptr;
+  hipStream_t s = (hipStream_t)stream;
+  if (D <= 32) return dtype == 0 ? da_launch_fwd<3, 32>(p, pl, s) : dtype == 1 ? da_launch_fwd<1, 32>(p, pl, s) : da_launch_fwd<2, 32>(p, pl, s);
+  return dtype == 0 ? da_launch_fwd<3, 64>(p, pl, s) : dtype == 1 ? da_launch_fwd<1, 64>(p, pl, s) : da_launch_fwd<2, 64>(p, pl, s);
+}
+
+extern "C" int hitadv_diff_attention_bwd(int dtype, const void *q, const void *k, const void *v, const float *lam, int lam_n, const int32_t *lengths,
+                                         const int64_t *strides, const void *dout, const float *stats, int B, int Nq, int Nk, int H, int Hkv, int D,
+                                         int causal, float scale, float *r, void *dq, void *dk, void *dv, float *dlam, void *stream) {
+  if (!q || !k || !v || !lam || !strides || !dout || !stats || !r || !dq || !dk != !dv || !da_shape_ok(dtype, B, Nq, Nk, H, Hkv, D) ||
+      (lam_n != 1 && lam_n != H) || !da_strides_ok(dtype, q, k, v, strides) ||
+      (((uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15))
+    return HITADV_E_ARG;
+  DaP p = {};
+  da_fill(p, B, Nq, Nk, H, Hkv, D, lam_n, causal != 0, scale, strides);
+  p.q = q; p.k = k; p.v = v; p.lam = lam; p.lengths = lengths; p.dout = dout; p.stats = const_cast<float *>(stats); p.r = r;
+  p.dq = dq; p.dk = dk; p.dv = dv;
+  hipStream_t s = (hipStream_t)stream;
+  if (D <= 32) return dtype == 0 ? da_launch_bwd<3, 32>(p, dlam, s) : dtype == 1 ? da_launch_bwd<1, 32>(p, dlam, s) : da_launch_bwd<2, 32>(p, dlam, s);
+  return dtype == 0 ? da_launch_bwd<3, 64>(p, dlam, s) : dtype == 1 ? da_launch_bwd<1, 64>(p, dlam, s) : da_launch_bwd<2, 64>(p, dlam, s);
+}

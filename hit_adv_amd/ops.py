@@ -1152,6 +1152,269 @@ def offset_attention_layer(x, Wq, Wv, bv, Wt, bt):
     return OffsetAttentionLayer.apply(x, Wq, Wv, bv, Wt, bt)
 
 
+# --------------------------------------------------------------------------- a set transformer's block
+_DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # include/hitadv.h HITADV_DTYPE_*
+
+
+def _call_on(t, name, *args):
+    """``_lib.call`` with the current stream of ``t``'s device as the last argument, on that device."""
+    if t.device.index != torch.cuda.current_device():
+        with torch.cuda.device(t.device):
+            _lib.call(name, *args, _stream())
+    else:
+        _lib.call(name, *args, _stream())
+
+
+def _typed(t, name, like=None, dtypes=_DTYPE_CODE):
+    """A GPU tensor of one of ``dtypes`` on the device of ``like``, as it is (no cast: the type says how outputs are rounded)."""
+    if not torch.is_tensor(t):
+        raise TypeError("%s must be a tensor" % name)
+    if not t.is_cuda:
+        raise RuntimeError("%s must live on the GPU: hit_adv_amd has no CPU path" % name)
+    if t.dtype not in dtypes:
+        raise TypeError("%s must be one of %s, got %s" % (name, ", ".join(str(d) for d in dtypes), t.dtype))
+    if like is not None and t.device != like.device:
+        raise RuntimeError("%s is on %s, not on %s" % (name, t.device, like.device))
+    return t
+
+
+def _aligned(t):
+    """``t`` contiguous with a 16-byte aligned first element."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _strided(t):
+    """(``t`` or a contiguous copy, its strides): last axis contiguous, 16-byte aligned rows -- views of a cache are taken as they are."""
+    unit = 16 // t.element_size()
+    strides = [0 if n == 1 else s for n, s in zip(t.shape, t.stride())]
+    if (t.stride(-1) != 1 and t.shape[-1] != 1) or t.data_ptr() % 16 or any(s % unit for s in strides[:-1]):
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+        strides = list(t.stride())
+    return t, strides[:-1]
+
+
+class DiffAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lam, scale, causal, lengths, keep):
+        B, Nq, H, _, D = q.shape
+        Nk, Hkv = k.shape[1], k.shape[2]
+        out = torch.empty(B, Nq, H, 2 * D, device=q.device, dtype=q.dtype)
+        ctx.empty = out.numel() == 0 or Nk == 0
+        stats = None
+        if ctx.empty:
+            out.zero_()
+        else:
+            q, qs = _strided(q)
+            k, ks = _strided(k)
+            v, vs = _strided(v)
+            ctx.strides = (ctypes.c_int64 * 11)(*qs, *ks, *vs)
+            if keep:
+                stats = torch.empty(4, B, H, Nq, device=q.device)
+            n = _lib.load().hitadv_diff_attention_scratch_floats(B, Nq, Nk, H, Hkv, D)
+            scratch = torch.empty(n, device=q.device) if n else None
+            lam32 = lam.contiguous()
+            _call_on(q, "hitadv_diff_attention_fwd", _DTYPE_CODE[q.dtype], _p(q), _p(k), _p(v), _p(lam32), lam.numel(), _p(lengths), ctx.strides,
+                     B, Nq, Nk, H, Hkv, D, int(causal), ctypes.c_float(scale), _p(out), _p(stats), _p(scratch))
+        if keep:
+            ctx.save_for_backward(q, k, v, lam, lengths, stats)
+            ctx.scale, ctx.causal = scale, causal
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        q, k, v, lam, lengths, stats = ctx.saved_tensors
+        B, Nq, H, _, D = q.shape
+        Nk, Hkv = k.shape[1], k.shape[2]
+        need = ctx.needs_input_grad
+        if ctx.empty:
+            return tuple(torch.zeros_like(t) if need[i] else None for i, t in enumerate((q, k, v, lam))) + (None,) * 4
+        g = _aligned(g)
+        r = torch.empty(2, B, H, Nq, device=q.device)
+        dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        dk = dv = dlam = None
+        if need[1] or need[2]:
+            dk, dv = torch.empty(k.shape, device=q.device, dtype=q.dtype), torch.empty(v.shape, device=q.device, dtype=q.dtype)
+        if need[3]:
+            dlam = torch.empty(lam.shape, device=q.device)
+        _call_on(q, "hitadv_diff_attention_bwd", _DTYPE_CODE[q.dtype], _p(q), _p(k), _p(v), _p(lam.contiguous()), lam.numel(), _p(lengths),
+                 ctx.strides, _p(g), _p(stats), B, Nq, Nk, H, Hkv, D, int(ctx.causal), ctypes.c_float(ctx.scale), _p(r), _p(dq), _p(dk), _p(dv),
+                 _p(dlam))
+        return dq, dk, dv, dlam, None, None, None, None
+
+
+def diff_attention(q, k, v, lam, scale=None, causal=False, key_lengths=None):
+    """Differential attention: ``(softmax(scale q1 k1^T) - lam softmax(scale q2 k2^T)) v``, differentiable in q, k, v and lam.
+
+    q [B,Nq,H,2,D], k [B,Nk,Hkv,2,D], v [B,Nk,Hkv,2D] of one type (fp32, bf16, fp16), H a multiple of Hkv (query head h reads key / value
+    head h // (H // Hkv)), D a multiple of 8 up to 64; lam fp32, [H] or one value for all heads -> [B,Nq,H,2D] of that type.  ``scale``
+    defaults to D ** -0.5.  ``causal``: query i sees the keys j <= i + Nk - Nq, so that a few new queries stand at the end of a cache.
+    ``key_lengths`` [B] int: only the keys below it (clamped to 0 .. Nk) exist; what lies behind it may hold anything.  A row that sees no key
+    is 0 and has no gradient.  Values that are visible to some row must be finite: a row that sees one that is not is NaN, and so may be
+    rows of the same tile from which only ``causal`` hides it.  Views whose last axis is contiguous and whose rows start at multiples of 16
+    bytes (a slice of a cache) are read where they are, others are copied.  Same bits on every run; no second derivative."""
+    _typed(q, "q")
+    for t, name in ((k, "k"), (v, "v")):
+        _typed(t, name, q)
+        if t.dtype != q.dtype:
+            raise TypeError("diff_attention: %s is %s, q is %s" % (name, t.dtype, q.dtype))
+    if q.dim() != 5 or k.dim() != 5 or v.dim() != 4 or q.shape[3] != 2 or k.shape[3] != 2:
+        raise ValueError("diff_attention: need q [B,Nq,H,2,D], k [B,Nk,Hkv,2,D], v [B,Nk,Hkv,2D], got %s, %s, %s"
+                         % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    B, Nq, H, _, D = q.shape
+    Nk, Hkv = k.shape[1], k.shape[2]
+    if k.shape[0] != B or k.shape[4] != D or tuple(v.shape) != (B, Nk, Hkv, 2 * D) or Hkv == 0 or H == 0 or H % Hkv:
+        raise ValueError("diff_attention: q %s does not fit k %s and v %s" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    _typed(lam, "lam", q, (torch.float32,))
+    if lam.dim() > 1 or lam.numel() not in (1, H):
+        raise ValueError("diff_attention: lam is one value or [H=%d], got %s" % (H, tuple(lam.shape)))
+    if key_lengths is not None:
+        _typed(key_lengths, "key_lengths", q, (torch.int32, torch.int64))
+        if tuple(key_lengths.shape) != (B,):
+            raise ValueError("diff_attention: key_lengths is [B=%d], got %s" % (B, tuple(key_lengths.shape)))
+        key_lengths = key_lengths.clamp(0, Nk).to(torch.int32) if key_lengths.dtype == torch.int64 else key_lengths.contiguous()
+    if B and Nq and Nk and not _lib.load().hitadv_diff_attention_supported(_DTYPE_CODE[q.dtype], B, Nq, Nk, H, Hkv, D):
+        raise ValueError("diff_attention: D=%d must be a multiple of 8 up to 64, Nq * H / Hkv and Nk at most 2,000,000 and B * Hkv at most 65535 "
+                         "(q %s, k %s)" % (D, tuple(q.shape), tuple(k.shape)))
+    scale = float(D) ** -0.5 if scale is None else float(scale)
+    keep = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or lam.requires_grad)
+    return DiffAttention.apply(q, k, v, lam, scale, bool(causal), key_lengths, keep)
+
+
+RMS_NORM_MAX_COLS = 16384
+
+
+class RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, eps, residual, keep):
+        x, weight = x.contiguous(), weight.contiguous()
+        C = x.shape[-1]
+        rows = x.numel() // C
+        y = torch.empty_like(x)
+        total = torch.empty_like(x) if residual is not None else None
+        rstd = torch.empty(rows, device=x.device) if keep else None
+        if rows:
+            _call_on(x, "hitadv_rms_norm_fwd", _DTYPE_CODE[x.dtype], _DTYPE_CODE[weight.dtype], _p(x),
+                     _p(residual.contiguous() if residual is not None else None), _p(weight), rows, C, ctypes.c_float(eps), _p(y), _p(total), _p(rstd))
+        if keep:
+            ctx.set_materialize_grads(False)
+            ctx.save_for_backward(x if residual is None else total, weight, rstd)
+        return y if residual is None else (y, total)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dsum=None):
+        s, weight, rstd = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        if dy is None:
+            return dsum if need[0] else None, None, None, dsum if need[3] else None, None
+        C = s.shape[-1]
+        rows = s.numel() // C
+        dx = torch.empty_like(s)
+        dw = scratch = None
+        if need[1]:
+            dw = torch.empty_like(weight)
+            scratch = torch.empty(_lib.load().hitadv_rms_norm_bwd_scratch_floats(rows, C), device=s.device)
+        if rows:
+            _call_on(s, "hitadv_rms_norm_bwd", _DTYPE_CODE[s.dtype], _DTYPE_CODE[weight.dtype], _p(s), _p(weight), _p(rstd), _p(dy.contiguous()),
+                     _p(dsum.contiguous() if dsum is not None else None), rows, C, _p(dx), _p(scratch), _p(dw))
+        elif dw is not None:
+            dw.zero_()
+        return dx if need[0] else None, dw, None, dx if need[3] else None, None
+
+
+def _rms_args(name, x, weight, residual):
+    _typed(x, "x")
+    _typed(weight, "weight", x)
+    if x.dim() < 1 or weight.dim() != 1 or weight.shape[0] != x.shape[-1]:
+        raise ValueError("%s: weight %s does not fit the last axis of x %s" % (name, tuple(weight.shape), tuple(x.shape)))
+    if weight.dtype not in (x.dtype, torch.float32):
+        raise TypeError("%s: weight must be float32 or x's type %s, got %s" % (name, x.dtype, weight.dtype))
+    if not 1 <= x.shape[-1] <= RMS_NORM_MAX_COLS:
+        raise ValueError("%s: the last axis must be 1 to %d long, got %d" % (name, RMS_NORM_MAX_COLS, x.shape[-1]))
+    if residual is not None:
+        _typed(residual, "residual", x)
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise ValueError("%s: residual %s %s does not fit x %s %s" % (name, tuple(residual.shape), residual.dtype, tuple(x.shape), x.dtype))
+    if x.numel() // x.shape[-1] >= 2 ** 31:
+        raise ValueError("%s: at most 2^31 - 1 rows" % name)
+
+
+def rms_norm(x, weight, eps=1e-6, residual=None):
+    """Root-mean-square norm of x's last axis: ``y = s / sqrt(mean(s^2) + eps) * weight`` with ``s = x``, or ``s = x + residual`` rounded to
+    x's type.  x fp32, bf16 or fp16, last axis 1 to 16384; weight [C] fp32 or x's type -> y, or (y, s) with a residual.  Differentiable in
+    x, weight and residual (s included); sums in fp32, the same bits on every run; no second derivative."""
+    _rms_args("rms_norm", x, weight, residual)
+    keep = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad))
+    return RmsNorm.apply(x, weight, float(eps), residual, keep)
+
+
+def rms_norm_quant(x, weight, eps=1e-6, residual=None):
+    """``rms_norm`` with an 8-bit output and a scale per row: -> (q float8_e4m3fn, scale fp32 [...]) with y ~ q scale, scale = max |y| / 448
+    (1 for a row of zeros), and s behind them if there is a residual.  For serving: no gradient."""
+    _rms_args("rms_norm_quant", x, weight, residual)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
+        raise RuntimeError("rms_norm_quant has no backward pass: call it under torch.no_grad(), or rms_norm")
+    x, weight = x.contiguous(), weight.contiguous()
+    C = x.shape[-1]
+    rows = x.numel() // C
+    q = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
+    scale = torch.empty(x.shape[:-1], device=x.device)
+    total = torch.empty_like(x) if residual is not None else None
+    if rows:
+        _call_on(x, "hitadv_rms_norm_e4m3", _DTYPE_CODE[x.dtype], _DTYPE_CODE[weight.dtype], _p(x),
+                 _p(residual.contiguous() if residual is not None else None), _p(weight), rows, C, ctypes.c_float(float(eps)), _p(q), _p(scale),
+                 _p(total))
+    return (q, scale) if residual is None else (q, scale, total)
+
+
+def _dropout_raw(x, residual, p, rng):
+    y = torch.empty_like(x)
+    if x.numel():
+        _call_on(x, "hitadv_dropout", _DTYPE_CODE[x.dtype], _p(x), _p(residual), _p(y), x.numel(), _p(rng), int(round(p * 2 ** 32)),
+                 ctypes.c_float(1.0 / (1.0 - p) if p < 1.0 else 0.0))
+    return y
+
+
+class Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, rng, residual):
+        ctx.p = p
+        ctx.save_for_backward(rng)
+        return _dropout_raw(x.contiguous(), residual.contiguous() if residual is not None else None, p, rng)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        rng, = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        return _dropout_raw(g.contiguous(), None, ctx.p, rng) if need[0] else None, None, None, g if need[3] else None
+
+
+def dropout(x, p, rng, residual=None):
+    """``y = keep x / (1 - p)``, plus ``residual`` if given: element i (in contiguous order) is kept where word i % 4 of Philox4x32-10 with the
+    counter (i / 4, offset) and the key seed is at least p 2^32.  x fp32, bf16 or fp16 of any shape; ``rng`` = int64 tensor [seed, offset] on
+    x's device: read when the kernel runs, so a captured call follows a new offset.  The mask is not stored -- the backward pass makes it again
+    from ``rng``, which must not be changed in place in between (autograd refuses that).  Differentiable in x and residual."""
+    _typed(x, "x")
+    _typed(rng, "rng", x, (torch.int64,))
+    if tuple(rng.shape) != (2,):
+        raise ValueError("dropout: rng is an int64 tensor [seed, offset], got %s" % (tuple(rng.shape),))
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError("dropout: p must be in [0, 1], got %g" % p)
+    if residual is not None:
+        _typed(residual, "residual", x)
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise ValueError("dropout: residual %s %s does not fit x %s %s" % (tuple(residual.shape), residual.dtype, tuple(x.shape), x.dtype))
+    if x.numel() > 2 ** 40:
+        raise ValueError("dropout: at most 2^40 elements")
+    return Dropout.apply(x, p, rng.contiguous(), residual)
+
+
 def gemm_f16x2_supported(N, K):
     """Whether ``gemm_f16x2`` / ``linear_lrelu_pool`` are built for N output columns over a K-deep contraction."""
     return bool(_lib.load().hitadv_gemm_f16x2_supported(int(N), int(K)))

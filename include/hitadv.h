@@ -667,6 +667,53 @@ int hitadv_knn_features(const float *X, const float *xx, int B, int N, int D, in
  * bits every run): the squared norms hitadv_knn_features takes.  Host-side helper of model/dgcnn_cls.py:9 (`xx = torch.sum(x ** 2, ...)`). */
 int hitadv_row_sqnorm(const float *X, int64_t rows, int D, float *xx, void *stream);
 
+/* ------------------------------------------------------------------ a set transformer's block
+ * Element types of the three operators below: fp32, bf16, fp16. */
+#define HITADV_DTYPE_F32 0
+#define HITADV_DTYPE_BF16 1
+#define HITADV_DTYPE_F16 2
+
+/* Differential attention: out[b,i,h] = sum_j (P1 - lam[h] P2)[i,j] v[b,j,h / G], P_m = softmax over the visible j of
+ * scale q[b,i,h,m] . k[b,j,h / G,m], m = 1, 2; G = H / Hkv query heads share a key / value head.
+ *   q [B,Nq,H,2,D], k [B,Nk,Hkv,2,D], v [B,Nk,Hkv,2D] in dtype, any strides (elements, HOST array `strides`: q's for b, query, head, map;
+ *   k's for b, key, head, map; v's for b, key, head), the last axis contiguous, bases 16-byte aligned, strides multiples of 16 bytes;
+ *   lam fp32 [H], or one value for all heads (lam_n = H or 1); lengths int32 [B] or NULL (device): key j is visible below lengths[b]
+ *   (clamped to 0 .. Nk; what lies behind it is not used, whatever it holds); causal: also only at j <= i + Nk - Nq.
+ *   out [B,Nq,H,2D] dtype, contiguous, 16-byte aligned; a row that sees no key is 0.
+ *   stats: NULL, or [4,B,H,Nq] fp32 for the backward pass (maximum and log2 of the sum of either map's row).
+ *   scratch: hitadv_diff_attention_scratch_floats(...) floats, 16-byte aligned (0: NULL is fine): few rows over many keys are split.
+ * backward: dout [B,Nq,H,2D] contiguous; r [2,B,H,Nq] fp32 scratch; dq, dk, dv contiguous in the shapes of q, k, v (dk, dv summed over a
+ *   group's heads; 0 behind the lengths; both or neither may be NULL); dlam [lam_n] fp32, or NULL if not wanted.  Every sum in a fixed order: no atomics.
+ * D a multiple of 8 up to 64, H a multiple of Hkv; hitadv_diff_attention_supported says whether the sizes are taken (rows Nq G and Nk up
+ * to 2,000,000, B Hkv up to 65535). */
+int hitadv_diff_attention_supported(int dtype, int64_t B, int64_t Nq, int64_t Nk, int64_t H, int64_t Hkv, int64_t D);
+int64_t hitadv_diff_attention_scratch_floats(int B, int Nq, int Nk, int H, int Hkv, int D);
+int hitadv_diff_attention_fwd(int dtype, const void *q, const void *k, const void *v, const float *lam, int lam_n, const int32_t *lengths,
+                              const int64_t *strides, int B, int Nq, int Nk, int H, int Hkv, int D, int causal, float scale, void *out,
+                              float *stats, float *scratch, void *stream);
+int hitadv_diff_attention_bwd(int dtype, const void *q, const void *k, const void *v, const float *lam, int lam_n, const int32_t *lengths,
+                              const int64_t *strides, const void *dout, const float *stats, int B, int Nq, int Nk, int H, int Hkv, int D,
+                              int causal, float scale, float *r, void *dq, void *dk, void *dv, float *dlam, void *stream);
+
+/* Root-mean-square norm of contiguous rows [rows,cols], 1 <= cols <= 16384: s = x + residual rounded to dtype (residual NULL: s = x),
+ * r = 1 / sqrt(mean(s^2) + eps), y = s r w.  w [cols] is fp32 or dtype (wtype).
+ *   fwd    y [rows,cols]; sum [rows,cols] = s if there is a residual; rstd [rows] = r, or NULL
+ *   e4m3   q [rows,cols] = e4m3(y / scale), scale [rows] = max |y| / 448 (1 for a row of zeros)
+ *   bwd    dx = r (g - s r^2 mean(g s)) + dsum, g = dy w (dsum NULL: without it; dx is the gradient of x and of the residual);
+ *          dw [cols] in wtype = sum over the rows of dy s r, or NULL; scratch: hitadv_rms_norm_bwd_scratch_floats if dw is wanted */
+int hitadv_rms_norm_fwd(int dtype, int wtype, const void *x, const void *residual, const void *w, int64_t rows, int cols, float eps,
+                        void *y, void *sum, float *rstd, void *stream);
+int hitadv_rms_norm_e4m3(int dtype, int wtype, const void *x, const void *residual, const void *w, int64_t rows, int cols, float eps,
+                         void *q, float *scale, void *sum, void *stream);
+int64_t hitadv_rms_norm_bwd_scratch_floats(int64_t rows, int cols);
+int hitadv_rms_norm_bwd(int dtype, int wtype, const void *s, const void *w, const float *rstd, const void *dy, const void *dsum,
+                        int64_t rows, int cols, void *dx, float *scratch, void *dw, void *stream);
+
+/* y[i] = keep(i) x[i] scale (+ residual[i]) over n contiguous elements; keep(i): word i mod 4 of Philox4x32-10 with the counter
+ * (i / 4, rng[1]) and the key rng[0] is >= threshold (= p 2^32; 2^32 drops everything).  rng: int64 [2] in DEVICE memory. */
+int hitadv_dropout(int dtype, const void *x, const void *residual, void *y, int64_t n, const int64_t *rng, uint64_t threshold, float scale,
+                   void *stream);
+
 #ifdef __cplusplus
 }
 #endif
