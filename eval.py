@@ -48,6 +48,8 @@ def parse_args(argv=None):
     p.add_argument('--use_uniform_sample', action='store_true')
     p.add_argument('--num_category', default=40, type=int, choices=[10, 16, 40])
     p.add_argument('--model', type=str, default='pointnet', choices=['pointnet', 'dgcnn', 'pointnet++', 'pct'])
+    p.add_argument('--attention', type=str, default='offset', choices=['offset', 'differential'],
+                   help="the layers of --model pct: the reference's offset attention, or differential attention (weights of its own)")
     p.add_argument('--emb_dims', type=int, default=1024)
     p.add_argument('--dropout', type=float, default=0.2)
     p.add_argument('--k', type=int, default=5, help='DGCNN graph degree and the neighbour count of the Uniform metric')

@@ -182,12 +182,31 @@ template <int NA, int NB> __device__ __forceinline__ f32x16 da_mfma(const bf16x8
 }
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-// c += a b for two inputs' operands
-template <int NP> __device__ __forceinline__ f32x16 da_mfma_in(const bf16x8 (&a)[DA_NR<NP>], const bf16x8 (&b)[DA_NR<NP>], f32x16 c) {
+// c += a b for two inputs' operands.  QUERY_A: the query's operand is a (else b); the piece products are taken in the same order either
+// way, so that every kernel computes a score and a dP to the same bits (a row with one key: dP - r = 0).
+template <int NP, bool QUERY_A> __device__ __forceinline__ f32x16 da_mfma_in(const bf16x8 (&a)[DA_NR<NP>], const bf16x8 (&b)[DA_NR<NP>], f32x16 c) {
   if constexpr (NP == 2)
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a[0]), __builtin_bit_cast(f16x8, b[0]), c, 0, 0, 0);
-  else
-    return da_mfma<DA_NR<NP>, DA_NR<NP>>(a, b, c);
+#pragma unroll
+  for (int s = DA_NR<NP> - 1; s >= 0; --s)  // the small products first
+#pragma unroll
+    for (int i = 0; i <= s; ++i) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[QUERY_A ? s - i : i], b[QUERY_A ? i : s - i], c, 0, 0, 0);
+  return c;
+}
+// The same with fp32's small products in a sum of their own: the instruction truncates what it aligns to a larger accumulator, always
+// downwards, and r = sum P dP adds such an offset of dP up over every row (dlam of 32 x 256 rows: 5.6e-6 off with one sum)
+template <int NP, bool QUERY_A>
+__device__ __forceinline__ void da_mfma_in2(const bf16x8 (&a)[DA_NR<NP>], const bf16x8 (&b)[DA_NR<NP>], f32x16 &c, f32x16 &small) {
+  if constexpr (NP == 3) {
+#pragma unroll
+    for (int s = 2; s >= 1; --s)
+#pragma unroll
+      for (int i = 0; i <= s; ++i)
+        small = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[QUERY_A ? s - i : i], b[QUERY_A ? i : s - i], small, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[0], c, 0, 0, 0);
+  } else {
+    c = da_mfma_in<NP, QUERY_A>(a, b, c);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------- LDS tiles
@@ -349,7 +368,7 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_fwd_k(DaP p) {
       for (int c = 0; c < KC; ++c) {
         bf16x8 a[NR];
         Tile::frag_row(Ks, col, m * DP + 16 * c + 8 * half, a);
-        s = da_mfma_in<NP>(a, qf[m][c], s);
+        s = da_mfma_in<NP, false>(a, qf[m][c], s);
       }
       float top = -DA_INF;
 #pragma unroll
@@ -542,13 +561,14 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dq_k(DaP p) {
       if (pass) da_stage_cols<NP, DP>(Kt, p.k, ks, tid, 64 * NW);
       __syncthreads();
       if (t >= lim_hi) continue;
-      f32x16 dp = da_zero16();
+      f32x16 dp = da_zero16(), small = da_zero16();
 #pragma unroll
       for (int c = 0; c < VC; ++c) {
         bf16x8 a[NR];
         Tile::frag_row(Vs, col, 16 * c + 8 * half, a);
-        dp = da_mfma_in<NP>(a, gf[c], dp);
+        da_mfma_in2<NP, false>(a, gf[c], dp, small);
       }
+      if (NP == 3) dp += small;
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         f32x16 s = da_zero16();
@@ -556,7 +576,7 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dq_k(DaP p) {
         for (int c = 0; c < KC; ++c) {
           bf16x8 a[NR];
           Tile::frag_row(Ks, col, m * DP + 16 * c + 8 * half, a);
-          s = da_mfma_in<NP>(a, qf[m][c], s);
+          s = da_mfma_in<NP, false>(a, qf[m][c], s);
         }
         float ds[16];
         const bool edge = t + DA_T > lim_lo;
@@ -688,7 +708,7 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dkv_k(DaP p) {
       lims[tid] = ok ? da_limit(p, i, len) : 0;
     }
     __syncthreads();
-    f32x16 dp = da_zero16();
+    f32x16 dp = da_zero16(), small = da_zero16();
 #pragma unroll
     for (int c = 0; c < VC; ++c) {
       bf16x8 a[NR];
@@ -697,12 +717,13 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dkv_k(DaP p) {
         bf16x8 w[NR];
 #pragma unroll
         for (int k = 0; k < NR; ++k) w[k] = k == NR - 1 ? as_bf16x8(parked[c * 64 * NW]) : vf[c][k];
-        dp = da_mfma_in<NP>(a, w, dp);
+        da_mfma_in2<NP, true>(a, w, dp, small);
       } else {
-        dp = da_mfma_in<NP>(a, vf[c], dp);
+        da_mfma_in2<NP, true>(a, vf[c], dp, small);
       }
       if (NP == 3) __builtin_amdgcn_sched_barrier(0);  // (without it the fragments of several products are fetched ahead and spill)
     }
+    if (NP == 3) dp += small;
     float A[16];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
@@ -715,9 +736,9 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dkv_k(DaP p) {
           bf16x8 w[NR];
 #pragma unroll
           for (int k = 0; k < NR; ++k) w[k] = k == NR - 1 ? as_bf16x8(parked[(VC + c) * 64 * NW]) : kf[m][c][k];
-          s = da_mfma_in<NP>(a, w, s);
+          s = da_mfma_in<NP, true>(a, w, s);
         } else {
-          s = da_mfma_in<NP>(a, kf[m][c], s);
+          s = da_mfma_in<NP, true>(a, kf[m][c], s);
         }
         if (NP == 3) __builtin_amdgcn_sched_barrier(0);
       }

@@ -138,6 +138,64 @@ class SA_Layer(nn.Module):
         return x + self.act(conv1x1(self.trans_conv, self.after_norm, x - x_r))
 
 
+class DA_Layer(nn.Module):
+    """A differential-attention layer in SA_Layer's place (not in the reference: ``Pct(args)`` with ``args.attention = 'differential'``):
+    ``x + dropout(out(head_norm(diff_attention(q, k, v, lam))))`` with q, k, v one projection of ``norm(x)``, channels / 64 heads of two maps
+    of 32 channels, lam = exp(lq1 . lk1) - exp(lq2 . lk2) + LAM_INIT per head, and (1 - LAM_INIT) folded into the head norm's initial
+    weight.  On the GPU every step between the two products is one launch of ops.rms_norm / diff_attention / dropout; with frozen weights
+    (eval mode) the gradient is the input's alone.  In training the mask's (seed, offset) live in ``rng``: a captured step draws a new
+    mask at every replay."""
+    LAM_INIT = 0.8
+
+    def __init__(self, channels, dropout=0.):
+        super().__init__()
+        if channels % 64:
+            raise ValueError("DA_Layer: channels must be a multiple of 64, got %d" % channels)
+        self.heads, self.p = channels // 64, float(dropout)
+        self.norm = nn.Parameter(torch.ones(channels))
+        self.qkv = nn.Linear(channels, 3 * channels, bias=False)
+        self.lam_q = nn.Parameter(torch.randn(2, self.heads, 32) * 0.1)
+        self.lam_k = nn.Parameter(torch.randn(2, self.heads, 32) * 0.1)
+        self.head_norm = nn.Parameter(torch.full((64,), 1. - self.LAM_INIT))
+        self.out = nn.Linear(channels, channels)
+        self.register_buffer("rng", torch.stack([torch.randint(0, 2 ** 62, ()), torch.zeros((), dtype=torch.int64)]), persistent=False)  # a seed per layer
+
+    @staticmethod
+    def _plain_norm(x, w):
+        return x * torch.rsqrt(x.pow(2).mean(dim=-1, keepdim=True) + 1e-6) * w
+
+    def forward_pm(self, x):
+        """x [B,N,C] points-major."""
+        from . import _pointwise as P
+        B, N, C = x.shape
+        H = self.heads
+        const = not self.training and not P.WEIGHT_GRADS
+        norm, Wqkv, lq, lk, head_norm, Wo, bo = (t.detach() if const else t for t in (
+            self.norm, self.qkv.weight, self.lam_q, self.lam_k, self.head_norm, self.out.weight, self.out.bias))
+        e = (lq * lk).sum(dim=-1).exp()
+        lam = e[0] - e[1] + self.LAM_INIT
+        h = F.linear(ops.rms_norm(x, norm) if x.is_cuda else self._plain_norm(x, norm), Wqkv)
+        q, k, v = h.view(B, N, 3, C).unbind(2)  # rows of 3 C: the attention reads the three slices where they are
+        q, k, v = q.view(B, N, H, 2, 32), k.view(B, N, H, 2, 32), v.view(B, N, H, 64)
+        if x.is_cuda:
+            a = ops.rms_norm(ops.diff_attention(q, k, v, lam.float()), head_norm)
+        else:
+            m = torch.softmax(torch.einsum("bihmd,bjhmd->bhmij", q, k) * 32 ** -0.5, dim=-1)
+            a = torch.einsum("bhij,bjhd->bihd", m[:, :, 0] - lam.view(-1, 1, 1) * m[:, :, 1], v)
+            a = self._plain_norm(a, head_norm)
+        y = F.linear(a.reshape(B, N, C), Wo, bo)
+        if not (self.training and self.p > 0.):
+            return x + y
+        if not x.is_cuda:
+            return x + F.dropout(y, self.p)
+        rng = self.rng.clone()  # the backward pass needs this call's offset
+        self.rng[1] += 1
+        return ops.dropout(y, self.p, rng, residual=x)
+
+    def forward(self, x):
+        return self.forward_pm(x.permute(0, 2, 1)).permute(0, 2, 1)
+
+
 class Point_Transformer_Last(nn.Module):
     def __init__(self, args, channels=256):
         super().__init__()
@@ -146,8 +204,12 @@ class Point_Transformer_Last(nn.Module):
         self.conv2 = nn.Conv1d(channels, channels, kernel_size=1, bias=False)
         self.bn1 = nn.BatchNorm1d(channels)
         self.bn2 = nn.BatchNorm1d(channels)
-        self.sa1, self.sa2 = SA_Layer(channels), SA_Layer(channels)
-        self.sa3, self.sa4 = SA_Layer(channels), SA_Layer(channels)
+        kind = getattr(args, 'attention', 'offset')
+        if kind not in ('offset', 'differential'):
+            raise ValueError("Pct: attention must be 'offset' or 'differential', got %r" % (kind,))
+        layer = SA_Layer if kind == 'offset' else lambda c: DA_Layer(c, getattr(args, 'dropout', 0.))
+        self.sa1, self.sa2 = layer(channels), layer(channels)
+        self.sa3, self.sa4 = layer(channels), layer(channels)
 
     def forward_pm(self, x):
         """x [B,N,C] points-major -> [B,N,4C]."""
