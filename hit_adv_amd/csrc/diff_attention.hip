@@ -568,7 +568,10 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dq_k(DaP p) {
         Tile::frag_row(Vs, col, 16 * c + 8 * half, a);
         da_mfma_in2<NP, false>(a, gf[c], dp, small);
       }
-      if (NP == 3) dp += small;
+      if (NP == 3) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dp[e] += small[e];
+      }
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         f32x16 s = da_zero16();
@@ -723,7 +726,10 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dkv_k(DaP p) {
       }
       if (NP == 3) __builtin_amdgcn_sched_barrier(0);  // (without it the fragments of several products are fetched ahead and spill)
     }
-    if (NP == 3) dp += small;
+    if (NP == 3) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) dp[e] += small[e];
+    }
     float A[16];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {

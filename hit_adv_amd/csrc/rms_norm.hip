@@ -218,6 +218,7 @@ __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void rms_norm_bwd_k(RnP p)
           if ((threadIdx.x & 63) < TEAM) share[(threadIdx.x >> 6) * SPAN + (k * TEAM + lane) * V + j] = acc[k][j];
         }
       __syncthreads();
+#pragma clang loop vectorize(disable)
       for (int c = threadIdx.x; c < p.cols; c += NT) {
         float t = share[c];
 #pragma unroll
@@ -243,6 +244,7 @@ __global__ __launch_bounds__(256) void rms_norm_dw_k(const float *__restrict__ p
   const int cl = threadIdx.x & 15, sl = threadIdx.x >> 4, c = blockIdx.x * 16 + cl;
   float t = 0.f;
   if (c < cols)
+#pragma clang loop vectorize(disable)
     for (int i = sl; i < n; i += 16) t += part[(int64_t)i * cols + c];
   s[sl][cl] = t;
   __syncthreads();

@@ -1157,12 +1157,19 @@ _DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # include
 
 
 def _call_on(t, name, *args):
-    """``_lib.call`` with the current stream of ``t``'s device as the last argument, on that device."""
-    if t.device.index != torch.cuda.current_device():
-        with torch.cuda.device(t.device):
-            _lib.call(name, *args, _stream())
+    """``_lib.call`` with the current stream of ``t``'s device as the last argument, on that device.  (The raw handle: torch.cuda.current_stream()
+    takes 19 us on autograd's worker thread, where every backward pass runs, against 0.3.)"""
+    dev = t.get_device()
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, stream)
     else:
-        _lib.call(name, *args, _stream())
+        _lib.call(name, *args, stream)
+
+
+def _at(t):
+    return 0 if t is None else t.data_ptr()
 
 
 def _typed(t, name, like=None, dtypes=_DTYPE_CODE):
@@ -1216,8 +1223,8 @@ class DiffAttention(torch.autograd.Function):
             n = _lib.load().hitadv_diff_attention_scratch_floats(B, Nq, Nk, H, Hkv, D)
             scratch = torch.empty(n, device=q.device) if n else None
             lam32 = lam.contiguous()
-            _call_on(q, "hitadv_diff_attention_fwd", _DTYPE_CODE[q.dtype], _p(q), _p(k), _p(v), _p(lam32), lam.numel(), _p(lengths), ctx.strides,
-                     B, Nq, Nk, H, Hkv, D, int(causal), ctypes.c_float(scale), _p(out), _p(stats), _p(scratch))
+            _call_on(q, "hitadv_diff_attention_fwd", _DTYPE_CODE[q.dtype], _at(q), _at(k), _at(v), _at(lam32), lam.numel(), _at(lengths), ctx.strides,
+                     B, Nq, Nk, H, Hkv, D, int(causal), scale, _at(out), _at(stats), _at(scratch))
         if keep:
             ctx.save_for_backward(q, k, v, lam, lengths, stats)
             ctx.scale, ctx.causal = scale, causal
@@ -1240,9 +1247,9 @@ class DiffAttention(torch.autograd.Function):
             dk, dv = torch.empty(k.shape, device=q.device, dtype=q.dtype), torch.empty(v.shape, device=q.device, dtype=q.dtype)
         if need[3]:
             dlam = torch.empty(lam.shape, device=q.device)
-        _call_on(q, "hitadv_diff_attention_bwd", _DTYPE_CODE[q.dtype], _p(q), _p(k), _p(v), _p(lam.contiguous()), lam.numel(), _p(lengths),
-                 ctx.strides, _p(g), _p(stats), B, Nq, Nk, H, Hkv, D, int(ctx.causal), ctypes.c_float(ctx.scale), _p(r), _p(dq), _p(dk), _p(dv),
-                 _p(dlam))
+        _call_on(q, "hitadv_diff_attention_bwd", _DTYPE_CODE[q.dtype], _at(q), _at(k), _at(v), _at(lam.contiguous()), lam.numel(), _at(lengths),
+                 ctx.strides, _at(g), _at(stats), B, Nq, Nk, H, Hkv, D, int(ctx.causal), ctx.scale, _at(r), _at(dq), _at(dk), _at(dv),
+                 _at(dlam))
         return dq, dk, dv, dlam, None, None, None, None
 
 
@@ -1297,8 +1304,8 @@ class RmsNorm(torch.autograd.Function):
         total = torch.empty_like(x) if residual is not None else None
         rstd = torch.empty(rows, device=x.device) if keep else None
         if rows:
-            _call_on(x, "hitadv_rms_norm_fwd", _DTYPE_CODE[x.dtype], _DTYPE_CODE[weight.dtype], _p(x),
-                     _p(residual.contiguous() if residual is not None else None), _p(weight), rows, C, ctypes.c_float(eps), _p(y), _p(total), _p(rstd))
+            _call_on(x, "hitadv_rms_norm_fwd", _DTYPE_CODE[x.dtype], _DTYPE_CODE[weight.dtype], _at(x),
+                     _at(residual.contiguous() if residual is not None else None), _at(weight), rows, C, eps, _at(y), _at(total), _at(rstd))
         if keep:
             ctx.set_materialize_grads(False)
             ctx.save_for_backward(x if residual is None else total, weight, rstd)
@@ -1319,8 +1326,8 @@ class RmsNorm(torch.autograd.Function):
             dw = torch.empty_like(weight)
             scratch = torch.empty(_lib.load().hitadv_rms_norm_bwd_scratch_floats(rows, C), device=s.device)
         if rows:
-            _call_on(s, "hitadv_rms_norm_bwd", _DTYPE_CODE[s.dtype], _DTYPE_CODE[weight.dtype], _p(s), _p(weight), _p(rstd), _p(dy.contiguous()),
-                     _p(dsum.contiguous() if dsum is not None else None), rows, C, _p(dx), _p(scratch), _p(dw))
+            _call_on(s, "hitadv_rms_norm_bwd", _DTYPE_CODE[s.dtype], _DTYPE_CODE[weight.dtype], _at(s), _at(weight), _at(rstd), _at(dy.contiguous()),
+                     _at(dsum.contiguous() if dsum is not None else None), rows, C, _at(dx), _at(scratch), _at(dw))
         elif dw is not None:
             dw.zero_()
         return dx if need[0] else None, dw, None, dx if need[3] else None, None
@@ -1365,17 +1372,17 @@ def rms_norm_quant(x, weight, eps=1e-6, residual=None):
     scale = torch.empty(x.shape[:-1], device=x.device)
     total = torch.empty_like(x) if residual is not None else None
     if rows:
-        _call_on(x, "hitadv_rms_norm_e4m3", _DTYPE_CODE[x.dtype], _DTYPE_CODE[weight.dtype], _p(x),
-                 _p(residual.contiguous() if residual is not None else None), _p(weight), rows, C, ctypes.c_float(float(eps)), _p(q), _p(scale),
-                 _p(total))
+        _call_on(x, "hitadv_rms_norm_e4m3", _DTYPE_CODE[x.dtype], _DTYPE_CODE[weight.dtype], _at(x),
+                 _at(residual.contiguous() if residual is not None else None), _at(weight), rows, C, float(eps), _at(q), _at(scale),
+                 _at(total))
     return (q, scale) if residual is None else (q, scale, total)
 
 
 def _dropout_raw(x, residual, p, rng):
     y = torch.empty_like(x)
     if x.numel():
-        _call_on(x, "hitadv_dropout", _DTYPE_CODE[x.dtype], _p(x), _p(residual), _p(y), x.numel(), _p(rng), int(round(p * 2 ** 32)),
-                 ctypes.c_float(1.0 / (1.0 - p) if p < 1.0 else 0.0))
+        _call_on(x, "hitadv_dropout", _DTYPE_CODE[x.dtype], _at(x), _at(residual), _at(y), x.numel(), _at(rng), int(round(p * 2 ** 32)),
+                 1.0 / (1.0 - p) if p < 1.0 else 0.0)
     return y
 
 
