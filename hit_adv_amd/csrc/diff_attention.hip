@@ -117,9 +117,8 @@ template <int NP> __device__ __forceinline__ void da_pieces8(const Raw8<NP> &r, 
       out[k] = make_uint4(pack_hi(p[0][k], p[1][k]), pack_hi(p[2][k], p[3][k]), pack_hi(p[4][k], p[5][k]), pack_hi(p[6][k], p[7][k]));
   }
 }
-// four rows of four values -> for each piece and column the four rows' values (a 4 x 4 transposition)
-template <int NP> __device__ __forceinline__ void da_transpose4(const Raw4<NP> (&r)[4], uint2 (&out)[NP][4]) {
-  uint32_t p[4][4][NP];  // [row][column][piece]
+// the pieces of four rows of four values, [row][column][piece]
+template <int NP> __device__ __forceinline__ void da_pieces4x4(const Raw4<NP> (&r)[4], uint32_t (&p)[4][4][NP]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if constexpr (NP == 3) {
@@ -139,11 +138,6 @@ template <int NP> __device__ __forceinline__ void da_transpose4(const Raw4<NP> (
       p[i][3][0] = r[i].a.y & 0xffff0000u;
     }
   }
-#pragma unroll
-  for (int k = 0; k < NP; ++k)
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      out[k][c] = make_uint2(pack_hi(p[0][c][k], p[1][c][k]), pack_hi(p[2][c][k], p[3][c][k]));
 }
 
 // eight probabilities -> NPP pieces, each the B operand of a matrix instruction
@@ -228,70 +222,134 @@ template <int NP, int DP> struct DaTile {
 #pragma unroll
     for (int k = 0; k < NR; ++k) *(uint4 *)(t + (k * DA_T + row) * RS + col) = p[k];
   }
-  // rows 4 rg .. 4 rg + 3, columns col .. col + 3: key 16 c + 8 y + 4 x + j sits at 16 c + 8 x + 4 y + j
-  static __device__ __forceinline__ void put_col(uint16_t *t, int rg, int col, const Raw4<NP> (&r)[4]) {
-    uint2 o[NP][4];
-    da_transpose4<NP>(r, o);
-    const int at = 16 * (rg >> 2) + 8 * (rg & 1) + 4 * ((rg >> 1) & 1);
+  // rows 4 rg .. 4 rg + 3, columns col .. col + 3, as rows and / or transposed: there row 16 c + 8 y + 4 x + j sits at 16 c + 8 x + 4 y + j
+  template <bool AS_ROWS, bool AS_COLS> static __device__ __forceinline__ void put_block(uint16_t *rows, uint16_t *cols, int rg, int col, const Raw4<NP> (&r)[4]) {
+    if constexpr (AS_ROWS) {
 #pragma unroll
-    for (int k = 0; k < NP; ++k)
+      for (int i = 0; i < 4; ++i) {
+        uint16_t *to = rows + (4 * rg + i) * RS + col;
+        if constexpr (NP == 3) {
+          uint32_t p[4][3];
+          da_pieces<3>(r[i].a.x, p[0]);
+          da_pieces<3>(r[i].a.y, p[1]);
+          da_pieces<3>(r[i].a.z, p[2]);
+          da_pieces<3>(r[i].a.w, p[3]);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) *(uint2 *)(t + (k * W + col + c) * DA_TS + at) = o[k][c];
+          for (int k = 0; k < 3; ++k) *(uint2 *)(to + k * DA_T * RS) = make_uint2(pack_hi(p[0][k], p[1][k]), pack_hi(p[2][k], p[3][k]));
+        } else {
+          *(uint2 *)to = r[i].a;
+        }
+      }
+    }
+    if constexpr (AS_COLS) {
+      uint32_t p[4][4][NP];
+      da_pieces4x4<NP>(r, p);
+      const int at = 16 * (rg >> 2) + 8 * (rg & 1) + 4 * ((rg >> 1) & 1);
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int k = 0; k < NP; ++k)
+          *(uint2 *)(cols + (k * W + col + c) * DA_TS + at) = make_uint2(pack_hi(p[0][c][k], p[1][c][k]), pack_hi(p[2][c][k], p[3][c][k]));
+    }
   }
 };
 
-// where a tile's rows come from: element offset of row `row`'s column `col` of the padded [2][DP] (or [2 DP]) row, or -1 for a zero
-template <int DP> struct DaKeys {  // key rows t .. t + 31 of k (maps of D) or v (2 D in one piece)
-  int64_t base, n, m;
-  int t, end, D;
-  bool maps;
-  __device__ __forceinline__ int64_t at(int row, int col) const {
-    const int key = t + row;
-    if (maps) {
-      const int map = col >= DP, d = col - (map ? DP : 0);
-      return key < end && d < D ? base + key * n + map * m + d : -1;
-    }
-    return key < end && col < 2 * D ? base + key * n + col : -1;
+// What a workgroup of NT threads fetches of the next tile while it computes on this one: raw elements in registers.  A thread's column is
+// the same in all its pieces; an address is a wave-uniform base plus a 32-bit offset of the thread (strides below 2^24 elements: the entry
+// points see to it).  Threads whose column is padding (D < DP) fetch and store nothing: their cells of the tile are zeroed once.
+template <int NP, int DP> struct DaFetch {
+  static constexpr int ES = NP == 3 ? 4 : 2;  // bytes of an element
+  int row, col;
+  uint32_t off;  // bytes
+  bool there;
+  __device__ __forceinline__ void bind_at(int row_, int col_, bool inside, int64_t n, int64_t m, int D, bool maps) {
+    row = row_;
+    col = col_;
+    const int map = maps && col >= DP ? 1 : 0, d = col - map * DP;
+    there = inside && d < (maps ? D : 2 * D);
+    off = (uint32_t)(row * (int)n + map * (int)m + d) * ES;
   }
 };
-template <int DP> struct DaRows {  // packed query rows t .. t + 31 of q (maps) or dout
-  int64_t base, n, h, m;
-  int t, end, D;
-  bool maps;
-  const DaP *p;
-  __device__ __forceinline__ int64_t at(int row, int col) const {
-    const int r = t + row;
-    if (r >= end) return -1;
-    const int i = da_div_g(*p, r), g = r - i * p->G;
-    if (maps) {
-      const int map = col >= DP, d = col - (map ? DP : 0);
-      return d < D ? base + i * n + g * h + map * m + d : -1;
-    }
-    return col < 2 * D ? base + i * n + g * h + col : -1;
-  }
-};
-
-template <int NP, int DP, class SRC> __device__ __forceinline__ void da_stage_rows(uint16_t *t, const void *src, const SRC &s, int tid, int nt) {
-  constexpr int CH = 2 * DP / 8;
-  for (int it = tid; it < DA_T * CH; it += nt) {
-    const int row = it / CH, col = 8 * (it % CH);
-    const int64_t at = s.at(row, col);
-    DaTile<NP, DP>::put_row(t, row, col, da_load8<NP>(src, at, at >= 0));
-  }
-}
-template <int NP, int DP, class SRC> __device__ __forceinline__ void da_stage_cols(uint16_t *t, const void *src, const SRC &s, int tid, int nt) {
-  constexpr int CH = 2 * DP / 4;
-  for (int it = tid; it < 8 * CH; it += nt) {
-    const int rg = it / CH, col = 4 * (it % CH);
-    Raw4<NP> r[4];
+template <int NP, int DP, int NT> struct DaFetchRows : DaFetch<NP, DP> {  // 16-byte (32-byte) pieces of 32 rows of k, v
+  static constexpr int CH = 2 * DP / 8, STEP = NT / CH, C = STEP >= DA_T ? 1 : DA_T / STEP;
+  using F = DaFetch<NP, DP>;
+  Raw8<NP> x[C];
+  __device__ __forceinline__ void bind(int64_t n, int64_t m, int D, bool maps, int tid) { F::bind_at(tid / CH, 8 * (tid % CH), tid / CH < DA_T, n, m, D, maps); }
+  // rows t .. t + 31 of the rows at `base` (elements, wave-uniform); `end`: the first row that does not exist (zeros from there on)
+  __device__ __forceinline__ void load(const void *src, int64_t base, int64_t n, int t, int end) {
+    if (!F::there) return;
+    const char *at = (const char *)src + (base + t * n) * F::ES;
+    if (t + DA_T <= end) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t at = s.at(4 * rg + j, col);
-      r[j] = da_load4<NP>(src, at, at >= 0);
+      for (int c = 0; c < C; ++c) x[c] = da_load8<NP>(at + c * STEP * n * F::ES + F::off, 0, true);
+    } else {
+#pragma unroll
+      for (int c = 0; c < C; ++c) x[c] = da_load8<NP>(at + c * STEP * n * F::ES + F::off, 0, t + c * STEP + F::row < end);
     }
-    DaTile<NP, DP>::put_col(t, rg, col, r);
   }
-}
+  __device__ __forceinline__ void put(uint16_t *rows) const {
+    if (!F::there) return;
+#pragma unroll
+    for (int c = 0; c < C; ++c) DaTile<NP, DP>::put_row(rows, F::row + c * STEP, F::col, x[c]);
+  }
+  __device__ __forceinline__ void zero_padding(uint16_t *rows) const {
+    if (F::there || F::row >= DA_T) return;
+#pragma unroll
+    for (int c = 0; c < C; ++c) DaTile<NP, DP>::put_row(rows, F::row + c * STEP, F::col, da_load8<NP>(nullptr, 0, false));
+  }
+};
+template <int NP, int DP, int NT> struct DaFetchBlocks : DaFetch<NP, DP> {  // 4 x 4 blocks, for a transposed tile, or both
+  static constexpr int CH = 2 * DP / 4, STEP = NT / CH, C = STEP >= 8 ? 1 : 8 / STEP;
+  using F = DaFetch<NP, DP>;
+  Raw4<NP> x[C][4];
+  __device__ __forceinline__ void bind(int64_t n, int64_t m, int D, bool maps, int tid) {
+    F::bind_at(4 * (tid / CH), 4 * (tid % CH), tid / CH < 8, n, m, D, maps);
+  }
+  __device__ __forceinline__ void load(const void *src, int64_t base, int64_t n, int t, int end) {
+    if (!F::there) return;
+    const char *at = (const char *)src + (base + t * n) * F::ES;
+    if (t + DA_T <= end) {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[c][i] = da_load4<NP>(at + (4 * c * STEP + i) * n * F::ES + F::off, 0, true);
+    } else {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          x[c][i] = da_load4<NP>(at + (4 * c * STEP + i) * n * F::ES + F::off, 0, t + F::row + 4 * c * STEP + i < end);
+    }
+  }
+  // packed query rows: row r is query r / G, head r % G
+  __device__ __forceinline__ void load_packed(const void *src, int64_t base, int64_t n, int64_t h, const DaP &p, int t) {
+    if (p.G == 1) return load(src, base, n, t, p.rows);
+    if (!F::there) return;
+    const char *at = (const char *)src + base * F::ES + (F::off - (uint32_t)(F::row * (int)n) * F::ES);
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = t + F::row + 4 * c * STEP + i, q = da_div_g(p, r);
+        x[c][i] = da_load4<NP>(at, q * n + (r - q * p.G) * h, r < p.rows);
+      }
+  }
+  template <bool ROWS, bool COLS> __device__ __forceinline__ void put(uint16_t *rows, uint16_t *cols) const {
+    if (!F::there) return;
+#pragma unroll
+    for (int c = 0; c < C; ++c) DaTile<NP, DP>::template put_block<ROWS, COLS>(rows, cols, F::row / 4 + c * STEP, F::col, x[c]);
+  }
+  template <bool ROWS, bool COLS> __device__ __forceinline__ void zero_padding(uint16_t *rows, uint16_t *cols) {
+    if (F::there || F::row >= DA_T) return;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      Raw4<NP> z[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) z[i] = da_load4<NP>(nullptr, 0, false);
+      DaTile<NP, DP>::template put_block<ROWS, COLS>(rows, cols, F::row / 4 + c * STEP, F::col, z);
+    }
+  }
+};
 
 // four consecutive outputs
 template <int NP> __device__ __forceinline__ void da_store4(void *base, int64_t at, float a, float b, float c, float d) {
@@ -313,144 +371,170 @@ __device__ __forceinline__ f32x16 da_zero16() {
 __device__ __forceinline__ int da_wave_id() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
 
 // ---------------------------------------------------------------------------------------------------------------- forward
-// One workgroup: NW waves of 32 packed rows each over the keys [split chunk, ...) of one (cloud, key / value head).
-template <int NP, int DP, int NW, bool SPLIT>
-__global__ __launch_bounds__(64 * NW) void diff_attn_fwd_k(DaP p) {
+// One workgroup: PAIRS pairs of waves over the keys [split chunk, ...) of one (cloud, key / value head); a pair has 32 packed rows, one of
+// its waves the first map, the other the second: half the accumulators each (two or three waves per SIMD, where one wave with both
+// maps fills the registers), and the difference is taken once, at the end, through LDS.  The next tile's elements are on their way in
+// registers while this one's are multiplied; two buffers, one barrier a tile.
+template <int NP, int DP, int PAIRS, bool SPLIT>
+__global__ __launch_bounds__(128 * PAIRS, 2) void diff_attn_fwd_k(DaP p) {
   using Tile = DaTile<NP, DP>;
-  constexpr int NR = DA_NR<NP>;
+  constexpr int NR = DA_NR<NP>, NT = 128 * PAIRS;
   constexpr int NPP = NP == 3 ? 3 : 2;  // pieces of a probability
   constexpr int KC = DP / 16, VB = 2 * DP / 32;
+  constexpr int BUF = Tile::ROWS + Tile::COLS;
   extern __shared__ __attribute__((aligned(16))) uint16_t da_lds[];
   uint16_t *Ks = da_lds, *Vt = da_lds + Tile::ROWS;
-  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = da_wave_id(), tid = threadIdx.x;
+  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = da_wave_id(), m = wave & 1, tid = threadIdx.x;
   const int b = blockIdx.x / p.Hkv, hk = blockIdx.x % p.Hkv, split = blockIdx.z;
   const int tile = p.causal ? (int)(gridDim.y - 1 - blockIdx.y) : (int)blockIdx.y;  // causal: the longest rows first
-  const int row0 = (tile * NW + wave) * DA_T, r = row0 + col;
-  const int i = da_div_g(p, r), g = r - i * p.G, h = hk * p.G + g;
-  const bool valid = r < p.rows;
-  const int len = da_len(p, b), lim = da_limit(p, i, len);
+  const int row0 = (tile * PAIRS + (wave >> 1)) * DA_T;
+  const int len = da_len(p, b);
   const int lim_lo = da_limit(p, da_div_g(p, row0), len), lim_hi = da_limit(p, da_div_g(p, row0 + DA_T - 1), len);
-  const int last = da_limit(p, da_div_g(p, min(p.rows, (tile + 1) * NW * DA_T) - 1), len);
+  const int last = da_limit(p, da_div_g(p, min(p.rows, (tile + 1) * PAIRS * DA_T) - 1), len);
   const int k0 = split * p.chunk, k1 = min(last, k0 + p.chunk);
-
-  bf16x8 qf[2][KC][NR];
-#pragma unroll
-  for (int m = 0; m < 2; ++m)
+  int lim;
+  bf16x8 qf[KC][NR];
+  {
+    const int r = row0 + col, i = da_div_g(p, r), h = hk * p.G + r - i * p.G;
+    lim = da_limit(p, i, len);
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
       const int d = 16 * c + 8 * half;
       uint4 w[NR];
-      da_pieces8<NP>(da_load8<NP>(p.q, b * p.q_b + i * p.q_n + h * p.q_h + m * p.q_m + d, valid && d < p.D), w);
+      da_pieces8<NP>(da_load8<NP>(p.q, b * p.q_b + i * p.q_n + h * p.q_h + m * p.q_m + d, r < p.rows && d < p.D), w);
 #pragma unroll
-      for (int k = 0; k < NR; ++k) qf[m][c][k] = as_bf16x8(w[k]);
+      for (int k = 0; k < NR; ++k) qf[c][k] = as_bf16x8(w[k]);
     }
+  }
 
-  f32x16 o[2][VB];
+  f32x16 o[VB];
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
-#pragma unroll
-    for (int v = 0; v < VB; ++v) o[m][v] = da_zero16();
-  float mx[2] = {-DA_INF, -DA_INF}, sum[2] = {0.f, 0.f};
+  for (int v = 0; v < VB; ++v) o[v] = da_zero16();
+  float mx = -DA_INF, sum = 0.f;
 
-  DaKeys<DP> ks{b * p.k_b + hk * p.k_h, p.k_n, p.k_m, 0, len, p.D, true}, vs{b * p.v_b + hk * p.v_h, p.v_n, 0, 0, len, p.D, false};
+  DaFetchRows<NP, DP, NT> fk;
+  DaFetchBlocks<NP, DP, NT> fv;
+  const int64_t k_at = b * p.k_b + hk * p.k_h, v_at = b * p.v_b + hk * p.v_h;
+  fk.bind(p.k_n, p.k_m, p.D, true, tid);
+  fv.bind(p.v_n, 0, p.D, false, tid);
+  fk.zero_padding(Ks);
+  fv.template zero_padding<false, true>(nullptr, Vt);
+  fk.zero_padding(Ks + BUF);
+  fv.template zero_padding<false, true>(nullptr, Vt + BUF);
+  if (k0 < k1) {
+    fk.load(p.k, k_at, p.k_n, k0, len);
+    fv.load(p.v, v_at, p.v_n, k0, len);
+    fk.put(Ks);
+    fv.template put<false, true>(nullptr, Vt);
+  }
+  __syncthreads();
+#pragma unroll 1
   for (int t = k0; t < k1; t += DA_T) {
-    __syncthreads();
-    ks.t = vs.t = t;
-    da_stage_rows<NP, DP>(Ks, p.k, ks, tid, 64 * NW);
-    da_stage_cols<NP, DP>(Vt, p.v, vs, tid, 64 * NW);
-    __syncthreads();
-    if (t >= lim_hi) continue;
-    float pr[2][16];
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
+    const bool more = t + DA_T < k1;
+    if (more) {
+      fk.load(p.k, k_at, p.k_n, t + DA_T, len);
+      fv.load(p.v, v_at, p.v_n, t + DA_T, len);
+    }
+    if (t < lim_hi) {
       f32x16 s = da_zero16();
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
         bf16x8 a[NR];
         Tile::frag_row(Ks, col, m * DP + 16 * c + 8 * half, a);
-        s = da_mfma_in<NP, false>(a, qf[m][c], s);
+        s = da_mfma_in<NP, false>(a, qf[c], s);
       }
-      float top = -DA_INF;
+      float pr[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) pr[m][e] = s[e] * p.scale2;
+      for (int e = 0; e < 16; ++e) pr[e] = s[e] * p.scale2;
       if (t + DA_T > lim_lo) {
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (t + 8 * (e >> 2) + 4 * half + (e & 3) >= lim) pr[m][e] = -DA_INF;
+          if (t + 8 * (e >> 2) + 4 * half + (e & 3) >= lim) pr[e] = -DA_INF;
       }
+      float top = pr[0];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) top = fmaxf(top, pr[m][e]);
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, pr[e]);
       top = fmaxf(top, __shfl_xor(top, 32, HITADV_WAVE));
-      if (__ballot(top > mx[m] + DA_SLACK) != 0ull) {  // (-inf + slack = -inf: the first visible key raises it)
-        const float nm = fmaxf(mx[m], top);
-        const float f = nm == -DA_INF ? 1.f : exp2_flush(mx[m] - nm);
-        sum[m] *= f;
-        mx[m] = nm;
+      if (__ballot(top > mx + DA_SLACK) != 0ull) {  // (-inf + slack = -inf: the first visible key raises it)
+        const float nm = fmaxf(mx, top);
+        const float f = nm == -DA_INF ? 1.f : exp2_flush(mx - nm);
+        sum *= f;
+        mx = nm;
 #pragma unroll
         for (int v = 0; v < VB; ++v)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[m][v][e] *= f;
+          for (int e = 0; e < 16; ++e) o[v][e] *= f;
       }
-      const float base = mx[m] == -DA_INF ? 0.f : mx[m];
+      const float base = mx == -DA_INF ? 0.f : mx;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        pr[m][e] = exp2_flush(pr[m][e] - base);
-        sum[m] += pr[m][e];
+        pr[e] = exp2_flush(pr[e] - base);
+        sum += pr[e];
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        bf16x8 bo[NPP];
+        da_operand<NPP>(&pr[8 * c], bo);
+#pragma unroll
+        for (int v = 0; v < VB; ++v) {
+          bf16x8 a[NP];
+          Tile::frag_col(Vt, 32 * v + col, c, half, a);
+          o[v] = da_mfma<NP, NPP>(a, bo, o[v]);
+        }
       }
     }
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      bf16x8 b1[NPP], b2[NPP];
-      da_operand<NPP>(&pr[0][8 * c], b1);
-      da_operand<NPP>(&pr[1][8 * c], b2);
-#pragma unroll
-      for (int v = 0; v < VB; ++v) {
-        bf16x8 a[NP];
-        Tile::frag_col(Vt, 32 * v + col, c, half, a);
-        o[0][v] = da_mfma<NP, NPP>(a, b1, o[0][v]);
-        o[1][v] = da_mfma<NP, NPP>(a, b2, o[1][v]);
-      }
+    Ks = Ks == da_lds ? da_lds + BUF : da_lds;  // the other buffer's readers met the barrier that ended the tile before this one
+    Vt = Ks + Tile::ROWS;
+    if (more) {
+      fk.put(Ks);
+      fv.template put<false, true>(nullptr, Vt);
     }
+    __syncthreads();
   }
 
-#pragma unroll
-  for (int m = 0; m < 2; ++m) sum[m] += __shfl_xor(sum[m], 32, HITADV_WAVE);
-  if (!valid) return;
+  sum += __shfl_xor(sum, 32, HITADV_WAVE);
+  const int r = row0 + col, i = da_div_g(p, r), h = hk * p.G + r - i * p.G;
+  const bool valid = r < p.rows;
   if (SPLIT) {
+    if (!valid) return;
     const int64_t row = ((int64_t)split * p.B * p.Hkv + blockIdx.x) * p.rows + r;
-    if (half == 0) *(float4 *)(p.part_ml + 4 * row) = make_float4(mx[0], sum[0], mx[1], sum[1]);
-    float *po = p.part_o + row * 4 * p.D;
+    if (half == 0) *(float2 *)(p.part_ml + 4 * row + 2 * m) = make_float2(mx, sum);
+    float *po = p.part_o + (2 * row + m) * 2 * p.D;
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int v = 0; v < VB; ++v)
 #pragma unroll
-      for (int v = 0; v < VB; ++v)
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          const int d = 32 * v + 2 * e + 4 * half;
-          if (d < 2 * p.D) *(float4 *)(po + m * 2 * p.D + d) = make_float4(o[m][v][e], o[m][v][e + 1], o[m][v][e + 2], o[m][v][e + 3]);
-        }
+      for (int e = 0; e < 16; e += 4) {
+        const int d = 32 * v + 2 * e + 4 * half;
+        if (d < 2 * p.D) *(float4 *)(po + d) = make_float4(o[v][e], o[v][e + 1], o[v][e + 2], o[v][e + 3]);
+      }
     return;
   }
-  const float w1 = sum[0] == 0.f ? 0.f : 1.f / sum[0], w2 = sum[1] == 0.f ? 0.f : -da_lam(p, h) / sum[1];
+  if (p.stats && valid && half == 0) {
+    const int64_t n = (int64_t)p.B * p.H * p.Nq, row = ((int64_t)b * p.H + h) * p.Nq + i;
+    p.stats[(2 * m) * n + row] = sum == 0.f ? 0.f : mx;
+    p.stats[(2 * m + 1) * n + row] = sum == 0.f ? DA_INF : log2f(sum);  // an empty row: every probability 2^-inf = 0
+  }
+  const float w = sum == 0.f ? 0.f : (m && valid ? -da_lam(p, h) : 1.f) / sum;
+  // the second map's part of a value block of 32 columns at a time, in the tiles' place (the last barrier is behind their readers)
+  float4 *part = (float4 *)da_lds + (wave >> 1) * 256 + lane;
   const int64_t at = (((int64_t)b * p.Nq + i) * p.H + h) * 2 * p.D;
 #pragma unroll
-  for (int v = 0; v < VB; ++v)
+  for (int v = 0; v < VB; ++v) {
+    if (m) {
 #pragma unroll
-    for (int e = 0; e < 16; e += 4) {
-      const int d = 32 * v + 2 * e + 4 * half;
-      if (d >= 2 * p.D) continue;
-      float x[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = o[0][v][e + j] * w1 + o[1][v][e + j] * w2;
-      da_store4<NP>(p.out, at + d, x[0], x[1], x[2], x[3]);
+      for (int e = 0; e < 4; ++e) part[64 * e] = make_float4(o[v][4 * e] * w, o[v][4 * e + 1] * w, o[v][4 * e + 2] * w, o[v][4 * e + 3] * w);
     }
-  if (p.stats && half == 0) {
-    const int64_t n = (int64_t)p.B * p.H * p.Nq, row = ((int64_t)b * p.H + h) * p.Nq + i;
+    __syncthreads();
+    if (!m && valid) {
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      p.stats[(2 * m) * n + row] = sum[m] == 0.f ? 0.f : mx[m];
-      p.stats[(2 * m + 1) * n + row] = sum[m] == 0.f ? DA_INF : log2f(sum[m]);  // an empty row: every probability 2^-inf = 0
+      for (int e = 0; e < 4; ++e) {
+        const float4 y = part[64 * e];
+        const int d = 32 * v + 8 * e + 4 * half;
+        if (d < 2 * p.D)
+          da_store4<NP>(p.out, at + d, o[v][4 * e] * w + y.x, o[v][4 * e + 1] * w + y.y, o[v][4 * e + 2] * w + y.z, o[v][4 * e + 3] * w + y.w);
+      }
     }
+    __syncthreads();
   }
 }
 
@@ -499,14 +583,18 @@ __global__ __launch_bounds__(128) void diff_attn_join_k(DaP p) {
 // second pass multiplies (not dO . out: out is rounded, and where a row sees one key dS has to vanish exactly).
 //
 // dQ: the forward kernel's layout, two passes over the keys: first r, then dQ_m^T = K_m^T dS_m^T.
+template <int NP, int DP> constexpr int DA_DQ_WAVES = NP == 3 ? 1 : 2;  // waves per SIMD: what the registers allow
 template <int NP, int DP, int NW>
-__global__ __launch_bounds__(64 * NW) void diff_attn_dq_k(DaP p) {
+__global__ __launch_bounds__(64 * NW, (DA_DQ_WAVES<NP, DP>)) void diff_attn_dq_k(DaP p) {
   using Tile = DaTile<NP, DP>;
   constexpr int NR = DA_NR<NP>;
   constexpr int NS = NP == 3 ? 3 : 2;  // pieces of dS
   constexpr int KC = DP / 16, VC = 2 * DP / 16, DB = DP / 32;
   extern __shared__ __attribute__((aligned(16))) uint16_t da_lds[];
   uint16_t *Ks = da_lds, *Vs = da_lds + Tile::ROWS, *Kt = da_lds + 2 * Tile::ROWS;
+  // 16-bit types: dO's operands are parked in LDS, read back by the lane that wrote them -- two waves per SIMD (256 registers)
+  constexpr bool PARK = NP != 3;
+  uint4 *parked = (uint4 *)(Kt + Tile::COLS) + threadIdx.x;
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = da_wave_id(), tid = threadIdx.x;
   const int b = blockIdx.x / p.Hkv, hk = blockIdx.x % p.Hkv;
   const int tile = p.causal ? (int)(gridDim.y - 1 - blockIdx.y) : (int)blockIdx.y;
@@ -536,12 +624,14 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dq_k(DaP p) {
     da_pieces8<NP>(da_load8<NP>(p.dout, (((int64_t)b * p.Nq + i) * p.H + h) * 2 * p.D + d, valid && d < 2 * p.D), w);
 #pragma unroll
     for (int k = 0; k < NR; ++k) gf[c][k] = as_bf16x8(w[k]);
+    if (PARK) parked[c * 64 * NW] = w[0];
   }
   float mx[2], ll[2], rs[2] = {0.f, 0.f};
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     mx[m] = valid ? p.stats[(2 * m) * n + srow] : 0.f;
     ll[m] = valid ? p.stats[(2 * m + 1) * n + srow] : DA_INF;
+    if (NP != 3) mx[m] += ll[m];  // one subtraction less; fp32 keeps the two apart: their sum's last bit is a probability's error
   }
   f32x16 acc[2][DB];
 #pragma unroll
@@ -549,24 +639,41 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dq_k(DaP p) {
 #pragma unroll
     for (int v = 0; v < DB; ++v) acc[m][v] = da_zero16();
 
-  DaKeys<DP> ks{b * p.k_b + hk * p.k_h, p.k_n, p.k_m, 0, len, p.D, true}, vs{b * p.v_b + hk * p.v_h, p.v_n, 0, 0, len, p.D, false};
+  DaFetchBlocks<NP, DP, 64 * NW> fk;
+  DaFetchRows<NP, DP, 64 * NW> fv;
+  const int64_t k_at = b * p.k_b + hk * p.k_h, v_at = b * p.v_b + hk * p.v_h;
+  fk.bind(p.k_n, p.k_m, p.D, true, tid);
+  fv.bind(p.v_n, 0, p.D, false, tid);
+  fk.template zero_padding<true, true>(Ks, Kt);
+  fv.zero_padding(Vs);
+  if (last > 0) {
+    fk.load(p.k, k_at, p.k_n, 0, len);
+    fv.load(p.v, v_at, p.v_n, 0, len);
+  }
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll 1
     for (int t = 0; t < last; t += DA_T) {
       __syncthreads();
-      ks.t = vs.t = t;
-      da_stage_rows<NP, DP>(Ks, p.k, ks, tid, 64 * NW);
-      da_stage_rows<NP, DP>(Vs, p.v, vs, tid, 64 * NW);
-      if (pass) da_stage_cols<NP, DP>(Kt, p.k, ks, tid, 64 * NW);
+      fv.put(Vs);
+      if (pass) fk.template put<true, true>(Ks, Kt);
+      else fk.template put<true, false>(Ks, nullptr);
       __syncthreads();
+      const int next = t + DA_T < last ? t + DA_T : 0;  // (behind the second pass: the first tile once more, not used)
+      fk.load(p.k, k_at, p.k_n, next, len);
+      fv.load(p.v, v_at, p.v_n, next, len);
       if (t >= lim_hi) continue;
       f32x16 dp = da_zero16(), small = da_zero16();
 #pragma unroll
       for (int c = 0; c < VC; ++c) {
         bf16x8 a[NR];
         Tile::frag_row(Vs, col, 16 * c + 8 * half, a);
-        da_mfma_in2<NP, false>(a, gf[c], dp, small);
+        if constexpr (PARK) {
+          const bf16x8 g[1] = {as_bf16x8(parked[c * 64 * NW])};
+          dp = da_mfma_in<NP, false>(a, g, dp);
+        } else {
+          da_mfma_in2<NP, false>(a, gf[c], dp, small);
+        }
       }
       if (NP == 3) {
 #pragma unroll
@@ -582,18 +689,19 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dq_k(DaP p) {
           s = da_mfma_in<NP, false>(a, qf[m][c], s);
         }
         float ds[16];
-        const bool edge = t + DA_T > lim_lo;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const bool seen = !edge || t + 8 * (e >> 2) + 4 * half + (e & 3) < lim;
-          ds[e] = seen ? exp2_flush((s[e] * p.scale2 - mx[m]) - ll[m]) : 0.f;
+        for (int e = 0; e < 16; ++e) ds[e] = exp2_flush(NP == 3 ? (s[e] * p.scale2 - mx[m]) - ll[m] : s[e] * p.scale2 - mx[m]);
+        if (t + DA_T > lim_lo) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (t + 8 * (e >> 2) + 4 * half + (e & 3) >= lim) ds[e] = 0.f;
         }
         if (pass == 0) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) rs[m] += ds[e] == 0.f ? 0.f : ds[e] * dp[e];
+          for (int e = 0; e < 16; ++e) rs[m] += ds[e] * dp[e];
         } else {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) ds[e] = ds[e] == 0.f ? 0.f : ds[e] * (dp[e] - rs[m]);
+          for (int e = 0; e < 16; ++e) ds[e] = ds[e] * (dp[e] - rs[m]);
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             bf16x8 bo[NS];
@@ -633,21 +741,19 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dq_k(DaP p) {
 }
 
 // dK and dV: a wave owns 32 keys (the lane's column) and walks over the packed rows of all G heads, so that the sum over the heads that
-// share a key needs no atomics: dV^T += dO^T A, dK_m^T += Q_m^T dS_m, A = P_1 - lam P_2.
-template <int NP, int DP, int NW>
+// share a key needs no atomics: dV^T += dO^T A, dK_m^T += Q_m^T dS_m, A = P_1 - lam P_2.  One launch for both, except for fp32 at DP = 64,
+// where three pieces of K and V and both accumulators are more than 512 registers: dV and dK in a launch each (the scores twice, a quarter
+// more products).
+template <int NP, int DP, int NW, bool DV, bool DK>
 __global__ __launch_bounds__(64 * NW) void diff_attn_dkv_k(DaP p) {
   using Tile = DaTile<NP, DP>;
   constexpr int NR = DA_NR<NP>;
   constexpr int NS = NP == 3 ? 3 : 2;
   constexpr int KC = DP / 16, VC = 2 * DP / 16, DB = DP / 32, VB = 2 * DP / 32;
   extern __shared__ __attribute__((aligned(16))) uint16_t da_lds[];
-  uint16_t *Qs = da_lds, *Gs = Qs + Tile::ROWS, *Qt = Gs + Tile::ROWS, *Gt = Qt + Tile::COLS;
-  float *st = (float *)(Gt + Tile::COLS);  // [7][32]: max 1, log2 sum 1, max 2, log2 sum 2, r 1, r 2, lam
+  uint16_t *Qs = da_lds, *Gs = Qs + Tile::ROWS, *Qt = Gs + (DK ? Tile::ROWS : 0), *Gt = Qt + (DK ? Tile::COLS : 0);
+  float *st = (float *)(Gt + (DV ? Tile::COLS : 0));  // [7][32]: max 1, log2 sum 1, max 2, log2 sum 2, r 1, r 2, lam
   int *lims = (int *)(st + 7 * DA_T);
-  // three pieces at DP = 64 do not fit the register file beside the accumulators: the third piece of V (and of a little of K) is
-  // parked in LDS, read back by the lane that wrote it
-  constexpr bool PARK = NP == 3 && DP == 64;
-  uint4 *parked = (uint4 *)(lims + DA_T) + threadIdx.x;
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = da_wave_id(), tid = threadIdx.x;
   const int b = blockIdx.x / p.Hkv, hk = blockIdx.x % p.Hkv;
   const int first = blockIdx.y * NW * DA_T, key0 = first + wave * DA_T, key = key0 + col;
@@ -664,16 +770,14 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dkv_k(DaP p) {
       da_pieces8<NP>(da_load8<NP>(p.k, b * p.k_b + key * p.k_n + hk * p.k_h + m * p.k_m + d, key < len && d < p.D), w);
 #pragma unroll
       for (int k = 0; k < NR; ++k) kf[m][c][k] = as_bf16x8(w[k]);
-      if (PARK && m == 0 && c < 2) parked[(VC + c) * 64 * NW] = w[NR - 1];
     }
 #pragma unroll
-  for (int c = 0; c < VC; ++c) {
+  for (int c = 0; c < (DK ? VC : 0); ++c) {
     const int d = 16 * c + 8 * half;
     uint4 w[NR];
     da_pieces8<NP>(da_load8<NP>(p.v, b * p.v_b + key * p.v_n + hk * p.v_h + d, key < len && d < 2 * p.D), w);
 #pragma unroll
     for (int k = 0; k < NR; ++k) vf[c][k] = as_bf16x8(w[k]);
-    if constexpr (PARK) parked[c * 64 * NW] = w[NR - 1];
   }
   f32x16 av[VB], ak[2][DB];
 #pragma unroll
@@ -686,51 +790,55 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dkv_k(DaP p) {
   // causal: query i sees key j when i >= j - (Nk - Nq): rows before that of the workgroup's first key have nothing here
   int begin = p.causal ? max(0, first - (p.Nk - p.Nq)) : 0;
   begin = first >= len ? p.rows : (int)min((int64_t)p.rows, (int64_t)begin * p.G) / DA_T * DA_T;
-  DaRows<DP> qs{b * p.q_b + hk * p.G * p.q_h, p.q_n, p.q_h, p.q_m, 0, p.rows, p.D, true, &p};
-  DaRows<DP> gs{((int64_t)b * p.Nq * p.H + hk * p.G) * 2 * p.D, (int64_t)p.H * 2 * p.D, 2 * p.D, 0, 0, p.rows, p.D, false, &p};
+  DaFetchBlocks<NP, DP, 64 * NW> fq, fg;
+  const int64_t g_n = (int64_t)p.H * 2 * p.D;
+  const int64_t q_at = b * p.q_b + hk * p.G * p.q_h, g_at = ((int64_t)b * p.Nq * p.H + hk * p.G) * 2 * p.D;
+  fq.bind(p.q_n, p.q_m, p.D, true, tid);
+  fg.bind(g_n, 0, p.D, false, tid);
+  fq.template zero_padding<true, DK>(Qs, Qt);
+  fg.template zero_padding<DK, DV>(Gs, Gt);
+  if (begin < p.rows) {
+    fq.load_packed(p.q, q_at, p.q_n, p.q_h, p, begin);
+    fg.load_packed(p.dout, g_at, g_n, 2 * p.D, p, begin);
+  }
 #pragma unroll 1
   for (int t = begin; t < p.rows; t += DA_T) {
     __syncthreads();
-    qs.t = gs.t = t;
-    da_stage_rows<NP, DP>(Qs, p.q, qs, tid, 64 * NW);
-    if (NP == 3) __builtin_amdgcn_sched_barrier(0);
-    da_stage_rows<NP, DP>(Gs, p.dout, gs, tid, 64 * NW);
-    if (NP == 3) __builtin_amdgcn_sched_barrier(0);
-    da_stage_cols<NP, DP>(Qt, p.q, qs, tid, 64 * NW);
-    if (NP == 3) __builtin_amdgcn_sched_barrier(0);
-    da_stage_cols<NP, DP>(Gt, p.dout, gs, tid, 64 * NW);
+    fq.template put<true, DK>(Qs, Qt);
+    fg.template put<DK, DV>(Gs, Gt);
     if (tid < DA_T) {
       const int r = t + tid, i = da_div_g(p, r), h = hk * p.G + r - i * p.G;
       const bool ok = r < p.rows;
       const int64_t srow = ((int64_t)b * p.H + h) * p.Nq + i;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) st[k * DA_T + tid] = ok ? p.stats[k * n + srow] : (k & 1) ? DA_INF : 0.f;
+      for (int k = 0; k < 4; k += 2) {
+        const float mx = ok ? p.stats[k * n + srow] : 0.f, ll = ok ? p.stats[(k + 1) * n + srow] : DA_INF;
+        st[k * DA_T + tid] = NP == 3 ? mx : mx + ll;  // (as in diff_attn_dq_k)
+        st[(k + 1) * DA_T + tid] = ll;
+      }
 #pragma unroll
       for (int k = 0; k < 2; ++k) st[(4 + k) * DA_T + tid] = ok ? p.r[k * n + srow] : 0.f;
       st[6 * DA_T + tid] = ok ? da_lam(p, h) : 0.f;
       lims[tid] = ok ? da_limit(p, i, len) : 0;
     }
     __syncthreads();
+    if (t + DA_T < p.rows) {
+      fq.load_packed(p.q, q_at, p.q_n, p.q_h, p, t + DA_T);
+      fg.load_packed(p.dout, g_at, g_n, 2 * p.D, p, t + DA_T);
+    }
     f32x16 dp = da_zero16(), small = da_zero16();
 #pragma unroll
-    for (int c = 0; c < VC; ++c) {
+    for (int c = 0; c < (DK ? VC : 0); ++c) {
       bf16x8 a[NR];
       Tile::frag_row(Gs, col, 16 * c + 8 * half, a);
-      if constexpr (PARK) {
-        bf16x8 w[NR];
-#pragma unroll
-        for (int k = 0; k < NR; ++k) w[k] = k == NR - 1 ? as_bf16x8(parked[c * 64 * NW]) : vf[c][k];
-        da_mfma_in2<NP, true>(a, w, dp, small);
-      } else {
-        da_mfma_in2<NP, true>(a, vf[c], dp, small);
-      }
-      if (NP == 3) __builtin_amdgcn_sched_barrier(0);  // (without it the fragments of several products are fetched ahead and spill)
+      da_mfma_in2<NP, true>(a, vf[c], dp, small);
     }
     if (NP == 3) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) dp[e] += small[e];
     }
     float A[16];
+    const bool edge = key0 + DA_T > da_limit(p, da_div_g(p, t), len);  // (limits grow with the row; rows that do not exist: 2^-inf = 0)
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       f32x16 s = da_zero16();
@@ -738,15 +846,7 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dkv_k(DaP p) {
       for (int c = 0; c < KC; ++c) {
         bf16x8 a[NR];
         Tile::frag_row(Qs, col, m * DP + 16 * c + 8 * half, a);
-        if (PARK && m == 0 && c < 2) {
-          bf16x8 w[NR];
-#pragma unroll
-          for (int k = 0; k < NR; ++k) w[k] = k == NR - 1 ? as_bf16x8(parked[(VC + c) * 64 * NW]) : kf[m][c][k];
-          s = da_mfma_in<NP, true>(a, w, s);
-        } else {
-          s = da_mfma_in<NP, true>(a, kf[m][c], s);
-        }
-        if (NP == 3) __builtin_amdgcn_sched_barrier(0);
+        s = da_mfma_in<NP, true>(a, kf[m][c], s);
       }
       float ds[16];
 #pragma unroll
@@ -760,16 +860,16 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dkv_k(DaP p) {
         const int lis[4] = {li.x, li.y, li.z, li.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float pm = key < lis[j] ? exp2_flush((s[e + j] * p.scale2 - mxs[j]) - lls[j]) : 0.f;
-          const float d = pm == 0.f ? 0.f : pm * (dp[e + j] - rrs[j]);
+          float pm = exp2_flush(NP == 3 ? (s[e + j] * p.scale2 - mxs[j]) - lls[j] : s[e + j] * p.scale2 - mxs[j]);
+          if (edge) pm = key < lis[j] ? pm : 0.f;
+          const float d = pm * (dp[e + j] - rrs[j]);
           if (m == 0) A[e + j] = pm;
           else A[e + j] = A[e + j] - las[j] * pm;
           ds[e + j] = m == 0 ? d : -las[j] * d;
         }
-        if (NP == 3) __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < (DK ? 2 : 0); ++c) {
         bf16x8 bo[NS];
         da_operand<NS>(&ds[8 * c], bo);
 #pragma unroll
@@ -777,12 +877,11 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dkv_k(DaP p) {
           bf16x8 a[NP];
           Tile::frag_col(Qt, m * DP + 32 * v + col, c, half, a);
           ak[m][v] = da_mfma<NP, NS>(a, bo, ak[m][v]);
-          if (NP == 3) __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < (DV ? 2 : 0); ++c) {
       bf16x8 bo[NS];
       da_operand<NS>(&A[8 * c], bo);
 #pragma unroll
@@ -790,21 +889,20 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dkv_k(DaP p) {
         bf16x8 a[NP];
         Tile::frag_col(Gt, 32 * v + col, c, half, a);
         av[v] = da_mfma<NP, NS>(a, bo, av[v]);
-        if (NP == 3) __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
   if (key >= p.Nk) return;
   const int64_t at = (((int64_t)b * p.Nk + key) * p.Hkv + hk) * 2 * p.D;
 #pragma unroll
-  for (int v = 0; v < VB; ++v)
+  for (int v = 0; v < (DV ? VB : 0); ++v)
 #pragma unroll
     for (int e = 0; e < 16; e += 4) {
       const int d = 32 * v + 2 * e + 4 * half;
       if (d < 2 * p.D) da_store4<NP>(p.dv, at + d, av[v][e], av[v][e + 1], av[v][e + 2], av[v][e + 3]);
     }
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+  for (int m = 0; m < (DK ? 2 : 0); ++m)
 #pragma unroll
     for (int v = 0; v < DB; ++v)
 #pragma unroll
@@ -818,31 +916,43 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dkv_k(DaP p) {
 
 // dlam[h] = -sum over clouds and queries of r_2 (one value for all heads: over the heads too); one workgroup per output, fixed order,
 // sums in double (a long sum of values of both signs)
-__global__ __launch_bounds__(256) void diff_attn_dlam_k(const float *__restrict__ r2, int B, int H, int Nq, int lam_n, float *__restrict__ dlam) {
-  __shared__ double part[4];
+__global__ __launch_bounds__(1024) void diff_attn_dlam_k(const float *__restrict__ r2, int B, int H, int Nq, int lam_n, float *__restrict__ dlam) {
+  __shared__ double part[16];
   double s = 0.0;
-  const int h0 = lam_n == 1 ? 0 : blockIdx.x, h1 = lam_n == 1 ? H : h0 + 1;
-  for (int b = 0; b < B; ++b)
-    for (int h = h0; h < h1; ++h)
-      for (int i = threadIdx.x; i < Nq; i += 256) s += (double)r2[((int64_t)b * H + h) * Nq + i];
+  const int heads = lam_n == 1 ? H : 1;
+  const int64_t n = (int64_t)B * heads * Nq;
+  for (int64_t at = threadIdx.x; at < n; at += 8192) {  // eight in flight
+    float x[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int64_t k = at + 1024 * u, bh = k < n ? k / Nq : 0;
+      x[u] = k < n ? r2[lam_n == 1 ? k : (bh * H + blockIdx.x) * Nq + (k - bh * Nq)] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s += (double)x[u];
+  }
   for (int m = 32; m >= 1; m >>= 1) s += __shfl_xor(s, m, HITADV_WAVE);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) dlam[blockIdx.x] = (float)-(((part[0] + part[1]) + part[2]) + part[3]);
+  if (threadIdx.x == 0) {
+    for (int u = 1; u < 16; ++u) s += part[u];
+    dlam[blockIdx.x] = (float)-s;
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
+constexpr int64_t DA_STRIDE = 1 << 24;
 struct DaPlan {
-  int nw, tiles, splits, chunk;
+  int pairs, tiles, splits, chunk;
 };
-// Few rows: workgroups of one wave and the keys split over enough of them to fill the chip; else four waves share a tile of keys.
+// Few rows: one pair of waves, the keys split over enough workgroups to fill the chip; else four pairs share a tile of keys.
 static DaPlan da_plan(int B, int Nq, int Nk, int H, int Hkv) {
   DaPlan pl;
   const int64_t rows = (int64_t)Nq * (H / Hkv), bh = (int64_t)B * Hkv;
-  pl.nw = rows <= 2 * DA_T ? 1 : 4;
-  pl.tiles = (int)((rows + DA_T * pl.nw - 1) / (DA_T * pl.nw));
-  const int64_t waves = bh * pl.tiles * pl.nw, want = (2048 + waves - 1) / waves, most = (Nk + 127) / 128;
-  int64_t s = waves >= 1024 ? 1 : want < most ? want : most;
+  pl.pairs = rows <= DA_T ? 1 : bh * ((rows + 4 * DA_T - 1) / (4 * DA_T)) < 512 ? 2 : 4;
+  pl.tiles = (int)((rows + DA_T * pl.pairs - 1) / (DA_T * pl.pairs));
+  const int64_t waves = bh * pl.tiles * pl.pairs * 2, want = (4096 + waves - 1) / waves, most = (Nk + 127) / 128;
+  int64_t s = waves >= 2048 ? 1 : want < most ? want : most;
   if (s < 1) s = 1;
   int64_t chunk = ((Nk + s - 1) / s + DA_T - 1) / DA_T * DA_T;
   if (chunk < DA_T) chunk = DA_T;
@@ -852,43 +962,49 @@ static DaPlan da_plan(int B, int Nq, int Nk, int H, int Hkv) {
   return pl;
 }
 
-template <int NP, int DP> static int da_launch_fwd(const DaP &p, const DaPlan &pl, hipStream_t s) {
-  const int lds = 2 * (DaTile<NP, DP>::ROWS + DaTile<NP, DP>::COLS);
+template <int NP, int DP, int PAIRS> static int da_launch_fwd_pairs(const DaP &p, const DaPlan &pl, hipStream_t s) {
+  const int tiles = 4 * (DaTile<NP, DP>::ROWS + DaTile<NP, DP>::COLS), parts = PAIRS * 4096;  // bytes
+  const int lds = tiles > parts ? tiles : parts;
   const dim3 grid(p.B * p.Hkv, pl.tiles, pl.splits);
-  if (pl.nw == 1 && pl.splits > 1) {
-    HITADV_RAISE_LDS((diff_attn_fwd_k<NP, DP, 1, true>), lds);
-    diff_attn_fwd_k<NP, DP, 1, true><<<grid, 64, lds, s>>>(p);
-  } else if (pl.nw == 1) {
-    HITADV_RAISE_LDS((diff_attn_fwd_k<NP, DP, 1, false>), lds);
-    diff_attn_fwd_k<NP, DP, 1, false><<<grid, 64, lds, s>>>(p);
-  } else if (pl.splits > 1) {
-    HITADV_RAISE_LDS((diff_attn_fwd_k<NP, DP, 4, true>), lds);
-    diff_attn_fwd_k<NP, DP, 4, true><<<grid, 256, lds, s>>>(p);
+  if (pl.splits > 1) {
+    HITADV_RAISE_LDS((diff_attn_fwd_k<NP, DP, PAIRS, true>), lds);
+    diff_attn_fwd_k<NP, DP, PAIRS, true><<<grid, 128 * PAIRS, lds, s>>>(p);
+    HITADV_LAUNCH_CHECK();
+    diff_attn_join_k<NP><<<dim3(p.rows, p.B * p.Hkv), 128, 0, s>>>(p);
   } else {
-    HITADV_RAISE_LDS((diff_attn_fwd_k<NP, DP, 4, false>), lds);
-    diff_attn_fwd_k<NP, DP, 4, false><<<grid, 256, lds, s>>>(p);
+    HITADV_RAISE_LDS((diff_attn_fwd_k<NP, DP, PAIRS, false>), lds);
+    diff_attn_fwd_k<NP, DP, PAIRS, false><<<grid, 128 * PAIRS, lds, s>>>(p);
   }
   HITADV_LAUNCH_CHECK();
-  if (pl.splits > 1) {
-    diff_attn_join_k<NP><<<dim3(p.rows, p.B * p.Hkv), 128, 0, s>>>(p);
-    HITADV_LAUNCH_CHECK();
-  }
   return 0;
 }
+template <int NP, int DP> static int da_launch_fwd(const DaP &p, const DaPlan &pl, hipStream_t s) {
+  return pl.pairs == 1 ? da_launch_fwd_pairs<NP, DP, 1>(p, pl, s)
+       : pl.pairs == 2 ? da_launch_fwd_pairs<NP, DP, 2>(p, pl, s) : da_launch_fwd_pairs<NP, DP, 4>(p, pl, s);
+}
 template <int NP, int DP> static int da_launch_bwd(const DaP &p, float *dlam, hipStream_t s) {
-  const int lds_q = 2 * (2 * DaTile<NP, DP>::ROWS + DaTile<NP, DP>::COLS);
-  const int lds_kv = 2 * (2 * DaTile<NP, DP>::ROWS + 2 * DaTile<NP, DP>::COLS) + 8 * DA_T * 4 + (NP == 3 && DP == 64 ? (2 * DP / 16 + 2) * 256 * 16 : 0);
+  const int lds_q = 2 * (2 * DaTile<NP, DP>::ROWS + DaTile<NP, DP>::COLS) + (NP != 3 ? 2 * DP / 16 * 256 * 16 : 0);
   const int tq = (p.rows + 4 * DA_T - 1) / (4 * DA_T), tk = (p.Nk + 4 * DA_T - 1) / (4 * DA_T);
   HITADV_RAISE_LDS((diff_attn_dq_k<NP, DP, 4>), lds_q);
   diff_attn_dq_k<NP, DP, 4><<<dim3(p.B * p.Hkv, tq), 256, lds_q, s>>>(p);
   HITADV_LAUNCH_CHECK();
   if (p.dk) {
-    HITADV_RAISE_LDS((diff_attn_dkv_k<NP, DP, 4>), lds_kv);
-    diff_attn_dkv_k<NP, DP, 4><<<dim3(p.B * p.Hkv, tk), 256, lds_kv, s>>>(p);
+    const dim3 grid(p.B * p.Hkv, tk);
+    constexpr int R = 2 * DaTile<NP, DP>::ROWS, C = 2 * DaTile<NP, DP>::COLS, ST = 8 * DA_T * 4;  // bytes
+    if constexpr (NP == 3 && DP == 64) {
+      HITADV_RAISE_LDS((diff_attn_dkv_k<NP, DP, 4, true, false>), R + C + ST);
+      diff_attn_dkv_k<NP, DP, 4, true, false><<<grid, 256, R + C + ST, s>>>(p);
+      HITADV_LAUNCH_CHECK();
+      HITADV_RAISE_LDS((diff_attn_dkv_k<NP, DP, 4, false, true>), 2 * R + C + ST);
+      diff_attn_dkv_k<NP, DP, 4, false, true><<<grid, 256, 2 * R + C + ST, s>>>(p);
+    } else {
+      HITADV_RAISE_LDS((diff_attn_dkv_k<NP, DP, 4, true, true>), 2 * (R + C) + ST);
+      diff_attn_dkv_k<NP, DP, 4, true, true><<<grid, 256, 2 * (R + C) + ST, s>>>(p);
+    }
     HITADV_LAUNCH_CHECK();
   }
   if (dlam) {
-    diff_attn_dlam_k<<<p.lam_n, 256, 0, s>>>(p.r + (int64_t)p.B * p.H * p.Nq, p.B, p.H, p.Nq, p.lam_n, dlam);
+    diff_attn_dlam_k<<<p.lam_n, 1024, 0, s>>>(p.r + (int64_t)p.B * p.H * p.Nq, p.B, p.H, p.Nq, p.lam_n, dlam);
     HITADV_LAUNCH_CHECK();
   }
   return 0;
@@ -916,7 +1032,8 @@ static bool da_strides_ok(int dtype, const void *q, const void *k, const void *v
   if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & 15) return false;
   for (int i = 0; i < 11; ++i)
     if (st[i] < 0 || st[i] % (dtype == 0 ? 4 : 8)) return false;
-  return true;
+  // a tile's 32 rows and its two maps are addressed with 32 bits
+  return st[1] < DA_STRIDE && st[3] < DA_STRIDE && st[5] < DA_STRIDE && st[7] < DA_STRIDE && st[9] < DA_STRIDE;
 }
 
 }  // namespace hitadv

@@ -237,20 +237,23 @@ __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void rms_norm_bwd_k(RnP p)
   }
 }
 
-// dw[c] = sum of the workgroups' shares: 16 columns x 16 slices a workgroup
+// dw[c] = sum of the workgroups' shares: 8 columns x 32 slices a workgroup, eight shares of a slice in flight
 template <int TW>
 __global__ __launch_bounds__(256) void rms_norm_dw_k(const float *__restrict__ part, int n, int cols, void *__restrict__ dw) {
-  __shared__ float s[16][17];
-  const int cl = threadIdx.x & 15, sl = threadIdx.x >> 4, c = blockIdx.x * 16 + cl;
+  __shared__ float s[32][9];
+  const int cl = threadIdx.x & 7, sl = threadIdx.x >> 3, c = blockIdx.x * 8 + cl;
   float t = 0.f;
-  if (c < cols)
-#pragma clang loop vectorize(disable)
-    for (int i = sl; i < n; i += 16) t += part[(int64_t)i * cols + c];
+  for (int i = sl; i < n; i += 256) {
+    float x[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) x[u] = c < cols && i + 32 * u < n ? part[(int64_t)(i + 32 * u) * cols + c] : 0.f;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) t += x[u];
+  }
   s[sl][cl] = t;
   __syncthreads();
   if (sl == 0 && c < cols) {
-#pragma unroll
-    for (int i = 1; i < 16; ++i) t += s[i][cl];
+    for (int i = 1; i < 32; ++i) t += s[i][cl];
     elem_store<TW>(dw, c, t);
   }
 }
@@ -346,7 +349,7 @@ extern "C" int hitadv_rms_norm_bwd(int dtype, int wtype, const void *s, const vo
   hipStream_t st = (hipStream_t)stream;
   const int rc = rn_run(p, dtype, 2, st);
   if (rc != 0 || !dw) return rc;
-  const unsigned g = (unsigned)((cols + 15) / 16);
+  const unsigned g = (unsigned)((cols + 7) / 8);
   const int n = rn_bwd_blocks(rows, cols);
   if (wtype == ELEM_F32) rms_norm_dw_k<ELEM_F32><<<g, 256, 0, st>>>(scratch, n, cols, dw);
   else if (wtype == ELEM_BF16) rms_norm_dw_k<ELEM_BF16><<<g, 256, 0, st>>>(scratch, n, cols, dw);

@@ -1192,10 +1192,11 @@ def _aligned(t):
 
 
 def _strided(t):
-    """(``t`` or a contiguous copy, its strides): last axis contiguous, 16-byte aligned rows -- views of a cache are taken as they are."""
+    """(``t`` or a contiguous copy, its strides): last axis contiguous, 16-byte aligned rows -- views of a cache are taken as they are (rows
+    2^24 elements apart and more are copied: the kernels address a tile's rows with 32 bits)."""
     unit = 16 // t.element_size()
     strides = [0 if n == 1 else s for n, s in zip(t.shape, t.stride())]
-    if (t.stride(-1) != 1 and t.shape[-1] != 1) or t.data_ptr() % 16 or any(s % unit for s in strides[:-1]):
+    if (t.stride(-1) != 1 and t.shape[-1] != 1) or t.data_ptr() % 16 or any(s % unit for s in strides[:-1]) or max([strides[1]] + strides[3:-1]) >= 2 ** 24:
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()

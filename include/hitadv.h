@@ -676,7 +676,8 @@ int hitadv_row_sqnorm(const float *X, int64_t rows, int D, float *xx, void *stre
 /* Differential attention: out[b,i,h] = sum_j (P1 - lam[h] P2)[i,j] v[b,j,h / G], P_m = softmax over the visible j of
  * scale q[b,i,h,m] . k[b,j,h / G,m], m = 1, 2; G = H / Hkv query heads share a key / value head.
  *   q [B,Nq,H,2,D], k [B,Nk,Hkv,2,D], v [B,Nk,Hkv,2D] in dtype, any strides (elements, HOST array `strides`: q's for b, query, head, map;
- *   k's for b, key, head, map; v's for b, key, head), the last axis contiguous, bases 16-byte aligned, strides multiples of 16 bytes;
+ *   k's for b, key, head, map; v's for b, key, head), the last axis contiguous, bases 16-byte aligned, strides multiples of 16 bytes, those of
+ *   queries, keys and maps below 2^24;
  *   lam fp32 [H], or one value for all heads (lam_n = H or 1); lengths int32 [B] or NULL (device): key j is visible below lengths[b]
  *   (clamped to 0 .. Nk; what lies behind it is not used, whatever it holds); causal: also only at j <= i + Nk - Nq.
  *   out [B,Nq,H,2D] dtype, contiguous, 16-byte aligned; a row that sees no key is 0.
