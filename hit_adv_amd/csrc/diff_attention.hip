@@ -257,97 +257,100 @@ template <int NP, int DP> struct DaTile {
 // What a workgroup of NT threads fetches of the next tile while it computes on this one: raw elements in registers.  A thread's column is
 // the same in all its pieces; an address is a wave-uniform base plus a 32-bit offset of the thread (strides below 2^24 elements: the entry
 // points see to it).  Threads whose column is padding (D < DP) fetch and store nothing: their cells of the tile are zeroed once.
-template <int NP, int DP> struct DaFetch {
-  static constexpr int ES = NP == 3 ? 4 : 2;  // bytes of an element
-  int row, col;
-  uint32_t off;  // bytes
-  bool there;
-  __device__ __forceinline__ void bind_at(int row_, int col_, bool inside, int64_t n, int64_t m, int D, bool maps) {
-    row = row_;
-    col = col_;
-    const int map = maps && col >= DP ? 1 : 0, d = col - map * DP;
-    there = inside && d < (maps ? D : 2 * D);
-    off = (uint32_t)(row * (int)n + map * (int)m + d) * ES;
-  }
-};
-template <int NP, int DP, int NT> struct DaFetchRows : DaFetch<NP, DP> {  // 16-byte (32-byte) pieces of 32 rows of k, v
-  static constexpr int CH = 2 * DP / 8, STEP = NT / CH, C = STEP >= DA_T ? 1 : DA_T / STEP;
-  using F = DaFetch<NP, DP>;
+template <int NP> constexpr int DA_ES = NP == 3 ? 4 : 2;  // bytes of an element
+// byte offset of a row's column of the padded [2][DP] (maps) or [2 DP] columns; false: padding
+template <int NP, int DP> __device__ __forceinline__ bool da_bind(int row, int col, int64_t n, int64_t m, int D, bool maps, uint32_t &off) {
+  const int map = maps && col >= DP ? 1 : 0, d = col - map * DP;
+  off = (uint32_t)(row * (int)n + map * (int)m + d) * DA_ES<NP>;
+  return d < (maps ? D : 2 * D);
+}
+template <int NP, int DP, int NT> struct DaFetchRows {  // 16-byte (32-byte) pieces of 32 rows of k, v
+  static constexpr int CH = 2 * DP / 8, STEP = NT / CH, C = STEP >= DA_T ? 1 : DA_T / STEP, ES = DA_ES<NP>;
   Raw8<NP> x[C];
-  __device__ __forceinline__ void bind(int64_t n, int64_t m, int D, bool maps, int tid) { F::bind_at(tid / CH, 8 * (tid % CH), tid / CH < DA_T, n, m, D, maps); }
+  int row, col;
+  uint32_t off;
+  bool there;
+  __device__ __forceinline__ void bind(int64_t n, int64_t m, int D, bool maps, int tid) {
+    row = tid / CH;
+    col = 8 * (tid % CH);
+    there = da_bind<NP, DP>(row, col, n, m, D, maps, off) && row < DA_T;
+  }
   // rows t .. t + 31 of the rows at `base` (elements, wave-uniform); `end`: the first row that does not exist (zeros from there on)
   __device__ __forceinline__ void load(const void *src, int64_t base, int64_t n, int t, int end) {
-    if (!F::there) return;
-    const char *at = (const char *)src + (base + t * n) * F::ES;
+    if (!there) return;
+    const char *at = (const char *)src + (base + t * n) * ES;
     if (t + DA_T <= end) {
 #pragma unroll
-      for (int c = 0; c < C; ++c) x[c] = da_load8<NP>(at + c * STEP * n * F::ES + F::off, 0, true);
+      for (int c = 0; c < C; ++c) x[c] = da_load8<NP>(at + c * STEP * n * ES + off, 0, true);
     } else {
 #pragma unroll
-      for (int c = 0; c < C; ++c) x[c] = da_load8<NP>(at + c * STEP * n * F::ES + F::off, 0, t + c * STEP + F::row < end);
+      for (int c = 0; c < C; ++c) x[c] = da_load8<NP>(at + c * STEP * n * ES + off, 0, t + c * STEP + row < end);
     }
   }
   __device__ __forceinline__ void put(uint16_t *rows) const {
-    if (!F::there) return;
+    if (!there) return;
 #pragma unroll
-    for (int c = 0; c < C; ++c) DaTile<NP, DP>::put_row(rows, F::row + c * STEP, F::col, x[c]);
+    for (int c = 0; c < C; ++c) DaTile<NP, DP>::put_row(rows, row + c * STEP, col, x[c]);
   }
   __device__ __forceinline__ void zero_padding(uint16_t *rows) const {
-    if (F::there || F::row >= DA_T) return;
+    if (there || row >= DA_T) return;
 #pragma unroll
-    for (int c = 0; c < C; ++c) DaTile<NP, DP>::put_row(rows, F::row + c * STEP, F::col, da_load8<NP>(nullptr, 0, false));
+    for (int c = 0; c < C; ++c) DaTile<NP, DP>::put_row(rows, row + c * STEP, col, da_load8<NP>(nullptr, 0, false));
   }
 };
-template <int NP, int DP, int NT> struct DaFetchBlocks : DaFetch<NP, DP> {  // 4 x 4 blocks, for a transposed tile, or both
-  static constexpr int CH = 2 * DP / 4, STEP = NT / CH, C = STEP >= 8 ? 1 : 8 / STEP;
-  using F = DaFetch<NP, DP>;
+// 4 x 4 blocks, for a transposed tile, or both.  Lanes: four row groups, then sixteen column groups.  Four lanes write 32 consecutive bytes of
+// a transposed row and the next four 16 banks on (columns in neighbouring lanes: eight on one bank); a wave still fetches 128 (256) bytes
+// of every row (eight row groups: 64, and the backward kernels 10 % slower).
+template <int NP, int DP, int NT> struct DaFetchBlocks {
+  static constexpr int CH = 2 * DP / 4, STEP = NT / 8, C = STEP >= CH ? 1 : CH / STEP, ES = DA_ES<NP>;
   Raw4<NP> x[C][4];
+  int row, col;
+  uint32_t off[C];
+  bool there[C];
   __device__ __forceinline__ void bind(int64_t n, int64_t m, int D, bool maps, int tid) {
-    F::bind_at(4 * (tid / CH), 4 * (tid % CH), tid / CH < 8, n, m, D, maps);
+    row = 4 * ((tid & 3) | ((tid >> 4) & 4));
+    col = 4 * (((tid >> 2) & 15) | ((tid >> 7) << 4));
+#pragma unroll
+    for (int c = 0; c < C; ++c) there[c] = da_bind<NP, DP>(row, col + 4 * c * STEP, n, m, D, maps, off[c]) && col < 2 * DP;
   }
   __device__ __forceinline__ void load(const void *src, int64_t base, int64_t n, int t, int end) {
-    if (!F::there) return;
-    const char *at = (const char *)src + (base + t * n) * F::ES;
-    if (t + DA_T <= end) {
+    const char *at = (const char *)src + (base + t * n) * ES;
 #pragma unroll
-      for (int c = 0; c < C; ++c)
+    for (int c = 0; c < C; ++c) {
+      if (!there[c]) continue;
+      if (t + DA_T <= end) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[c][i] = da_load4<NP>(at + (4 * c * STEP + i) * n * F::ES + F::off, 0, true);
-    } else {
+        for (int i = 0; i < 4; ++i) x[c][i] = da_load4<NP>(at + i * n * ES + off[c], 0, true);
+      } else {
 #pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          x[c][i] = da_load4<NP>(at + (4 * c * STEP + i) * n * F::ES + F::off, 0, t + F::row + 4 * c * STEP + i < end);
+        for (int i = 0; i < 4; ++i) x[c][i] = da_load4<NP>(at + i * n * ES + off[c], 0, t + row + i < end);
+      }
     }
   }
   // packed query rows: row r is query r / G, head r % G
   __device__ __forceinline__ void load_packed(const void *src, int64_t base, int64_t n, int64_t h, const DaP &p, int t) {
     if (p.G == 1) return load(src, base, n, t, p.rows);
-    if (!F::there) return;
-    const char *at = (const char *)src + base * F::ES + (F::off - (uint32_t)(F::row * (int)n) * F::ES);
 #pragma unroll
-    for (int c = 0; c < C; ++c)
+    for (int i = 0; i < 4; ++i) {
+      const int r = t + row + i, q = da_div_g(p, r);
+      const char *at = (const char *)src + (base + q * n + (r - q * p.G) * h) * ES;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = t + F::row + 4 * c * STEP + i, q = da_div_g(p, r);
-        x[c][i] = da_load4<NP>(at, q * n + (r - q * p.G) * h, r < p.rows);
-      }
+      for (int c = 0; c < C; ++c)
+        if (there[c]) x[c][i] = da_load4<NP>(at + (off[c] - (uint32_t)(row * (int)n) * ES), 0, r < p.rows);
+    }
   }
   template <bool ROWS, bool COLS> __device__ __forceinline__ void put(uint16_t *rows, uint16_t *cols) const {
-    if (!F::there) return;
 #pragma unroll
-    for (int c = 0; c < C; ++c) DaTile<NP, DP>::template put_block<ROWS, COLS>(rows, cols, F::row / 4 + c * STEP, F::col, x[c]);
+    for (int c = 0; c < C; ++c)
+      if (there[c]) DaTile<NP, DP>::template put_block<ROWS, COLS>(rows, cols, row / 4, col + 4 * c * STEP, x[c]);
   }
   template <bool ROWS, bool COLS> __device__ __forceinline__ void zero_padding(uint16_t *rows, uint16_t *cols) {
-    if (F::there || F::row >= DA_T) return;
+    Raw4<NP> z[4];
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      Raw4<NP> z[4];
+    for (int i = 0; i < 4; ++i) z[i] = da_load4<NP>(nullptr, 0, false);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) z[i] = da_load4<NP>(nullptr, 0, false);
-      DaTile<NP, DP>::template put_block<ROWS, COLS>(rows, cols, F::row / 4 + c * STEP, F::col, z);
-    }
+    for (int c = 0; c < C; ++c)
+      if (!there[c] && col < 2 * DP) DaTile<NP, DP>::template put_block<ROWS, COLS>(rows, cols, row / 4, col + 4 * c * STEP, z);
   }
 };
 
@@ -376,7 +379,7 @@ __device__ __forceinline__ int da_wave_id() { return __builtin_amdgcn_readfirstl
 // maps fills the registers), and the difference is taken once, at the end, through LDS.  The next tile's elements are on their way in
 // registers while this one's are multiplied; two buffers, one barrier a tile.
 template <int NP, int DP, int PAIRS, bool SPLIT>
-__global__ __launch_bounds__(128 * PAIRS, 2) void diff_attn_fwd_k(DaP p) {
+__global__ __launch_bounds__(128 * PAIRS, (NP == 3 && DP == 64 && PAIRS == 1 ? 1 : 2)) void diff_attn_fwd_k(DaP p) {
   using Tile = DaTile<NP, DP>;
   constexpr int NR = DA_NR<NP>, NT = 128 * PAIRS;
   constexpr int NPP = NP == 3 ? 3 : 2;  // pieces of a probability
@@ -538,43 +541,59 @@ __global__ __launch_bounds__(128 * PAIRS, 2) void diff_attn_fwd_k(DaP p) {
   }
 }
 
-// joins the splits of a row: thread = value column
+// joins the splits of a row: waves 0 and 1 weigh a map's splits each, then a thread has a (map, value column), eight splits in flight
+constexpr int DA_MAX_SPLITS = 1024;
 template <int NP>
-__global__ __launch_bounds__(128) void diff_attn_join_k(DaP p) {
-  const int r = blockIdx.x, bh = blockIdx.y, d = threadIdx.x;
+__global__ __launch_bounds__(256) void diff_attn_join_k(DaP p) {
+  __shared__ float weight[2][DA_MAX_SPLITS], total[2], other[128];
+  const int r = blockIdx.x, bh = blockIdx.y, lane = threadIdx.x & 63, wave = da_wave_id();
   const int b = bh / p.Hkv, hk = bh % p.Hkv, i = da_div_g(p, r), h = hk * p.G + r - i * p.G;
   const int64_t step = (int64_t)p.B * p.Hkv * p.rows, row = (int64_t)bh * p.rows + r;
-  float mx[2] = {-DA_INF, -DA_INF};
-  for (int s = 0; s < p.splits; ++s) {
-    const float4 ml = *(const float4 *)(p.part_ml + 4 * (row + s * step));
-    mx[0] = fmaxf(mx[0], ml.x);
-    mx[1] = fmaxf(mx[1], ml.z);
-  }
-  const float b0 = mx[0] == -DA_INF ? 0.f : mx[0], b1 = mx[1] == -DA_INF ? 0.f : mx[1];
-  float sum[2] = {0.f, 0.f}, o[2] = {0.f, 0.f};
-  for (int s = 0; s < p.splits; ++s) {
-    const float4 ml = *(const float4 *)(p.part_ml + 4 * (row + s * step));
-    const float w0 = exp2_flush(ml.x - b0), w1 = exp2_flush(ml.z - b1);  // a split that saw nothing: 2^-inf = 0
-    sum[0] += ml.y * w0;
-    sum[1] += ml.w * w1;
-    if (d < 2 * p.D) {
-      const float *po = p.part_o + (row + s * step) * 4 * p.D;
-      o[0] += po[d] * w0;
-      o[1] += po[2 * p.D + d] * w1;
+  if (wave < 2) {
+    float mx = -DA_INF, sum = 0.f;
+    for (int s = lane; s < p.splits; s += 64) mx = fmaxf(mx, p.part_ml[4 * (row + s * step) + 2 * wave]);
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) mx = fmaxf(mx, __shfl_xor(mx, d, HITADV_WAVE));
+    const float base = mx == -DA_INF ? 0.f : mx;
+    for (int s = lane; s < p.splits; s += 64) {
+      const float2 ml = *(const float2 *)(p.part_ml + 4 * (row + s * step) + 2 * wave);
+      const float w = exp2_flush(ml.x - base);  // a split that saw nothing: 2^-inf = 0
+      weight[wave][s] = w;
+      sum += ml.y * w;
+    }
+    sum = wave_sum(sum);
+    if (lane == 0) {
+      total[wave] = sum == 0.f ? 0.f : (wave ? -da_lam(p, h) : 1.f) / sum;
+      if (p.stats) {
+        const int64_t n = (int64_t)p.B * p.H * p.Nq, srow = ((int64_t)b * p.H + h) * p.Nq + i;
+        p.stats[(2 * wave) * n + srow] = sum == 0.f ? 0.f : mx;
+        p.stats[(2 * wave + 1) * n + srow] = sum == 0.f ? DA_INF : log2f(sum);
+      }
     }
   }
+  __syncthreads();
+  const int m = threadIdx.x >> 7, d = threadIdx.x & 127;
+  float o = 0.f;
   if (d < 2 * p.D) {
-    const float w0 = sum[0] == 0.f ? 0.f : 1.f / sum[0], w1 = sum[1] == 0.f ? 0.f : -da_lam(p, h) / sum[1];
-    const float x = o[0] * w0 + o[1] * w1;
+    const float *po = p.part_o + (2 * row + m) * 2 * p.D + d;
+    const int64_t st = step * 4 * p.D;
+    for (int s = 0; s < p.splits; s += 8) {
+      float x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) x[u] = s + u < p.splits ? po[(s + u) * st] : 0.f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) o += s + u < p.splits ? x[u] * weight[m][s + u] : 0.f;
+    }
+    o *= total[m];
+  }
+  if (m) other[d] = o;
+  __syncthreads();
+  if (!m && d < 2 * p.D) {
+    const float x = o + other[d];
     const int64_t at = (((int64_t)b * p.Nq + i) * p.H + h) * 2 * p.D + d;
     if constexpr (NP == 3) ((float *)p.out)[at] = x;
     else if constexpr (NP == 2) ((_Float16 *)p.out)[at] = (_Float16)x;
     else ((uint16_t *)p.out)[at] = (uint16_t)(bf16_pair(x, 0.f) & 0xffffu);
-  }
-  if (p.stats && d < 2) {
-    const int64_t n = (int64_t)p.B * p.H * p.Nq, srow = ((int64_t)b * p.H + h) * p.Nq + i;
-    p.stats[(2 * d) * n + srow] = sum[d] == 0.f ? 0.f : mx[d];
-    p.stats[(2 * d + 1) * n + srow] = sum[d] == 0.f ? DA_INF : log2f(sum[d]);
   }
 }
 
@@ -951,9 +970,10 @@ static DaPlan da_plan(int B, int Nq, int Nk, int H, int Hkv) {
   const int64_t rows = (int64_t)Nq * (H / Hkv), bh = (int64_t)B * Hkv;
   pl.pairs = rows <= DA_T ? 1 : bh * ((rows + 4 * DA_T - 1) / (4 * DA_T)) < 512 ? 2 : 4;
   pl.tiles = (int)((rows + DA_T * pl.pairs - 1) / (DA_T * pl.pairs));
-  const int64_t waves = bh * pl.tiles * pl.pairs * 2, want = (4096 + waves - 1) / waves, most = (Nk + 127) / 128;
+  const int64_t waves = bh * pl.tiles * pl.pairs * 2, want = (4096 + waves - 1) / waves, most = (Nk + 255) / 256;
   int64_t s = waves >= 2048 ? 1 : want < most ? want : most;
   if (s < 1) s = 1;
+  if (s > DA_MAX_SPLITS) s = DA_MAX_SPLITS;
   int64_t chunk = ((Nk + s - 1) / s + DA_T - 1) / DA_T * DA_T;
   if (chunk < DA_T) chunk = DA_T;
   pl.chunk = (int)chunk;
@@ -970,7 +990,7 @@ template <int NP, int DP, int PAIRS> static int da_launch_fwd_pairs(const DaP &p
     HITADV_RAISE_LDS((diff_attn_fwd_k<NP, DP, PAIRS, true>), lds);
     diff_attn_fwd_k<NP, DP, PAIRS, true><<<grid, 128 * PAIRS, lds, s>>>(p);
     HITADV_LAUNCH_CHECK();
-    diff_attn_join_k<NP><<<dim3(p.rows, p.B * p.Hkv), 128, 0, s>>>(p);
+    diff_attn_join_k<NP><<<dim3(p.rows, p.B * p.Hkv), 256, 0, s>>>(p);
   } else {
     HITADV_RAISE_LDS((diff_attn_fwd_k<NP, DP, PAIRS, false>), lds);
     diff_attn_fwd_k<NP, DP, PAIRS, false><<<grid, 128 * PAIRS, lds, s>>>(p);
