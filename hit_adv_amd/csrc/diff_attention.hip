@@ -23,6 +23,8 @@
 #include "elements.hpp"
 #include "hitadv.h"
 
+#include <type_traits>
+
 namespace hitadv {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -45,7 +47,8 @@ struct DaP {
   int64_t q_b, q_n, q_h, q_m, k_b, k_n, k_h, k_m, v_b, v_n, v_h;
   int B, Nq, Nk, H, Hkv, D, G, lam_n, causal, rows, chunk, splits;
   uint32_t g_magic;      // ceil(2^32 / G), G > 1
-  float scale, scale2;   // scale, scale * log2(e)
+  float scale, scale2;   // scale, |scale| log2(e) (1 if scale is 0)
+  uint32_t s_and, s_xor; // what makes one operand of the scores carry the scale's sign (or its zero): its elements' words and, xor these
 };
 
 __device__ __forceinline__ int da_div_g(const DaP &p, int r) { return p.G == 1 ? r : (int)(((uint64_t)(uint32_t)r * p.g_magic) >> 32); }
@@ -116,6 +119,12 @@ template <int NP> __device__ __forceinline__ void da_pieces8(const Raw8<NP> &r, 
     for (int k = 0; k < 3; ++k)
       out[k] = make_uint4(pack_hi(p[0][k], p[1][k]), pack_hi(p[2][k], p[3][k]), pack_hi(p[4][k], p[5][k]), pack_hi(p[6][k], p[7][k]));
   }
+}
+// a score's operand with the scale's sign (pieces are 16-bit values of either format: two to a word)
+template <int N> __device__ __forceinline__ void da_sign(uint4 (&w)[N], const DaP &p) {
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    w[k] = make_uint4((w[k].x & p.s_and) ^ p.s_xor, (w[k].y & p.s_and) ^ p.s_xor, (w[k].z & p.s_and) ^ p.s_xor, (w[k].w & p.s_and) ^ p.s_xor);
 }
 // the pieces of four rows of four values, [row][column][piece]
 template <int NP> __device__ __forceinline__ void da_pieces4x4(const Raw4<NP> (&r)[4], uint32_t (&p)[4][4][NP]) {
@@ -405,6 +414,7 @@ __global__ __launch_bounds__(128 * PAIRS, (NP == 3 && DP == 64 && PAIRS == 1 ? 1
       const int d = 16 * c + 8 * half;
       uint4 w[NR];
       da_pieces8<NP>(da_load8<NP>(p.q, b * p.q_b + i * p.q_n + h * p.q_h + m * p.q_m + d, r < p.rows && d < p.D), w);
+      da_sign(w, p);
 #pragma unroll
       for (int k = 0; k < NR; ++k) qf[c][k] = as_bf16x8(w[k]);
     }
@@ -447,17 +457,15 @@ __global__ __launch_bounds__(128 * PAIRS, (NP == 3 && DP == 64 && PAIRS == 1 ? 1
         s = da_mfma_in<NP, false>(a, qf[c], s);
       }
       float pr[16];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) pr[e] = s[e] * p.scale2;
       if (t + DA_T > lim_lo) {
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (t + 8 * (e >> 2) + 4 * half + (e & 3) >= lim) pr[e] = -DA_INF;
+          if (t + 8 * (e >> 2) + 4 * half + (e & 3) >= lim) s[e] = -DA_INF;
       }
-      float top = pr[0];
+      float top = s[0];
 #pragma unroll
-      for (int e = 1; e < 16; ++e) top = fmaxf(top, pr[e]);
-      top = fmaxf(top, __shfl_xor(top, 32, HITADV_WAVE));
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
+      top = fmaxf(top, __shfl_xor(top, 32, HITADV_WAVE)) * p.scale2;
       if (__ballot(top > mx + DA_SLACK) != 0ull) {  // (-inf + slack = -inf: the first visible key raises it)
         const float nm = fmaxf(mx, top);
         const float f = nm == -DA_INF ? 1.f : exp2_flush(mx - nm);
@@ -471,7 +479,7 @@ __global__ __launch_bounds__(128 * PAIRS, (NP == 3 && DP == 64 && PAIRS == 1 ? 1
       const float base = mx == -DA_INF ? 0.f : mx;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        pr[e] = exp2_flush(pr[e] - base);
+        pr[e] = exp2_flush(__builtin_fmaf(s[e], p.scale2, -base));
         sum += pr[e];
       }
 #pragma unroll
@@ -601,19 +609,17 @@ __global__ __launch_bounds__(256) void diff_attn_join_k(DaP p) {
 // dP = dO V^T;  r_m = sum_j P_m dP;  dS_1 = P_1 (dP - r_1), dS_2 = -lam P_2 (dP - r_2).  The r are sums over the very P and dP that the
 // second pass multiplies (not dO . out: out is rounded, and where a row sees one key dS has to vanish exactly).
 //
-// dQ: the forward kernel's layout, two passes over the keys: first r, then dQ_m^T = K_m^T dS_m^T.
-template <int NP, int DP> constexpr int DA_DQ_WAVES = NP == 3 ? 1 : 2;  // waves per SIMD: what the registers allow
+// dQ: the forward kernel's layout, two passes over the keys: first r, then dQ_m^T = K_m^T dS_m^T.  Matrix and vector instructions of a SIMD do
+// not overlap here, so what costs is waiting: a phase's LDS operands are fetched together, ahead of it, into the registers that one wave
+// per SIMD has (two waves with 256 registers and single fetches: 534 us where this takes ~).
 template <int NP, int DP, int NW>
-__global__ __launch_bounds__(64 * NW, (DA_DQ_WAVES<NP, DP>)) void diff_attn_dq_k(DaP p) {
+__global__ __launch_bounds__(64 * NW) void diff_attn_dq_k(DaP p) {
   using Tile = DaTile<NP, DP>;
   constexpr int NR = DA_NR<NP>;
   constexpr int NS = NP == 3 ? 3 : 2;  // pieces of dS
   constexpr int KC = DP / 16, VC = 2 * DP / 16, DB = DP / 32;
   extern __shared__ __attribute__((aligned(16))) uint16_t da_lds[];
   uint16_t *Ks = da_lds, *Vs = da_lds + Tile::ROWS, *Kt = da_lds + 2 * Tile::ROWS;
-  // 16-bit types: dO's operands are parked in LDS, read back by the lane that wrote them -- two waves per SIMD (256 registers)
-  constexpr bool PARK = NP != 3;
-  uint4 *parked = (uint4 *)(Kt + Tile::COLS) + threadIdx.x;
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = da_wave_id(), tid = threadIdx.x;
   const int b = blockIdx.x / p.Hkv, hk = blockIdx.x % p.Hkv;
   const int tile = p.causal ? (int)(gridDim.y - 1 - blockIdx.y) : (int)blockIdx.y;
@@ -633,6 +639,7 @@ __global__ __launch_bounds__(64 * NW, (DA_DQ_WAVES<NP, DP>)) void diff_attn_dq_k
       const int d = 16 * c + 8 * half;
       uint4 w[NR];
       da_pieces8<NP>(da_load8<NP>(p.q, b * p.q_b + i * p.q_n + h * p.q_h + m * p.q_m + d, valid && d < p.D), w);
+      da_sign(w, p);
 #pragma unroll
       for (int k = 0; k < NR; ++k) qf[m][c][k] = as_bf16x8(w[k]);
     }
@@ -643,9 +650,8 @@ __global__ __launch_bounds__(64 * NW, (DA_DQ_WAVES<NP, DP>)) void diff_attn_dq_k
     da_pieces8<NP>(da_load8<NP>(p.dout, (((int64_t)b * p.Nq + i) * p.H + h) * 2 * p.D + d, valid && d < 2 * p.D), w);
 #pragma unroll
     for (int k = 0; k < NR; ++k) gf[c][k] = as_bf16x8(w[k]);
-    if (PARK) parked[c * 64 * NW] = w[0];
   }
-  float mx[2], ll[2], rs[2] = {0.f, 0.f};
+  float mx[2], ll[2], rs[2] = {0.f, 0.f}, only = 0.f;
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     mx[m] = valid ? p.stats[(2 * m) * n + srow] : 0.f;
@@ -669,77 +675,99 @@ __global__ __launch_bounds__(64 * NW, (DA_DQ_WAVES<NP, DP>)) void diff_attn_dq_k
     fk.load(p.k, k_at, p.k_n, 0, len);
     fv.load(p.v, v_at, p.v_n, 0, len);
   }
-#pragma unroll 1
-  for (int pass = 0; pass < 2; ++pass) {
+  constexpr bool AHEAD = NP != 3 || DP == 32;  // (three pieces at DP = 64: no registers left for it)
+  auto sweep = [&](auto second) {
+    constexpr bool SECOND = decltype(second)::value;
 #pragma unroll 1
     for (int t = 0; t < last; t += DA_T) {
       __syncthreads();
       fv.put(Vs);
-      if (pass) fk.template put<true, true>(Ks, Kt);
-      else fk.template put<true, false>(Ks, nullptr);
+      fk.template put<true, SECOND>(Ks, Kt);
       __syncthreads();
       const int next = t + DA_T < last ? t + DA_T : 0;  // (behind the second pass: the first tile once more, not used)
       fk.load(p.k, k_at, p.k_n, next, len);
       fv.load(p.v, v_at, p.v_n, next, len);
       if (t >= lim_hi) continue;
-      f32x16 dp = da_zero16(), small = da_zero16();
+      bf16x8 va[VC][NR], ka[2][KC][NR];
+      if (AHEAD) {
+#pragma unroll
+        for (int c = 0; c < VC; ++c) Tile::frag_row(Vs, col, 16 * c + 8 * half, va[c]);
+#pragma unroll
+        for (int c = 0; c < 2 * KC; ++c) Tile::frag_row(Ks, col, (c & 1) * DP + 16 * (c >> 1) + 8 * half, ka[c & 1][c >> 1]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      f32x16 dp = da_zero16(), small = da_zero16(), s[2] = {da_zero16(), da_zero16()};
 #pragma unroll
       for (int c = 0; c < VC; ++c) {
-        bf16x8 a[NR];
-        Tile::frag_row(Vs, col, 16 * c + 8 * half, a);
-        if constexpr (PARK) {
-          const bf16x8 g[1] = {as_bf16x8(parked[c * 64 * NW])};
-          dp = da_mfma_in<NP, false>(a, g, dp);
-        } else {
-          da_mfma_in2<NP, false>(a, gf[c], dp, small);
+        if (!AHEAD) Tile::frag_row(Vs, col, 16 * c + 8 * half, va[c]);
+        da_mfma_in2<NP, false>(va[c], gf[c], dp, small);
+        if (c & 1) {
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            if (!AHEAD) Tile::frag_row(Ks, col, m * DP + 16 * (c >> 1) + 8 * half, ka[m][c >> 1]);
+            s[m] = da_mfma_in<NP, false>(ka[m][c >> 1], qf[m][c >> 1], s[m]);
+          }
         }
+      }
+      bf16x8 kt[SECOND ? 2 : 1][2][DB][NP];
+      if (AHEAD && SECOND) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int v = 0; v < DB; ++v) Tile::frag_col(Kt, m * DP + 32 * v + col, c, half, kt[m][c][v]);
+        __builtin_amdgcn_sched_barrier(0);
       }
       if (NP == 3) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) dp[e] += small[e];
       }
+      if (!SECOND && t == 0) only = dp[0];
+      float pr[2][16];
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float x = __builtin_fmaf(s[m][e], p.scale2, -mx[m]);
+          pr[m][e] = exp2_flush(NP == 3 ? x - ll[m] : x);
+        }
+      if (t + DA_T > lim_lo) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (t + 8 * (e >> 2) + 4 * half + (e & 3) >= lim) pr[0][e] = pr[1][e] = 0.f;
+      }
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        f32x16 s = da_zero16();
+        if constexpr (!SECOND) {
 #pragma unroll
-        for (int c = 0; c < KC; ++c) {
-          bf16x8 a[NR];
-          Tile::frag_row(Ks, col, m * DP + 16 * c + 8 * half, a);
-          s = da_mfma_in<NP, false>(a, qf[m][c], s);
-        }
-        float ds[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) ds[e] = exp2_flush(NP == 3 ? (s[e] * p.scale2 - mx[m]) - ll[m] : s[e] * p.scale2 - mx[m]);
-        if (t + DA_T > lim_lo) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (t + 8 * (e >> 2) + 4 * half + (e & 3) >= lim) ds[e] = 0.f;
-        }
-        if (pass == 0) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) rs[m] += ds[e] * dp[e];
+          for (int e = 0; e < 16; ++e) rs[m] = __builtin_fmaf(pr[m][e], dp[e], rs[m]);
         } else {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) ds[e] = ds[e] * (dp[e] - rs[m]);
+          for (int e = 0; e < 16; ++e) pr[m][e] *= dp[e] - rs[m];
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             bf16x8 bo[NS];
-            da_operand<NS>(&ds[8 * c], bo);
+            da_operand<NS>(&pr[m][8 * c], bo);
 #pragma unroll
             for (int v = 0; v < DB; ++v) {
-              bf16x8 a[NP];
-              Tile::frag_col(Kt, m * DP + 32 * v + col, c, half, a);
-              acc[m][v] = da_mfma<NP, NS>(a, bo, acc[m][v]);
+              if (!AHEAD) Tile::frag_col(Kt, m * DP + 32 * v + col, c, half, kt[m][c][v]);
+              acc[m][v] = da_mfma<NP, NS>(kt[m][c][v], bo, acc[m][v]);
             }
           }
         }
       }
     }
-    if (pass == 0) {
+  };
+  sweep(std::false_type());
+  only = __shfl(only, col, HITADV_WAVE);  // key 0 is the first register of the lower half
 #pragma unroll
-      for (int m = 0; m < 2; ++m) rs[m] += __shfl_xor(rs[m], 32, HITADV_WAVE);
-    }
+  for (int m = 0; m < 2; ++m) {
+    rs[m] += __shfl_xor(rs[m], 32, HITADV_WAVE);
+    if (lim == 1) rs[m] = only;  // a row with one key: its probability is 1, dP - r exactly 0
   }
+  sweep(std::true_type());
   if (!valid) return;
   if (half == 0) {
     p.r[srow] = rs[0];
@@ -771,7 +799,7 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dkv_k(DaP p) {
   constexpr int KC = DP / 16, VC = 2 * DP / 16, DB = DP / 32, VB = 2 * DP / 32;
   extern __shared__ __attribute__((aligned(16))) uint16_t da_lds[];
   uint16_t *Qs = da_lds, *Gs = Qs + Tile::ROWS, *Qt = Gs + (DK ? Tile::ROWS : 0), *Gt = Qt + (DK ? Tile::COLS : 0);
-  float *st = (float *)(Gt + (DV ? Tile::COLS : 0));  // [7][32]: max 1, log2 sum 1, max 2, log2 sum 2, r 1, r 2, lam
+  float *st = (float *)(Gt + (DV ? Tile::COLS : 0));  // [7][32]: max 1, log2 sum 1, max 2, log2 sum 2, r 1, r 2, -lam
   int *lims = (int *)(st + 7 * DA_T);
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = da_wave_id(), tid = threadIdx.x;
   const int b = blockIdx.x / p.Hkv, hk = blockIdx.x % p.Hkv;
@@ -787,6 +815,7 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dkv_k(DaP p) {
       const int d = 16 * c + 8 * half;
       uint4 w[NR];
       da_pieces8<NP>(da_load8<NP>(p.k, b * p.k_b + key * p.k_n + hk * p.k_h + m * p.k_m + d, key < len && d < p.D), w);
+      da_sign(w, p);
 #pragma unroll
       for (int k = 0; k < NR; ++k) kf[m][c][k] = as_bf16x8(w[k]);
     }
@@ -837,7 +866,7 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dkv_k(DaP p) {
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k) st[(4 + k) * DA_T + tid] = ok ? p.r[k * n + srow] : 0.f;
-      st[6 * DA_T + tid] = ok ? da_lam(p, h) : 0.f;
+      st[6 * DA_T + tid] = ok ? -da_lam(p, h) : 0.f;
       lims[tid] = ok ? da_limit(p, i, len) : 0;
     }
     __syncthreads();
@@ -845,69 +874,111 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dkv_k(DaP p) {
       fq.load_packed(p.q, q_at, p.q_n, p.q_h, p, t + DA_T);
       fg.load_packed(p.dout, g_at, g_n, 2 * p.D, p, t + DA_T);
     }
-    f32x16 dp = da_zero16(), small = da_zero16();
+    constexpr bool AHEAD = NP != 3 || DP == 32;  // (as in diff_attn_dq_k)
+    bf16x8 ga[VC][NR], qa[2][KC][NR];
+    if (AHEAD) {
 #pragma unroll
-    for (int c = 0; c < (DK ? VC : 0); ++c) {
-      bf16x8 a[NR];
-      Tile::frag_row(Gs, col, 16 * c + 8 * half, a);
-      da_mfma_in2<NP, true>(a, vf[c], dp, small);
+      for (int c = 0; c < (DK ? VC : 0); ++c) Tile::frag_row(Gs, col, 16 * c + 8 * half, ga[c]);
+#pragma unroll
+      for (int c = 0; c < 2 * KC; ++c) Tile::frag_row(Qs, col, (c & 1) * DP + 16 * (c >> 1) + 8 * half, qa[c & 1][c >> 1]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    f32x16 dp = da_zero16(), small = da_zero16(), s[2] = {da_zero16(), da_zero16()};
+#pragma unroll
+    for (int c = 0; c < VC; ++c) {
+      if (DK) {
+        if (!AHEAD) Tile::frag_row(Gs, col, 16 * c + 8 * half, ga[c]);
+        da_mfma_in2<NP, true>(ga[c], vf[c], dp, small);
+      }
+      if (c & 1) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          if (!AHEAD) Tile::frag_row(Qs, col, m * DP + 16 * (c >> 1) + 8 * half, qa[m][c >> 1]);
+          s[m] = da_mfma_in<NP, true>(qa[m][c >> 1], kf[m][c >> 1], s[m]);
+        }
+      }
+    }
+    bf16x8 qt[2][2][DB][NP], gt[2][VB][NP];
+    if (AHEAD) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int m = 0; m < (DK ? 2 : 0); ++m)
+#pragma unroll
+          for (int v = 0; v < DB; ++v) Tile::frag_col(Qt, m * DP + 32 * v + col, c, half, qt[m][c][v]);
+#pragma unroll
+        for (int v = 0; v < (DV ? VB : 0); ++v) Tile::frag_col(Gt, 32 * v + col, c, half, gt[c][v]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
     if (NP == 3) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) dp[e] += small[e];
     }
-    float A[16];
-    const bool edge = key0 + DA_T > da_limit(p, da_div_g(p, t), len);  // (limits grow with the row; rows that do not exist: 2^-inf = 0)
+    float pr[2][16];
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      f32x16 s = da_zero16();
+    for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        bf16x8 a[NR];
-        Tile::frag_row(Qs, col, m * DP + 16 * c + 8 * half, a);
-        s = da_mfma_in<NP, true>(a, kf[m][c], s);
-      }
-      float ds[16];
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const int row = 2 * e + 4 * half;  // rows row .. row + 3 in registers e .. e + 3
-        const float4 mx = *(const float4 *)(st + (2 * m) * DA_T + row), ll = *(const float4 *)(st + (2 * m + 1) * DA_T + row);
-        const float4 rr = *(const float4 *)(st + (4 + m) * DA_T + row), lam = *(const float4 *)(st + 6 * DA_T + row);
-        const int4 li = *(const int4 *)(lims + row);
-        const float mxs[4] = {mx.x, mx.y, mx.z, mx.w}, lls[4] = {ll.x, ll.y, ll.z, ll.w}, rrs[4] = {rr.x, rr.y, rr.z, rr.w};
-        const float las[4] = {lam.x, lam.y, lam.z, lam.w};
-        const int lis[4] = {li.x, li.y, li.z, li.w};
+      for (int e = 0; e < 16; e += 4) {  // rows row .. row + 3 in registers e .. e + 3
+        const int row = 2 * e + 4 * half;
+        const float4 mx = *(const float4 *)(st + (2 * m) * DA_T + row);
+        const float mxs[4] = {mx.x, mx.y, mx.z, mx.w};
+        float lls[4] = {0.f, 0.f, 0.f, 0.f};
+        if (NP == 3) {
+          const float4 ll = *(const float4 *)(st + (2 * m + 1) * DA_T + row);
+          lls[0] = ll.x, lls[1] = ll.y, lls[2] = ll.z, lls[3] = ll.w;
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          float pm = exp2_flush(NP == 3 ? (s[e + j] * p.scale2 - mxs[j]) - lls[j] : s[e + j] * p.scale2 - mxs[j]);
-          if (edge) pm = key < lis[j] ? pm : 0.f;
-          const float d = pm * (dp[e + j] - rrs[j]);
-          if (m == 0) A[e + j] = pm;
-          else A[e + j] = A[e + j] - las[j] * pm;
-          ds[e + j] = m == 0 ? d : -las[j] * d;
+          const float x = __builtin_fmaf(s[m][e + j], p.scale2, -mxs[j]);
+          pr[m][e + j] = exp2_flush(NP == 3 ? x - lls[j] : x);
         }
       }
+    if (key0 + DA_T > da_limit(p, da_div_g(p, t), len)) {  // (limits grow with the row; rows that do not exist: 2^-inf = 0)
 #pragma unroll
-      for (int c = 0; c < (DK ? 2 : 0); ++c) {
-        bf16x8 bo[NS];
-        da_operand<NS>(&ds[8 * c], bo);
+      for (int e = 0; e < 16; e += 4) {
+        const int4 li = *(const int4 *)(lims + 2 * e + 4 * half);
+        const int lis[4] = {li.x, li.y, li.z, li.w};
 #pragma unroll
-        for (int v = 0; v < DB; ++v) {
-          bf16x8 a[NP];
-          Tile::frag_col(Qt, m * DP + 32 * v + col, c, half, a);
-          ak[m][v] = da_mfma<NP, NS>(a, bo, ak[m][v]);
-        }
+        for (int j = 0; j < 4; ++j)
+          if (key >= lis[j]) pr[0][e + j] = pr[1][e + j] = 0.f;
+      }
+    }
+    float A[16];
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const int row = 2 * e + 4 * half;
+      const float4 r1 = *(const float4 *)(st + 4 * DA_T + row), r2 = *(const float4 *)(st + 5 * DA_T + row), nl = *(const float4 *)(st + 6 * DA_T + row);
+      const float r1s[4] = {r1.x, r1.y, r1.z, r1.w}, r2s[4] = {r2.x, r2.y, r2.z, r2.w}, nls[4] = {nl.x, nl.y, nl.z, nl.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float p1 = pr[0][e + j], p2 = pr[1][e + j] * nls[j];  // -lam P_2
+        A[e + j] = p1 + p2;
+        pr[0][e + j] = p1 * (dp[e + j] - r1s[j]);
+        pr[1][e + j] = p2 * (dp[e + j] - r2s[j]);
       }
     }
 #pragma unroll
-    for (int c = 0; c < (DV ? 2 : 0); ++c) {
-      bf16x8 bo[NS];
-      da_operand<NS>(&A[8 * c], bo);
+    for (int c = 0; c < 2; ++c) {
 #pragma unroll
-      for (int v = 0; v < VB; ++v) {
-        bf16x8 a[NP];
-        Tile::frag_col(Gt, 32 * v + col, c, half, a);
-        av[v] = da_mfma<NP, NS>(a, bo, av[v]);
+      for (int m = 0; m < (DK ? 2 : 0); ++m) {
+        bf16x8 bo[NS];
+        da_operand<NS>(&pr[m][8 * c], bo);
+#pragma unroll
+        for (int v = 0; v < DB; ++v) {
+          if (!AHEAD) Tile::frag_col(Qt, m * DP + 32 * v + col, c, half, qt[m][c][v]);
+          ak[m][v] = da_mfma<NP, NS>(qt[m][c][v], bo, ak[m][v]);
+        }
+      }
+      if (DV) {
+        bf16x8 bo[NS];
+        da_operand<NS>(&A[8 * c], bo);
+#pragma unroll
+        for (int v = 0; v < VB; ++v) {
+          if (!AHEAD) Tile::frag_col(Gt, 32 * v + col, c, half, gt[c][v]);
+          av[v] = da_mfma<NP, NS>(gt[c][v], bo, av[v]);
+        }
       }
     }
   }
@@ -1003,7 +1074,7 @@ template <int NP, int DP> static int da_launch_fwd(const DaP &p, const DaPlan &p
        : pl.pairs == 2 ? da_launch_fwd_pairs<NP, DP, 2>(p, pl, s) : da_launch_fwd_pairs<NP, DP, 4>(p, pl, s);
 }
 template <int NP, int DP> static int da_launch_bwd(const DaP &p, float *dlam, hipStream_t s) {
-  const int lds_q = 2 * (2 * DaTile<NP, DP>::ROWS + DaTile<NP, DP>::COLS) + (NP != 3 ? 2 * DP / 16 * 256 * 16 : 0);
+  const int lds_q = 2 * (2 * DaTile<NP, DP>::ROWS + DaTile<NP, DP>::COLS);
   const int tq = (p.rows + 4 * DA_T - 1) / (4 * DA_T), tk = (p.Nk + 4 * DA_T - 1) / (4 * DA_T);
   HITADV_RAISE_LDS((diff_attn_dq_k<NP, DP, 4>), lds_q);
   diff_attn_dq_k<NP, DP, 4><<<dim3(p.B * p.Hkv, tq), 256, lds_q, s>>>(p);
@@ -1043,7 +1114,10 @@ static void da_fill(DaP &p, int B, int Nq, int Nk, int H, int Hkv, int D, int la
   p.rows = Nq * p.G;
   p.g_magic = p.G > 1 ? (uint32_t)(((1ull << 32) + p.G - 1) / p.G) : 0u;
   p.scale = scale;
-  p.scale2 = scale * DA_LOG2E;
+  // a positive factor: the maximum of the scaled scores is the scaled maximum
+  p.scale2 = scale == 0.f ? 1.f : (scale < 0.f ? -scale : scale) * DA_LOG2E;
+  p.s_and = scale == 0.f ? 0u : ~0u;
+  p.s_xor = scale < 0.f ? 0x80008000u : 0u;
   p.q_b = st[0]; p.q_n = st[1]; p.q_h = st[2]; p.q_m = st[3];
   p.k_b = st[4]; p.k_n = st[5]; p.k_h = st[6]; p.k_m = st[7];
   p.v_b = st[8]; p.v_n = st[9]; p.v_h = st[10];
