@@ -30,7 +30,6 @@ namespace hitadv {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int DA_T = 32;          // rows (keys) of a tile = the matrix instruction's width
-constexpr int DA_TS = DA_T + 8;   // row stride of a transposed tile (16-bit elements): 80 bytes, 16 rows on 16 different bank groups
 constexpr float DA_LOG2E = 1.4426950408889634f;
 constexpr float DA_SLACK = 8.0f;  // the running maximum is raised only when it would rise by 2^8: a probability stays below 2^8
 #define DA_INF __builtin_inff()
@@ -51,6 +50,15 @@ struct DaP {
   uint32_t s_and, s_xor; // what makes one operand of the scores carry the scale's sign (or its zero): its elements' words and, xor these
 };
 
+// The row (key) tile of a workgroup; causal: tile 0 has the least (of the backward pass over keys: the most) work.  A grid of up to
+// `resident` workgroups, two or three a CU at once, takes the heavy half first and the light half in rising order, so that the two of a CU even out; a longer one
+// takes the heaviest first.
+__device__ __forceinline__ int da_tile(bool causal, bool rising, int resident) {
+  const int y = blockIdx.y, n = gridDim.y;
+  if (!causal) return y;
+  const int heavy_first = (int64_t)gridDim.x * n <= resident && y >= n - n / 2 ? y - (n - n / 2) : n - 1 - y;
+  return rising ? heavy_first : n - 1 - heavy_first;
+}
 __device__ __forceinline__ int da_div_g(const DaP &p, int r) { return p.G == 1 ? r : (int)(((uint64_t)(uint32_t)r * p.g_magic) >> 32); }
 __device__ __forceinline__ float da_lam(const DaP &p, int h) { return p.lam[p.lam_n == 1 ? 0 : h]; }
 __device__ __forceinline__ int da_len(const DaP &p, int b) {
@@ -213,30 +221,37 @@ __device__ __forceinline__ void da_mfma_in2(const bf16x8 (&a)[DA_NR<NP>], const 
 }
 
 // ---------------------------------------------------------------------------------------------------------------- LDS tiles
-// a tile of 32 rows: [DA_NR][32][2 DP + 8]; its transpose: [NP][2 DP][DA_TS] with the rows in operand order
+// A tile of 32 rows: [DA_NR][32][2 DP]; its transpose: [NP][2 DP][32] with the rows in operand order.  No padding (two workgroups of the
+// backward kernels share a CU's LDS); instead the 16-byte pieces are permuted so that the lanes of an access lie on different banks:
+// a row's pieces by xor with the row; a transposed row goes to place `place(c)` (the two low pairs of bits of its column swapped: lanes that
+// write have columns four apart, lanes that read neighbouring ones) and its four pieces by xor with the column's low bits.
 template <int NP, int DP> struct DaTile {
-  static constexpr int W = 2 * DP, RS = W + 8, NR = DA_NR<NP>;
-  static constexpr int ROWS = NR * DA_T * RS, COLS = NP * W * DA_TS;  // 16-bit elements
+  static constexpr int W = 2 * DP, NR = DA_NR<NP>, M = W / 8 < 16 ? W / 8 - 1 : 15;
+  static constexpr int ROWS = NR * DA_T * W, COLS = NP * W * DA_T;  // 16-bit elements
+  static __device__ __forceinline__ int row_at(int row, int col) { return row * W + (((col >> 3) ^ (row & M)) << 3) + (col & 7); }
+  static __device__ __forceinline__ int col_at(int c, int row) {
+    return ((c & ~15) | ((c & 3) << 2) | ((c >> 2) & 3)) * DA_T + (((row >> 3) ^ (c & 3)) << 3) + (row & 7);
+  }
   static __device__ __forceinline__ void frag_row(const uint16_t *t, int row, int col, bf16x8 (&f)[NR]) {
 #pragma unroll
-    for (int k = 0; k < NR; ++k) f[k] = as_bf16x8(*(const uint4 *)(t + (k * DA_T + row) * RS + col));
+    for (int k = 0; k < NR; ++k) f[k] = as_bf16x8(*(const uint4 *)(t + k * DA_T * W + row_at(row, col)));
   }
   static __device__ __forceinline__ void frag_col(const uint16_t *t, int col, int chunk, int half, bf16x8 (&f)[NP]) {
 #pragma unroll
-    for (int k = 0; k < NP; ++k) f[k] = as_bf16x8(*(const uint4 *)(t + (k * W + col) * DA_TS + 16 * chunk + 8 * half));
+    for (int k = 0; k < NP; ++k) f[k] = as_bf16x8(*(const uint4 *)(t + k * W * DA_T + col_at(col, 16 * chunk + 8 * half)));
   }
   static __device__ __forceinline__ void put_row(uint16_t *t, int row, int col, const Raw8<NP> &r) {
     uint4 p[NR];
     da_pieces8<NP>(r, p);
 #pragma unroll
-    for (int k = 0; k < NR; ++k) *(uint4 *)(t + (k * DA_T + row) * RS + col) = p[k];
+    for (int k = 0; k < NR; ++k) *(uint4 *)(t + k * DA_T * W + row_at(row, col)) = p[k];
   }
   // rows 4 rg .. 4 rg + 3, columns col .. col + 3, as rows and / or transposed: there row 16 c + 8 y + 4 x + j sits at 16 c + 8 x + 4 y + j
   template <bool AS_ROWS, bool AS_COLS> static __device__ __forceinline__ void put_block(uint16_t *rows, uint16_t *cols, int rg, int col, const Raw4<NP> (&r)[4]) {
     if constexpr (AS_ROWS) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        uint16_t *to = rows + (4 * rg + i) * RS + col;
+        uint16_t *to = rows + row_at(4 * rg + i, col);
         if constexpr (NP == 3) {
           uint32_t p[4][3];
           da_pieces<3>(r[i].a.x, p[0]);
@@ -244,7 +259,7 @@ template <int NP, int DP> struct DaTile {
           da_pieces<3>(r[i].a.z, p[2]);
           da_pieces<3>(r[i].a.w, p[3]);
 #pragma unroll
-          for (int k = 0; k < 3; ++k) *(uint2 *)(to + k * DA_T * RS) = make_uint2(pack_hi(p[0][k], p[1][k]), pack_hi(p[2][k], p[3][k]));
+          for (int k = 0; k < 3; ++k) *(uint2 *)(to + k * DA_T * W) = make_uint2(pack_hi(p[0][k], p[1][k]), pack_hi(p[2][k], p[3][k]));
         } else {
           *(uint2 *)to = r[i].a;
         }
@@ -258,14 +273,11 @@ template <int NP, int DP> struct DaTile {
       for (int c = 0; c < 4; ++c)
 #pragma unroll
         for (int k = 0; k < NP; ++k)
-          *(uint2 *)(cols + (k * W + col + c) * DA_TS + at) = make_uint2(pack_hi(p[0][c][k], p[1][c][k]), pack_hi(p[2][c][k], p[3][c][k]));
+          *(uint2 *)(cols + k * W * DA_T + col_at(col + c, at)) = make_uint2(pack_hi(p[0][c][k], p[1][c][k]), pack_hi(p[2][c][k], p[3][c][k]));
     }
   }
 };
 
-// What a workgroup of NT threads fetches of the next tile while it computes on this one: raw elements in registers.  A thread's column is
-// the same in all its pieces; an address is a wave-uniform base plus a 32-bit offset of the thread (strides below 2^24 elements: the entry
-// points see to it).  Threads whose column is padding (D < DP) fetch and store nothing: their cells of the tile are zeroed once.
 template <int NP> constexpr int DA_ES = NP == 3 ? 4 : 2;  // bytes of an element
 // byte offset of a row's column of the padded [2][DP] (maps) or [2 DP] columns; false: padding
 template <int NP, int DP> __device__ __forceinline__ bool da_bind(int row, int col, int64_t n, int64_t m, int D, bool maps, uint32_t &off) {
@@ -387,8 +399,9 @@ __device__ __forceinline__ int da_wave_id() { return __builtin_amdgcn_readfirstl
 // its waves the first map, the other the second: half the accumulators each (two or three waves per SIMD, where one wave with both
 // maps fills the registers), and the difference is taken once, at the end, through LDS.  The next tile's elements are on their way in
 // registers while this one's are multiplied; two buffers, one barrier a tile.
+template <int NP, int DP, int PAIRS> constexpr int DA_FWD_WAVES = NP == 3 && DP == 64 && PAIRS == 1 ? 1 : 2;  // waves per SIMD
 template <int NP, int DP, int PAIRS, bool SPLIT>
-__global__ __launch_bounds__(128 * PAIRS, (NP == 3 && DP == 64 && PAIRS == 1 ? 1 : 2)) void diff_attn_fwd_k(DaP p) {
+__global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_FWD_WAVES<NP, DP, PAIRS>)) void diff_attn_fwd_k(DaP p) {
   using Tile = DaTile<NP, DP>;
   constexpr int NR = DA_NR<NP>, NT = 128 * PAIRS;
   constexpr int NPP = NP == 3 ? 3 : 2;  // pieces of a probability
@@ -398,7 +411,7 @@ __global__ __launch_bounds__(128 * PAIRS, (NP == 3 && DP == 64 && PAIRS == 1 ? 1
   uint16_t *Ks = da_lds, *Vt = da_lds + Tile::ROWS;
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = da_wave_id(), m = wave & 1, tid = threadIdx.x;
   const int b = blockIdx.x / p.Hkv, hk = blockIdx.x % p.Hkv, split = blockIdx.z;
-  const int tile = p.causal ? (int)(gridDim.y - 1 - blockIdx.y) : (int)blockIdx.y;  // causal: the longest rows first
+  const int tile = da_tile(p.causal, true, PAIRS == 4 ? 0 : 512);
   const int row0 = (tile * PAIRS + (wave >> 1)) * DA_T;
   const int len = da_len(p, b);
   const int lim_lo = da_limit(p, da_div_g(p, row0), len), lim_hi = da_limit(p, da_div_g(p, row0 + DA_T - 1), len);
@@ -609,27 +622,33 @@ __global__ __launch_bounds__(256) void diff_attn_join_k(DaP p) {
 // dP = dO V^T;  r_m = sum_j P_m dP;  dS_1 = P_1 (dP - r_1), dS_2 = -lam P_2 (dP - r_2).  The r are sums over the very P and dP that the
 // second pass multiplies (not dO . out: out is rounded, and where a row sees one key dS has to vanish exactly).
 //
-// dQ: the forward kernel's layout, two passes over the keys: first r, then dQ_m^T = K_m^T dS_m^T.  Matrix and vector instructions of a SIMD do
-// not overlap here, so what costs is waiting: a phase's LDS operands are fetched together, ahead of it, into the registers that one wave
-// per SIMD has (two waves with 256 registers and single fetches: 534 us where this takes ~).
-template <int NP, int DP, int NW>
-__global__ __launch_bounds__(64 * NW) void diff_attn_dq_k(DaP p) {
+// dQ: the forward kernel's layout, two passes over the keys: first r, then dQ_m^T = K_m^T dS_m^T.
+// A pair of waves shares 32 packed rows and takes the even and the odd tiles of 32 keys; the two meet in LDS (r behind the first pass, dQ at
+// the end): half the longest row's way through the keys, and twice the waves where clouds are few or short.
+template <int NP, int DP> constexpr int DA_DQ_WAVES = NP == 3 && DP == 64 ? 1 : 2;  // waves per SIMD
+template <int NP, int DP, int PAIRS>
+__global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_DQ_WAVES<NP, DP>)) void diff_attn_dq_k(DaP p) {
   using Tile = DaTile<NP, DP>;
   constexpr int NR = DA_NR<NP>;
   constexpr int NS = NP == 3 ? 3 : 2;  // pieces of dS
   constexpr int KC = DP / 16, VC = 2 * DP / 16, DB = DP / 32;
+  constexpr int SET = 2 * Tile::ROWS + Tile::COLS, NT = 64 * PAIRS;
   extern __shared__ __attribute__((aligned(16))) uint16_t da_lds[];
-  uint16_t *Ks = da_lds, *Vs = da_lds + Tile::ROWS, *Kt = da_lds + 2 * Tile::ROWS;
+  float *red = (float *)(da_lds + 2 * SET);  // [2 parities][PAIRS][3][32]: either map's r, key 0's dP
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = da_wave_id(), tid = threadIdx.x;
+  const int pair = wave >> 1, odd = wave & 1;
   const int b = blockIdx.x / p.Hkv, hk = blockIdx.x % p.Hkv;
-  const int tile = p.causal ? (int)(gridDim.y - 1 - blockIdx.y) : (int)blockIdx.y;
-  const int row0 = (tile * NW + wave) * DA_T, r = row0 + col;
+  const int tile = da_tile(p.causal, true, 0);
+  const int row0 = (tile * PAIRS + pair) * DA_T, r = row0 + col;
   const int i = da_div_g(p, r), g = r - i * p.G, h = hk * p.G + g;
   const bool valid = r < p.rows;
   const int len = da_len(p, b), lim = da_limit(p, i, len);
   const int lim_lo = da_limit(p, da_div_g(p, row0), len), lim_hi = da_limit(p, da_div_g(p, row0 + DA_T - 1), len);
-  const int last = da_limit(p, da_div_g(p, min(p.rows, (tile + 1) * NW * DA_T) - 1), len);
+  const int last = da_limit(p, da_div_g(p, min(p.rows, (tile + 1) * PAIRS * DA_T) - 1), len);
   const int64_t n = (int64_t)p.B * p.H * p.Nq, srow = ((int64_t)b * p.H + h) * p.Nq + i;
+  const uint16_t *Ks = da_lds + odd * SET, *Vs = Ks + Tile::ROWS, *Kt = Vs + Tile::ROWS;  // the wave's tiles
+  const int ph = wave / PAIRS;  // the parity that the wave stages
+  uint16_t *Kp = da_lds + ph * SET, *Vp = Kp + Tile::ROWS, *Tp = Vp + Tile::ROWS;
 
   bf16x8 qf[2][KC][NR], gf[VC][NR];
 #pragma unroll
@@ -651,7 +670,7 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dq_k(DaP p) {
 #pragma unroll
     for (int k = 0; k < NR; ++k) gf[c][k] = as_bf16x8(w[k]);
   }
-  float mx[2], ll[2], rs[2] = {0.f, 0.f}, only = 0.f;
+  float mx[2], ll[2], rs[2] = {0.f, 0.f};
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     mx[m] = valid ? p.stats[(2 * m) * n + srow] : 0.f;
@@ -664,96 +683,78 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dq_k(DaP p) {
 #pragma unroll
     for (int v = 0; v < DB; ++v) acc[m][v] = da_zero16();
 
-  DaFetchBlocks<NP, DP, 64 * NW> fk;
-  DaFetchRows<NP, DP, 64 * NW> fv;
+  DaFetchBlocks<NP, DP, NT> fk;
+  DaFetchRows<NP, DP, NT> fv;
   const int64_t k_at = b * p.k_b + hk * p.k_h, v_at = b * p.v_b + hk * p.v_h;
-  fk.bind(p.k_n, p.k_m, p.D, true, tid);
-  fv.bind(p.v_n, 0, p.D, false, tid);
-  fk.template zero_padding<true, true>(Ks, Kt);
-  fv.zero_padding(Vs);
+  fk.bind(p.k_n, p.k_m, p.D, true, tid % NT);
+  fv.bind(p.v_n, 0, p.D, false, tid % NT);
+  fk.template zero_padding<true, true>(Kp, Tp);
+  fv.zero_padding(Vp);
   if (last > 0) {
-    fk.load(p.k, k_at, p.k_n, 0, len);
-    fv.load(p.v, v_at, p.v_n, 0, len);
+    fk.load(p.k, k_at, p.k_n, ph * DA_T, len);
+    fv.load(p.v, v_at, p.v_n, ph * DA_T, len);
   }
-  constexpr bool AHEAD = NP != 3 || DP == 32;  // (three pieces at DP = 64: no registers left for it)
   auto sweep = [&](auto second) {
     constexpr bool SECOND = decltype(second)::value;
 #pragma unroll 1
-    for (int t = 0; t < last; t += DA_T) {
+    for (int t0 = 0; t0 < last; t0 += 2 * DA_T) {
       __syncthreads();
-      fv.put(Vs);
-      fk.template put<true, SECOND>(Ks, Kt);
+      fv.put(Vp);
+      fk.template put<true, SECOND>(Kp, Tp);
       __syncthreads();
-      const int next = t + DA_T < last ? t + DA_T : 0;  // (behind the second pass: the first tile once more, not used)
+      const int next = (t0 + 2 * DA_T < last ? t0 + 2 * DA_T : 0) + ph * DA_T;  // (behind the second pass: the first tiles once more, not used)
       fk.load(p.k, k_at, p.k_n, next, len);
       fv.load(p.v, v_at, p.v_n, next, len);
+      const int t = t0 + odd * DA_T;
       if (t >= lim_hi) continue;
-      bf16x8 va[VC][NR], ka[2][KC][NR];
-      if (AHEAD) {
-#pragma unroll
-        for (int c = 0; c < VC; ++c) Tile::frag_row(Vs, col, 16 * c + 8 * half, va[c]);
-#pragma unroll
-        for (int c = 0; c < 2 * KC; ++c) Tile::frag_row(Ks, col, (c & 1) * DP + 16 * (c >> 1) + 8 * half, ka[c & 1][c >> 1]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      f32x16 dp = da_zero16(), small = da_zero16(), s[2] = {da_zero16(), da_zero16()};
+      f32x16 dp = da_zero16(), small = da_zero16();
 #pragma unroll
       for (int c = 0; c < VC; ++c) {
-        if (!AHEAD) Tile::frag_row(Vs, col, 16 * c + 8 * half, va[c]);
-        da_mfma_in2<NP, false>(va[c], gf[c], dp, small);
-        if (c & 1) {
-#pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            if (!AHEAD) Tile::frag_row(Ks, col, m * DP + 16 * (c >> 1) + 8 * half, ka[m][c >> 1]);
-            s[m] = da_mfma_in<NP, false>(ka[m][c >> 1], qf[m][c >> 1], s[m]);
-          }
-        }
-      }
-      bf16x8 kt[SECOND ? 2 : 1][2][DB][NP];
-      if (AHEAD && SECOND) {
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int v = 0; v < DB; ++v) Tile::frag_col(Kt, m * DP + 32 * v + col, c, half, kt[m][c][v]);
-        __builtin_amdgcn_sched_barrier(0);
+        bf16x8 a[NR];
+        Tile::frag_row(Vs, col, 16 * c + 8 * half, a);
+        da_mfma_in2<NP, false>(a, gf[c], dp, small);
       }
       if (NP == 3) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) dp[e] += small[e];
       }
-      if (!SECOND && t == 0) only = dp[0];
-      float pr[2][16];
-#pragma unroll
-      for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float x = __builtin_fmaf(s[m][e], p.scale2, -mx[m]);
-          pr[m][e] = exp2_flush(NP == 3 ? x - ll[m] : x);
-        }
-      if (t + DA_T > lim_lo) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (t + 8 * (e >> 2) + 4 * half + (e & 3) >= lim) pr[0][e] = pr[1][e] = 0.f;
-      }
+      if (!SECOND && t == 0 && half == 0) red[(pair * 3 + 2) * 32 + col] = dp[0];  // key 0
+      const bool edge = t + DA_T > lim_lo;
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
+        f32x16 s = da_zero16();
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+          bf16x8 a[NR];
+          Tile::frag_row(Ks, col, m * DP + 16 * c + 8 * half, a);
+          s = da_mfma_in<NP, false>(a, qf[m][c], s);
+        }
+        float pr[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float x = __builtin_fmaf(s[e], p.scale2, -mx[m]);
+          pr[e] = exp2_flush(NP == 3 ? x - ll[m] : x);
+        }
+        if (edge) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (t + 8 * (e >> 2) + 4 * half + (e & 3) >= lim) pr[e] = 0.f;
+        }
         if constexpr (!SECOND) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) rs[m] = __builtin_fmaf(pr[m][e], dp[e], rs[m]);
+          for (int e = 0; e < 16; ++e) rs[m] = __builtin_fmaf(pr[e], dp[e], rs[m]);
         } else {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) pr[m][e] *= dp[e] - rs[m];
+          for (int e = 0; e < 16; ++e) pr[e] *= dp[e] - rs[m];
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             bf16x8 bo[NS];
-            da_operand<NS>(&pr[m][8 * c], bo);
+            da_operand<NS>(&pr[8 * c], bo);
 #pragma unroll
             for (int v = 0; v < DB; ++v) {
-              if (!AHEAD) Tile::frag_col(Kt, m * DP + 32 * v + col, c, half, kt[m][c][v]);
-              acc[m][v] = da_mfma<NP, NS>(kt[m][c][v], bo, acc[m][v]);
+              bf16x8 a[NP];
+              Tile::frag_col(Kt, m * DP + 32 * v + col, c, half, a);
+              acc[m][v] = da_mfma<NP, NS>(a, bo, acc[m][v]);
             }
           }
         }
@@ -761,13 +762,40 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dq_k(DaP p) {
     }
   };
   sweep(std::false_type());
-  only = __shfl(only, col, HITADV_WAVE);  // key 0 is the first register of the lower half
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     rs[m] += __shfl_xor(rs[m], 32, HITADV_WAVE);
-    if (lim == 1) rs[m] = only;  // a row with one key: its probability is 1, dP - r exactly 0
+    if (half == 0) red[((odd * PAIRS + pair) * 3 + m) * 32 + col] = rs[m];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    rs[m] = red[(pair * 3 + m) * 32 + col] + red[((PAIRS + pair) * 3 + m) * 32 + col];
+    if (lim == 1) rs[m] = red[(pair * 3 + 2) * 32 + col];  // a row with one key: its probability is 1, dP - r exactly 0
   }
   sweep(std::true_type());
+  // the odd wave's dQ, a block of 32 columns at a time, in the tiles' place
+  float4 *part = (float4 *)da_lds + pair * 256 + lane;
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int v = 0; v < DB; ++v) {
+      __syncthreads();
+      if (odd) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          part[64 * e] = make_float4(acc[m][v][4 * e], acc[m][v][4 * e + 1], acc[m][v][4 * e + 2], acc[m][v][4 * e + 3]);
+      }
+      __syncthreads();
+      if (!odd) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float4 y = part[64 * e];
+          acc[m][v][4 * e] += y.x, acc[m][v][4 * e + 1] += y.y, acc[m][v][4 * e + 2] += y.z, acc[m][v][4 * e + 3] += y.w;
+        }
+      }
+    }
+  if (odd) return;
   if (!valid) return;
   if (half == 0) {
     p.r[srow] = rs[0];
@@ -791,8 +819,9 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dq_k(DaP p) {
 // share a key needs no atomics: dV^T += dO^T A, dK_m^T += Q_m^T dS_m, A = P_1 - lam P_2.  One launch for both, except for fp32 at DP = 64,
 // where three pieces of K and V and both accumulators are more than 512 registers: dV and dK in a launch each (the scores twice, a quarter
 // more products).
+template <int NP, int DP> constexpr int DA_DKV_WAVES = NP != 3 && DP == 32 ? 2 : 1;  // waves per SIMD
 template <int NP, int DP, int NW, bool DV, bool DK>
-__global__ __launch_bounds__(64 * NW) void diff_attn_dkv_k(DaP p) {
+__global__ __launch_bounds__(64 * NW) HITADV_WAVES_PER_SIMD((DA_DKV_WAVES<NP, DP>)) void diff_attn_dkv_k(DaP p) {
   using Tile = DaTile<NP, DP>;
   constexpr int NR = DA_NR<NP>;
   constexpr int NS = NP == 3 ? 3 : 2;
@@ -803,7 +832,7 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dkv_k(DaP p) {
   int *lims = (int *)(st + 7 * DA_T);
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = da_wave_id(), tid = threadIdx.x;
   const int b = blockIdx.x / p.Hkv, hk = blockIdx.x % p.Hkv;
-  const int first = blockIdx.y * NW * DA_T, key0 = first + wave * DA_T, key = key0 + col;
+  const int first = da_tile(p.causal, false, DP == 64 ? 0 : 512) * NW * DA_T, key0 = first + wave * DA_T, key = key0 + col;
   const int len = da_len(p, b);
   const int64_t n = (int64_t)p.B * p.H * p.Nq;
 
@@ -845,7 +874,43 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dkv_k(DaP p) {
   fg.bind(g_n, 0, p.D, false, tid);
   fq.template zero_padding<true, DK>(Qs, Qt);
   fg.template zero_padding<DK, DV>(Gs, Gt);
+  // the rows' own values, fetched ahead like the tiles: thread (w = tid / 32, row): w = 0, 1 a map's maximum and log2 sum, 2 both r, 3 -lam and
+  // the first key that the row does not see
+  float ahead[2] = {0.f, 0.f};
+  auto load_row = [&](int t) {
+    if (tid >= 4 * DA_T) return;
+    const int w = tid >> 5, r = t + (tid & 31), i = da_div_g(p, r), h = hk * p.G + r - i * p.G;
+    ahead[0] = 0.f;
+    ahead[1] = w < 2 ? DA_INF : 0.f;  // a row that does not exist: probability 2^-inf
+    if (r >= p.rows) return;
+    const int64_t srow = ((int64_t)b * p.H + h) * p.Nq + i;
+    if (w < 2) {
+      ahead[0] = p.stats[2 * w * n + srow];
+      ahead[1] = p.stats[(2 * w + 1) * n + srow];
+    } else if (w == 2) {
+      ahead[0] = p.r[srow];
+      ahead[1] = p.r[n + srow];
+    } else {
+      ahead[0] = -da_lam(p, h);
+      ahead[1] = __int_as_float(da_limit(p, i, len));
+    }
+  };
+  auto put_row = [&]() {
+    if (tid >= 4 * DA_T) return;
+    const int w = tid >> 5, at = tid & 31;
+    if (w < 2) {
+      st[2 * w * DA_T + at] = NP == 3 ? ahead[0] : ahead[0] + ahead[1];  // (as in diff_attn_dq_k)
+      st[(2 * w + 1) * DA_T + at] = ahead[1];
+    } else if (w == 2) {
+      st[4 * DA_T + at] = ahead[0];
+      st[5 * DA_T + at] = ahead[1];
+    } else {
+      st[6 * DA_T + at] = ahead[0];
+      lims[at] = __float_as_int(ahead[1]);
+    }
+  };
   if (begin < p.rows) {
+    load_row(begin);
     fq.load_packed(p.q, q_at, p.q_n, p.q_h, p, begin);
     fg.load_packed(p.dout, g_at, g_n, 2 * p.D, p, begin);
   }
@@ -854,131 +919,135 @@ __global__ __launch_bounds__(64 * NW) void diff_attn_dkv_k(DaP p) {
     __syncthreads();
     fq.template put<true, DK>(Qs, Qt);
     fg.template put<DK, DV>(Gs, Gt);
-    if (tid < DA_T) {
-      const int r = t + tid, i = da_div_g(p, r), h = hk * p.G + r - i * p.G;
-      const bool ok = r < p.rows;
-      const int64_t srow = ((int64_t)b * p.H + h) * p.Nq + i;
-#pragma unroll
-      for (int k = 0; k < 4; k += 2) {
-        const float mx = ok ? p.stats[k * n + srow] : 0.f, ll = ok ? p.stats[(k + 1) * n + srow] : DA_INF;
-        st[k * DA_T + tid] = NP == 3 ? mx : mx + ll;  // (as in diff_attn_dq_k)
-        st[(k + 1) * DA_T + tid] = ll;
-      }
-#pragma unroll
-      for (int k = 0; k < 2; ++k) st[(4 + k) * DA_T + tid] = ok ? p.r[k * n + srow] : 0.f;
-      st[6 * DA_T + tid] = ok ? -da_lam(p, h) : 0.f;
-      lims[tid] = ok ? da_limit(p, i, len) : 0;
-    }
+    put_row();
     __syncthreads();
     if (t + DA_T < p.rows) {
+      load_row(t + DA_T);
       fq.load_packed(p.q, q_at, p.q_n, p.q_h, p, t + DA_T);
       fg.load_packed(p.dout, g_at, g_n, 2 * p.D, p, t + DA_T);
     }
-    constexpr bool AHEAD = NP != 3 || DP == 32;  // (as in diff_attn_dq_k)
+    constexpr bool FENCED = NP != 3 && DP == 64;      // (as in diff_attn_dq_k)
+    constexpr bool SPOT = (NP == 3) == (DP == 64);    // read where they are used: no registers left, or two waves to a SIMD
     bf16x8 ga[VC][NR], qa[2][KC][NR];
-    if (AHEAD) {
+    auto read_q = [&](int m) {
 #pragma unroll
-      for (int c = 0; c < (DK ? VC : 0); ++c) Tile::frag_row(Gs, col, 16 * c + 8 * half, ga[c]);
+      for (int c = 0; c < KC; ++c) Tile::frag_row(Qs, col, m * DP + 16 * c + 8 * half, qa[m][c]);
+      if (FENCED) __builtin_amdgcn_sched_barrier(0);
+    };
 #pragma unroll
-      for (int c = 0; c < 2 * KC; ++c) Tile::frag_row(Qs, col, (c & 1) * DP + 16 * (c >> 1) + 8 * half, qa[c & 1][c >> 1]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
+    for (int c = 0; c < (DK && !SPOT ? VC : 0); ++c) Tile::frag_row(Gs, col, 16 * c + 8 * half, ga[c]);
+    if (!SPOT) read_q(0);
     f32x16 dp = da_zero16(), small = da_zero16(), s[2] = {da_zero16(), da_zero16()};
 #pragma unroll
-    for (int c = 0; c < VC; ++c) {
-      if (DK) {
-        if (!AHEAD) Tile::frag_row(Gs, col, 16 * c + 8 * half, ga[c]);
-        da_mfma_in2<NP, true>(ga[c], vf[c], dp, small);
-      }
-      if (c & 1) {
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          if (!AHEAD) Tile::frag_row(Qs, col, m * DP + 16 * (c >> 1) + 8 * half, qa[m][c >> 1]);
-          s[m] = da_mfma_in<NP, true>(qa[m][c >> 1], kf[m][c >> 1], s[m]);
-        }
-      }
+    for (int c = 0; c < (DK ? VC : 0); ++c) {
+      if (SPOT) Tile::frag_row(Gs, col, 16 * c + 8 * half, ga[c]);
+      da_mfma_in2<NP, true>(ga[c], vf[c], dp, small);
     }
-    bf16x8 qt[2][2][DB][NP], gt[2][VB][NP];
-    if (AHEAD) {
-      __builtin_amdgcn_sched_barrier(0);
+    if (FENCED) __builtin_amdgcn_sched_barrier(0);
+    if (!SPOT) read_q(1);
+    auto scores = [&](int m) {
+      if (SPOT) read_q(m);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-#pragma unroll
-        for (int m = 0; m < (DK ? 2 : 0); ++m)
-#pragma unroll
-          for (int v = 0; v < DB; ++v) Tile::frag_col(Qt, m * DP + 32 * v + col, c, half, qt[m][c][v]);
-#pragma unroll
-        for (int v = 0; v < (DV ? VB : 0); ++v) Tile::frag_col(Gt, 32 * v + col, c, half, gt[c][v]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
+      for (int c = 0; c < KC; ++c) s[m] = da_mfma_in<NP, true>(qa[m][c], kf[m][c], s[m]);
+    };
+    if (!SPOT) {
+      scores(0);
+      scores(1);
     }
+    if (FENCED) __builtin_amdgcn_sched_barrier(0);
     if (NP == 3) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) dp[e] += small[e];
     }
-    float pr[2][16];
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {  // rows row .. row + 3 in registers e .. e + 3
-        const int row = 2 * e + 4 * half;
-        const float4 mx = *(const float4 *)(st + (2 * m) * DA_T + row);
-        const float mxs[4] = {mx.x, mx.y, mx.z, mx.w};
-        float lls[4] = {0.f, 0.f, 0.f, 0.f};
-        if (NP == 3) {
-          const float4 ll = *(const float4 *)(st + (2 * m + 1) * DA_T + row);
-          lls[0] = ll.x, lls[1] = ll.y, lls[2] = ll.z, lls[3] = ll.w;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float x = __builtin_fmaf(s[m][e + j], p.scale2, -mxs[j]);
-          pr[m][e + j] = exp2_flush(NP == 3 ? x - lls[j] : x);
-        }
-      }
-    if (key0 + DA_T > da_limit(p, da_div_g(p, t), len)) {  // (limits grow with the row; rows that do not exist: 2^-inf = 0)
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const int4 li = *(const int4 *)(lims + 2 * e + 4 * half);
-        const int lis[4] = {li.x, li.y, li.z, li.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (key >= lis[j]) pr[0][e + j] = pr[1][e + j] = 0.f;
-      }
-    }
+    const bool edge = key0 + DA_T > da_limit(p, da_div_g(p, t), len);  // (limits grow with the row; rows that do not exist: 2^-inf = 0)
+    bf16x8 gt[2][VB][NP];
     float A[16];
 #pragma unroll
-    for (int e = 0; e < 16; e += 4) {
-      const int row = 2 * e + 4 * half;
-      const float4 r1 = *(const float4 *)(st + 4 * DA_T + row), r2 = *(const float4 *)(st + 5 * DA_T + row), nl = *(const float4 *)(st + 6 * DA_T + row);
-      const float r1s[4] = {r1.x, r1.y, r1.z, r1.w}, r2s[4] = {r2.x, r2.y, r2.z, r2.w}, nls[4] = {nl.x, nl.y, nl.z, nl.w};
+    for (int m = 0; m < 2; ++m) {
+      if (SPOT) scores(m);
+      // rows 8 q + 4 half .. + 3 in registers 4 q .. 4 q + 3
+      float4 mx[4], ll[4], rr[4], nl[4];
+      bf16x8 qt[2][DB][NP];
+      auto read_softmax = [&](int q) {
+        mx[q] = *(const float4 *)(st + (2 * m) * DA_T + 8 * q + 4 * half);
+        if (NP == 3) ll[q] = *(const float4 *)(st + (2 * m + 1) * DA_T + 8 * q + 4 * half);
+      };
+      auto read_r = [&](int q) {
+        if (DK) rr[q] = *(const float4 *)(st + (4 + m) * DA_T + 8 * q + 4 * half);
+        if (m) nl[q] = *(const float4 *)(st + 6 * DA_T + 8 * q + 4 * half);
+      };
+      if (!SPOT) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float p1 = pr[0][e + j], p2 = pr[1][e + j] * nls[j];  // -lam P_2
-        A[e + j] = p1 + p2;
-        pr[0][e + j] = p1 * (dp[e + j] - r1s[j]);
-        pr[1][e + j] = p2 * (dp[e + j] - r2s[j]);
+        for (int q = 0; q < 4; ++q) {
+          read_softmax(q);
+          read_r(q);
+        }
+#pragma unroll
+        for (int c = 0; c < (DK ? 2 : 0); ++c)
+#pragma unroll
+          for (int v = 0; v < DB; ++v) Tile::frag_col(Qt, m * DP + 32 * v + col, c, half, qt[c][v]);
+        if (DV && m) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int v = 0; v < VB; ++v) Tile::frag_col(Gt, 32 * v + col, c, half, gt[c][v]);
+        }
+      }
+      if (FENCED) __builtin_amdgcn_sched_barrier(0);
+      float pr[16];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (SPOT) read_softmax(q);
+        const float mxs[4] = {mx[q].x, mx[q].y, mx[q].z, mx[q].w};
+        float lls[4] = {0.f, 0.f, 0.f, 0.f};
+        if (NP == 3) lls[0] = ll[q].x, lls[1] = ll[q].y, lls[2] = ll[q].z, lls[3] = ll[q].w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float x = __builtin_fmaf(s[m][4 * q + j], p.scale2, -mxs[j]);
+          pr[4 * q + j] = exp2_flush(NP == 3 ? x - lls[j] : x);
+        }
+      }
+      if (edge) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int4 li = *(const int4 *)(lims + 8 * q + 4 * half);
+          const int lis[4] = {li.x, li.y, li.z, li.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (key >= lis[j]) pr[4 * q + j] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (SPOT) read_r(q);
+        float *x = &pr[4 * q];
+        if (m) x[0] *= nl[q].x, x[1] *= nl[q].y, x[2] *= nl[q].z, x[3] *= nl[q].w;  // -lam P_2
+#pragma unroll
+        for (int j = 0; j < 4; ++j) A[4 * q + j] = m ? A[4 * q + j] + x[j] : x[j];
+        if (DK) {
+          const f32x16 &d = dp;
+          x[0] *= d[4 * q] - rr[q].x, x[1] *= d[4 * q + 1] - rr[q].y, x[2] *= d[4 * q + 2] - rr[q].z, x[3] *= d[4 * q + 3] - rr[q].w;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < (DK ? 2 : 0); ++c) {
+        bf16x8 bo[NS];
+        da_operand<NS>(&pr[8 * c], bo);
+#pragma unroll
+        for (int v = 0; v < DB; ++v) {
+          if (SPOT) Tile::frag_col(Qt, m * DP + 32 * v + col, c, half, qt[c][v]);
+          ak[m][v] = da_mfma<NP, NS>(qt[c][v], bo, ak[m][v]);
+        }
       }
     }
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < (DV ? 2 : 0); ++c) {
+      bf16x8 bo[NS];
+      da_operand<NS>(&A[8 * c], bo);
 #pragma unroll
-      for (int m = 0; m < (DK ? 2 : 0); ++m) {
-        bf16x8 bo[NS];
-        da_operand<NS>(&pr[m][8 * c], bo);
-#pragma unroll
-        for (int v = 0; v < DB; ++v) {
-          if (!AHEAD) Tile::frag_col(Qt, m * DP + 32 * v + col, c, half, qt[m][c][v]);
-          ak[m][v] = da_mfma<NP, NS>(qt[m][c][v], bo, ak[m][v]);
-        }
-      }
-      if (DV) {
-        bf16x8 bo[NS];
-        da_operand<NS>(&A[8 * c], bo);
-#pragma unroll
-        for (int v = 0; v < VB; ++v) {
-          if (!AHEAD) Tile::frag_col(Gt, 32 * v + col, c, half, gt[c][v]);
-          av[v] = da_mfma<NP, NS>(gt[c][v], bo, av[v]);
-        }
+      for (int v = 0; v < VB; ++v) {
+        if (SPOT) Tile::frag_col(Gt, 32 * v + col, c, half, gt[c][v]);
+        av[v] = da_mfma<NP, NS>(gt[c][v], bo, av[v]);
       }
     }
   }
@@ -1073,12 +1142,18 @@ template <int NP, int DP> static int da_launch_fwd(const DaP &p, const DaPlan &p
   return pl.pairs == 1 ? da_launch_fwd_pairs<NP, DP, 1>(p, pl, s)
        : pl.pairs == 2 ? da_launch_fwd_pairs<NP, DP, 2>(p, pl, s) : da_launch_fwd_pairs<NP, DP, 4>(p, pl, s);
 }
-template <int NP, int DP> static int da_launch_bwd(const DaP &p, float *dlam, hipStream_t s) {
-  const int lds_q = 2 * (2 * DaTile<NP, DP>::ROWS + DaTile<NP, DP>::COLS);
-  const int tq = (p.rows + 4 * DA_T - 1) / (4 * DA_T), tk = (p.Nk + 4 * DA_T - 1) / (4 * DA_T);
-  HITADV_RAISE_LDS((diff_attn_dq_k<NP, DP, 4>), lds_q);
-  diff_attn_dq_k<NP, DP, 4><<<dim3(p.B * p.Hkv, tq), 256, lds_q, s>>>(p);
+template <int NP, int DP, int PAIRS> static int da_launch_dq(const DaP &p, hipStream_t s) {
+  const int lds = 4 * (2 * DaTile<NP, DP>::ROWS + DaTile<NP, DP>::COLS) + 2 * PAIRS * 3 * 32 * 4;  // bytes
+  const int tiles = (p.rows + PAIRS * DA_T - 1) / (PAIRS * DA_T);
+  HITADV_RAISE_LDS((diff_attn_dq_k<NP, DP, PAIRS>), lds);
+  diff_attn_dq_k<NP, DP, PAIRS><<<dim3(p.B * p.Hkv, tiles), 128 * PAIRS, lds, s>>>(p);
   HITADV_LAUNCH_CHECK();
+  return 0;
+}
+template <int NP, int DP> static int da_launch_bwd(const DaP &p, float *dlam, hipStream_t s) {
+  const int tk = (p.Nk + 4 * DA_T - 1) / (4 * DA_T);
+  const int rc = da_launch_dq<NP, DP, NP == 3 && DP == 64 ? 2 : 4>(p, s);
+  if (rc != 0) return rc;
   if (p.dk) {
     const dim3 grid(p.B * p.Hkv, tk);
     constexpr int R = 2 * DaTile<NP, DP>::ROWS, C = 2 * DaTile<NP, DP>::COLS, ST = 8 * DA_T * 4;  // bytes

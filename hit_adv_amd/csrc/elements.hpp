@@ -2,6 +2,13 @@
 #pragma once
 #include "common.hpp"
 
+// exactly n waves per SIMD: the scheduler uses the registers that leaves instead of saving some for more waves
+#ifdef HITADV_EMULATED
+#define HITADV_WAVES_PER_SIMD(n)
+#else
+#define HITADV_WAVES_PER_SIMD(n) __attribute__((amdgpu_waves_per_eu(n, n)))
+#endif
+
 namespace hitadv {
 
 // two floats -> two bf16, to nearest even
