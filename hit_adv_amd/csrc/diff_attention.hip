@@ -639,43 +639,48 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_DQ_WAVES<NP,
   const int pair = wave >> 1, odd = wave & 1;
   const int b = blockIdx.x / p.Hkv, hk = blockIdx.x % p.Hkv;
   const int tile = da_tile(p.causal, true, 0);
-  const int row0 = (tile * PAIRS + pair) * DA_T, r = row0 + col;
-  const int i = da_div_g(p, r), g = r - i * p.G, h = hk * p.G + g;
-  const bool valid = r < p.rows;
-  const int len = da_len(p, b), lim = da_limit(p, i, len);
+  const int row0 = (tile * PAIRS + pair) * DA_T;
+  const int len = da_len(p, b);
   const int lim_lo = da_limit(p, da_div_g(p, row0), len), lim_hi = da_limit(p, da_div_g(p, row0 + DA_T - 1), len);
   const int last = da_limit(p, da_div_g(p, min(p.rows, (tile + 1) * PAIRS * DA_T) - 1), len);
-  const int64_t n = (int64_t)p.B * p.H * p.Nq, srow = ((int64_t)b * p.H + h) * p.Nq + i;
+  const int64_t n = (int64_t)p.B * p.H * p.Nq;
   const uint16_t *Ks = da_lds + odd * SET, *Vs = Ks + Tile::ROWS, *Kt = Vs + Tile::ROWS;  // the wave's tiles
   const int ph = wave / PAIRS;  // the parity that the wave stages
   uint16_t *Kp = da_lds + ph * SET, *Vp = Kp + Tile::ROWS, *Tp = Vp + Tile::ROWS;
 
   bf16x8 qf[2][KC][NR], gf[VC][NR];
+  float mx[2], ll[2], rs[2] = {0.f, 0.f};
+  int lim;
+  {
+    const int r = row0 + col, i = da_div_g(p, r), h = hk * p.G + r - i * p.G;
+    const bool valid = r < p.rows;
+    const int64_t srow = ((int64_t)b * p.H + h) * p.Nq + i;
+    lim = da_limit(p, i, len);
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int c = 0; c < KC; ++c) {
+      for (int c = 0; c < KC; ++c) {
+        const int d = 16 * c + 8 * half;
+        uint4 w[NR];
+        da_pieces8<NP>(da_load8<NP>(p.q, b * p.q_b + i * p.q_n + h * p.q_h + m * p.q_m + d, valid && d < p.D), w);
+        da_sign(w, p);
+#pragma unroll
+        for (int k = 0; k < NR; ++k) qf[m][c][k] = as_bf16x8(w[k]);
+      }
+#pragma unroll
+    for (int c = 0; c < VC; ++c) {
       const int d = 16 * c + 8 * half;
       uint4 w[NR];
-      da_pieces8<NP>(da_load8<NP>(p.q, b * p.q_b + i * p.q_n + h * p.q_h + m * p.q_m + d, valid && d < p.D), w);
-      da_sign(w, p);
+      da_pieces8<NP>(da_load8<NP>(p.dout, (((int64_t)b * p.Nq + i) * p.H + h) * 2 * p.D + d, valid && d < 2 * p.D), w);
 #pragma unroll
-      for (int k = 0; k < NR; ++k) qf[m][c][k] = as_bf16x8(w[k]);
+      for (int k = 0; k < NR; ++k) gf[c][k] = as_bf16x8(w[k]);
     }
 #pragma unroll
-  for (int c = 0; c < VC; ++c) {
-    const int d = 16 * c + 8 * half;
-    uint4 w[NR];
-    da_pieces8<NP>(da_load8<NP>(p.dout, (((int64_t)b * p.Nq + i) * p.H + h) * 2 * p.D + d, valid && d < 2 * p.D), w);
-#pragma unroll
-    for (int k = 0; k < NR; ++k) gf[c][k] = as_bf16x8(w[k]);
-  }
-  float mx[2], ll[2], rs[2] = {0.f, 0.f};
-#pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    mx[m] = valid ? p.stats[(2 * m) * n + srow] : 0.f;
-    ll[m] = valid ? p.stats[(2 * m + 1) * n + srow] : DA_INF;
-    if (NP != 3) mx[m] += ll[m];  // one subtraction less; fp32 keeps the two apart: their sum's last bit is a probability's error
+    for (int m = 0; m < 2; ++m) {
+      mx[m] = valid ? p.stats[(2 * m) * n + srow] : 0.f;
+      ll[m] = valid ? p.stats[(2 * m + 1) * n + srow] : DA_INF;
+      if (NP != 3) mx[m] += ll[m];  // one subtraction less; fp32 keeps the two apart: their sum's last bit is a probability's error
+    }
   }
   f32x16 acc[2][DB];
 #pragma unroll
@@ -694,6 +699,10 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_DQ_WAVES<NP,
     fk.load(p.k, k_at, p.k_n, ph * DA_T, len);
     fv.load(p.v, v_at, p.v_n, ph * DA_T, len);
   }
+  // Matrix and vector instructions of a SIMD do not overlap here, so a wave's time is its instructions and its waits; left to itself the
+  // compiler reads an LDS operand, waits, multiplies and reads the next.  Scheduling fences hold the reads ahead (three pieces have six
+  // products to an operand and no registers for more than one).
+  constexpr int AHEAD = NP == 3 ? 1 : 4;
   auto sweep = [&](auto second) {
     constexpr bool SECOND = decltype(second)::value;
 #pragma unroll 1
@@ -707,12 +716,28 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_DQ_WAVES<NP,
       fv.load(p.v, v_at, p.v_n, next, len);
       const int t = t0 + odd * DA_T;
       if (t >= lim_hi) continue;
-      f32x16 dp = da_zero16(), small = da_zero16();
+      // V's operands, then the first map's K's: a stream read AHEAD operands before the products that take them
+      bf16x8 fr[VC + KC][NR], kt[2][DB][NP];
+      auto read = [&](int c) {
+        if (c < VC) Tile::frag_row(Vs, col, 16 * c + 8 * half, fr[c]);
+        else Tile::frag_row(Ks, col, 16 * (c - VC) + 8 * half, fr[c]);
+      };
+      auto read_kt = [&](int m) {
 #pragma unroll
-      for (int c = 0; c < VC; ++c) {
-        bf16x8 a[NR];
-        Tile::frag_row(Vs, col, 16 * c + 8 * half, a);
-        da_mfma_in2<NP, false>(a, gf[c], dp, small);
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int v = 0; v < DB; ++v) Tile::frag_col(Kt, m * DP + 32 * v + col, c, half, kt[c][v]);
+      };
+      f32x16 dp = da_zero16(), small = da_zero16(), s = da_zero16();
+#pragma unroll
+      for (int c = 0; c < AHEAD; ++c) read(c);
+      if (AHEAD > 1) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int c = 0; c < VC + KC; ++c) {
+        if (c + AHEAD < VC + KC) read(c + AHEAD);
+        if (AHEAD > 1) __builtin_amdgcn_sched_barrier(0);
+        if (c < VC) da_mfma_in2<NP, false>(fr[c], gf[c < VC ? c : 0], dp, small);
+        else s = da_mfma_in<NP, false>(fr[c], qf[0][c < VC ? 0 : c - VC], s);
       }
       if (NP == 3) {
 #pragma unroll
@@ -722,13 +747,8 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_DQ_WAVES<NP,
       const bool edge = t + DA_T > lim_lo;
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        f32x16 s = da_zero16();
-#pragma unroll
-        for (int c = 0; c < KC; ++c) {
-          bf16x8 a[NR];
-          Tile::frag_row(Ks, col, m * DP + 16 * c + 8 * half, a);
-          s = da_mfma_in<NP, false>(a, qf[m][c], s);
-        }
+        if (SECOND && NP == 1) read_kt(m);
+        if (AHEAD > 1) __builtin_amdgcn_sched_barrier(0);
         float pr[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -740,22 +760,33 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_DQ_WAVES<NP,
           for (int e = 0; e < 16; ++e)
             if (t + 8 * (e >> 2) + 4 * half + (e & 3) >= lim) pr[e] = 0.f;
         }
+        bf16x8 kn[KC][NR];
+        if (m == 0 && AHEAD > 1) {
+#pragma unroll
+          for (int c = 0; c < KC; ++c) Tile::frag_row(Ks, col, DP + 16 * c + 8 * half, kn[c]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
         if constexpr (!SECOND) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) rs[m] = __builtin_fmaf(pr[e], dp[e], rs[m]);
         } else {
 #pragma unroll
           for (int e = 0; e < 16; ++e) pr[e] *= dp[e] - rs[m];
+          if (NP != 1) read_kt(m);
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             bf16x8 bo[NS];
             da_operand<NS>(&pr[8 * c], bo);
 #pragma unroll
-            for (int v = 0; v < DB; ++v) {
-              bf16x8 a[NP];
-              Tile::frag_col(Kt, m * DP + 32 * v + col, c, half, a);
-              acc[m][v] = da_mfma<NP, NS>(a, bo, acc[m][v]);
-            }
+            for (int v = 0; v < DB; ++v) acc[m][v] = da_mfma<NP, NS>(kt[c][v], bo, acc[m][v]);
+          }
+        }
+        if (m == 0) {
+          s = da_zero16();
+#pragma unroll
+          for (int c = 0; c < KC; ++c) {
+            if (AHEAD == 1) Tile::frag_row(Ks, col, DP + 16 * c + 8 * half, kn[c]);
+            s = da_mfma_in<NP, false>(kn[c], qf[1][c], s);
           }
         }
       }
@@ -796,8 +827,10 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_DQ_WAVES<NP,
       }
     }
   if (odd) return;
-  if (!valid) return;
-  if (half == 0) {
+  const int ln = lane_counted(), r = row0 + (ln & 31), i = da_div_g(p, r), h = hk * p.G + r - i * p.G;
+  if (r >= p.rows) return;
+  if (ln < 32) {
+    const int64_t srow = ((int64_t)b * p.H + h) * p.Nq + i;
     p.r[srow] = rs[0];
     p.r[n + srow] = rs[1];
   }
@@ -809,7 +842,7 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_DQ_WAVES<NP,
     for (int v = 0; v < DB; ++v)
 #pragma unroll
       for (int e = 0; e < 16; e += 4) {
-        const int d = 32 * v + 2 * e + 4 * half;
+        const int d = 32 * v + 2 * e + 4 * (ln >> 5);
         if (d < p.D) da_store4<NP>(p.dq, at + m * p.D + d, acc[m][v][e] * w, acc[m][v][e + 1] * w, acc[m][v][e + 2] * w, acc[m][v][e + 3] * w);
       }
   }

@@ -11,6 +11,15 @@
 
 namespace hitadv {
 
+// the lane, counted anew: what an epilogue computes from it is not kept in registers throughout the loop in front
+__device__ __forceinline__ int lane_counted() {
+#ifdef HITADV_EMULATED
+  return threadIdx.x & 63;
+#else
+  return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+#endif
+}
+
 // two floats -> two bf16, to nearest even
 __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
 #ifdef HITADV_EMULATED
