@@ -50,14 +50,9 @@ struct DaP {
   uint32_t s_and, s_xor; // what makes one operand of the scores carry the scale's sign (or its zero): its elements' words and, xor these
 };
 
-// The row (key) tile of a workgroup; causal: tile 0 has the least (of the backward pass over keys: the most) work.  A grid of up to
-// `resident` workgroups, two or three a CU at once, takes the heavy half first and the light half in rising order, so that the two of a CU even out; a longer one
-// takes the heaviest first.
-__device__ __forceinline__ int da_tile(bool causal, bool rising, int resident) {
-  const int y = blockIdx.y, n = gridDim.y;
-  if (!causal) return y;
-  const int heavy_first = (int64_t)gridDim.x * n <= resident && y >= n - n / 2 ? y - (n - n / 2) : n - 1 - y;
-  return rising ? heavy_first : n - 1 - heavy_first;
+// The row (key) tile of a workgroup, causal: the heaviest first -- the last rows, or (`rising` false: tiles of keys) the first keys.
+__device__ __forceinline__ int da_tile(bool causal, bool rising) {
+  return causal && rising ? (int)(gridDim.y - 1 - blockIdx.y) : (int)blockIdx.y;
 }
 __device__ __forceinline__ int da_div_g(const DaP &p, int r) { return p.G == 1 ? r : (int)(((uint64_t)(uint32_t)r * p.g_magic) >> 32); }
 __device__ __forceinline__ float da_lam(const DaP &p, int h) { return p.lam[p.lam_n == 1 ? 0 : h]; }
@@ -76,31 +71,26 @@ template <> struct Raw8<3> { float4 a, b; };
 template <int NP> struct Raw4 { uint2 a; };
 template <> struct Raw4<3> { float4 a; };
 
-template <int NP> __device__ __forceinline__ Raw8<NP> da_load8(const void *base, int64_t at, bool ok) {
+template <class R> __device__ __forceinline__ R da_zero() { return R{}; }
+template <int NP> __device__ __forceinline__ Raw8<NP> da_load8(const char *at) {
   Raw8<NP> r;
   if constexpr (NP == 3) {
-    r.a = r.b = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (ok) {
-      const float4 *s = (const float4 *)((const float *)base + at);
-      r.a = s[0];
-      r.b = s[1];
-    }
+    r.a = ((const float4 *)at)[0];
+    r.b = ((const float4 *)at)[1];
   } else {
-    r.a = make_uint4(0u, 0u, 0u, 0u);
-    if (ok) r.a = *(const uint4 *)((const uint16_t *)base + at);
+    r.a = *(const uint4 *)at;
   }
   return r;
 }
-template <int NP> __device__ __forceinline__ Raw4<NP> da_load4(const void *base, int64_t at, bool ok) {
+template <int NP> __device__ __forceinline__ Raw4<NP> da_load4(const char *at) {
   Raw4<NP> r;
-  if constexpr (NP == 3) {
-    r.a = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (ok) r.a = *(const float4 *)((const float *)base + at);
-  } else {
-    r.a = make_uint2(0u, 0u);
-    if (ok) r.a = *(const uint2 *)((const uint16_t *)base + at);
-  }
+  if constexpr (NP == 3) r.a = *(const float4 *)at;
+  else r.a = *(const uint2 *)at;
   return r;
+}
+// eight elements, or zeros
+template <int NP> __device__ __forceinline__ Raw8<NP> da_load8_if(const void *base, int64_t at, bool ok) {
+  return ok ? da_load8<NP>((const char *)base + at * (NP == 3 ? 4 : 2)) : da_zero<Raw8<NP>>();
 }
 
 // the pieces of a value, each a bf16 in the upper half of a word
@@ -279,96 +269,105 @@ template <int NP, int DP> struct DaTile {
 };
 
 template <int NP> constexpr int DA_ES = NP == 3 ? 4 : 2;  // bytes of an element
-// byte offset of a row's column of the padded [2][DP] (maps) or [2 DP] columns; false: padding
-template <int NP, int DP> __device__ __forceinline__ bool da_bind(int row, int col, int64_t n, int64_t m, int D, bool maps, uint32_t &off) {
+// byte offset of a column of the padded [2][DP] (maps) or [2 DP] columns; false: padding
+template <int NP, int DP> __device__ __forceinline__ bool da_bind(int col, int64_t m, int D, bool maps, uint32_t &off) {
   const int map = maps && col >= DP ? 1 : 0, d = col - map * DP;
-  off = (uint32_t)(row * (int)n + map * (int)m + d) * DA_ES<NP>;
+  off = (uint32_t)(map * (int)m + d) * DA_ES<NP>;
   return d < (maps ? D : 2 * D);
 }
+// Rows that do not exist are fetched as the last one that does and zeroed when they are stored: a load behind a branch, its register zeroed
+// first, has the compiler wait for every load in flight (with that the backward kernels took 1.5x as long).
 template <int NP, int DP, int NT> struct DaFetchRows {  // 16-byte (32-byte) pieces of 32 rows of k, v
   static constexpr int CH = 2 * DP / 8, STEP = NT / CH, C = STEP >= DA_T ? 1 : DA_T / STEP, ES = DA_ES<NP>;
   Raw8<NP> x[C];
-  int row, col;
-  uint32_t off;
+  int row, col, left;
+  uint32_t off;  // of the column
   bool there;
-  __device__ __forceinline__ void bind(int64_t n, int64_t m, int D, bool maps, int tid) {
+  __device__ __forceinline__ void bind(int64_t m, int D, bool maps, int tid) {
     row = tid / CH;
     col = 8 * (tid % CH);
-    there = da_bind<NP, DP>(row, col, n, m, D, maps, off) && row < DA_T;
+    there = da_bind<NP, DP>(col, m, D, maps, off) && row < DA_T;
   }
-  // rows t .. t + 31 of the rows at `base` (elements, wave-uniform); `end`: the first row that does not exist (zeros from there on)
+  // rows t .. t + 31 of the rows at `base` (elements, wave-uniform); `end` > 0: the first row that does not exist
   __device__ __forceinline__ void load(const void *src, int64_t base, int64_t n, int t, int end) {
+    left = end - t;
     if (!there) return;
-    const char *at = (const char *)src + (base + t * n) * ES;
-    if (t + DA_T <= end) {
+    const int first = min(t, end - 1);
+    const char *at = (const char *)src + (base + first * n) * ES;
 #pragma unroll
-      for (int c = 0; c < C; ++c) x[c] = da_load8<NP>(at + c * STEP * n * ES + off, 0, true);
-    } else {
-#pragma unroll
-      for (int c = 0; c < C; ++c) x[c] = da_load8<NP>(at + c * STEP * n * ES + off, 0, t + c * STEP + row < end);
-    }
+    for (int c = 0; c < C; ++c) x[c] = da_load8<NP>(at + (uint32_t)(min(row + c * STEP, end - 1 - first) * (int)n) * ES + off);
   }
-  __device__ __forceinline__ void put(uint16_t *rows) const {
+  __device__ __forceinline__ void put(uint16_t *rows) {
     if (!there) return;
+    if (left < DA_T) {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        if (row + c * STEP >= left) x[c] = da_zero<Raw8<NP>>();
+    }
 #pragma unroll
     for (int c = 0; c < C; ++c) DaTile<NP, DP>::put_row(rows, row + c * STEP, col, x[c]);
   }
   __device__ __forceinline__ void zero_padding(uint16_t *rows) const {
     if (there || row >= DA_T) return;
 #pragma unroll
-    for (int c = 0; c < C; ++c) DaTile<NP, DP>::put_row(rows, row + c * STEP, col, da_load8<NP>(nullptr, 0, false));
+    for (int c = 0; c < C; ++c) DaTile<NP, DP>::put_row(rows, row + c * STEP, col, da_zero<Raw8<NP>>());
   }
 };
-// 4 x 4 blocks, for a transposed tile, or both.  Lanes: four row groups, then sixteen column groups.  Four lanes write 32 consecutive bytes of
-// a transposed row and the next four 16 banks on (columns in neighbouring lanes: eight on one bank); a wave still fetches 128 (256) bytes
-// of every row (eight row groups: 64, and the backward kernels 10 % slower).
+// 4 x 4 blocks, for a transposed tile, or both.  Lanes: four row groups, then sixteen column groups: sixteen lanes write on different
+// banks, and a wave still fetches 128 (256) bytes of every row (eight row groups: 64, and the backward kernels 10 % slower).
 template <int NP, int DP, int NT> struct DaFetchBlocks {
   static constexpr int CH = 2 * DP / 4, STEP = NT / 8, C = STEP >= CH ? 1 : CH / STEP, ES = DA_ES<NP>;
   Raw4<NP> x[C][4];
-  int row, col;
+  int row, col, left;
   uint32_t off[C];
   bool there[C];
-  __device__ __forceinline__ void bind(int64_t n, int64_t m, int D, bool maps, int tid) {
+  __device__ __forceinline__ void bind(int64_t m, int D, bool maps, int tid) {
     row = 4 * ((tid & 3) | ((tid >> 4) & 4));
     col = 4 * (((tid >> 2) & 15) | ((tid >> 7) << 4));
 #pragma unroll
-    for (int c = 0; c < C; ++c) there[c] = da_bind<NP, DP>(row, col + 4 * c * STEP, n, m, D, maps, off[c]) && col < 2 * DP;
+    for (int c = 0; c < C; ++c) there[c] = da_bind<NP, DP>(col + 4 * c * STEP, m, D, maps, off[c]) && col < 2 * DP;
   }
   __device__ __forceinline__ void load(const void *src, int64_t base, int64_t n, int t, int end) {
-    const char *at = (const char *)src + (base + t * n) * ES;
+    left = end - t;
+    const int first = min(t, end - 1);
+    const char *at = (const char *)src + (base + first * n) * ES;
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = (uint32_t)(min(row + i, end - 1 - first) * (int)n) * ES;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       if (!there[c]) continue;
-      if (t + DA_T <= end) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[c][i] = da_load4<NP>(at + i * n * ES + off[c], 0, true);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[c][i] = da_load4<NP>(at + i * n * ES + off[c], 0, t + row + i < end);
-      }
+      for (int i = 0; i < 4; ++i) x[c][i] = da_load4<NP>(at + (o[i] + off[c]));
     }
   }
   // packed query rows: row r is query r / G, head r % G
   __device__ __forceinline__ void load_packed(const void *src, int64_t base, int64_t n, int64_t h, const DaP &p, int t) {
     if (p.G == 1) return load(src, base, n, t, p.rows);
+    left = p.rows - t;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int r = t + row + i, q = da_div_g(p, r);
+      const int r = min(t + row + i, p.rows - 1), q = da_div_g(p, r);
       const char *at = (const char *)src + (base + q * n + (r - q * p.G) * h) * ES;
 #pragma unroll
       for (int c = 0; c < C; ++c)
-        if (there[c]) x[c][i] = da_load4<NP>(at + (off[c] - (uint32_t)(row * (int)n) * ES), 0, r < p.rows);
+        if (there[c]) x[c][i] = da_load4<NP>(at + off[c]);
     }
   }
-  template <bool ROWS, bool COLS> __device__ __forceinline__ void put(uint16_t *rows, uint16_t *cols) const {
+  template <bool ROWS, bool COLS> __device__ __forceinline__ void put(uint16_t *rows, uint16_t *cols) {
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-      if (there[c]) DaTile<NP, DP>::template put_block<ROWS, COLS>(rows, cols, row / 4, col + 4 * c * STEP, x[c]);
+    for (int c = 0; c < C; ++c) {
+      if (!there[c]) continue;
+      if (left < DA_T) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (row + i >= left) x[c][i] = da_zero<Raw4<NP>>();
+      }
+      DaTile<NP, DP>::template put_block<ROWS, COLS>(rows, cols, row / 4, col + 4 * c * STEP, x[c]);
+    }
   }
-  template <bool ROWS, bool COLS> __device__ __forceinline__ void zero_padding(uint16_t *rows, uint16_t *cols) {
-    Raw4<NP> z[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) z[i] = da_load4<NP>(nullptr, 0, false);
+  template <bool ROWS, bool COLS> __device__ __forceinline__ void zero_padding(uint16_t *rows, uint16_t *cols) const {
+    const Raw4<NP> z[4] = {da_zero<Raw4<NP>>(), da_zero<Raw4<NP>>(), da_zero<Raw4<NP>>(), da_zero<Raw4<NP>>()};
 #pragma unroll
     for (int c = 0; c < C; ++c)
       if (!there[c] && col < 2 * DP) DaTile<NP, DP>::template put_block<ROWS, COLS>(rows, cols, row / 4, col + 4 * c * STEP, z);
@@ -411,7 +410,7 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_FWD_WAVES<NP
   uint16_t *Ks = da_lds, *Vt = da_lds + Tile::ROWS;
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = da_wave_id(), m = wave & 1, tid = threadIdx.x;
   const int b = blockIdx.x / p.Hkv, hk = blockIdx.x % p.Hkv, split = blockIdx.z;
-  const int tile = da_tile(p.causal, true, PAIRS == 4 ? 0 : 512);
+  const int tile = da_tile(p.causal, true);
   const int row0 = (tile * PAIRS + (wave >> 1)) * DA_T;
   const int len = da_len(p, b);
   const int lim_lo = da_limit(p, da_div_g(p, row0), len), lim_hi = da_limit(p, da_div_g(p, row0 + DA_T - 1), len);
@@ -426,7 +425,7 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_FWD_WAVES<NP
     for (int c = 0; c < KC; ++c) {
       const int d = 16 * c + 8 * half;
       uint4 w[NR];
-      da_pieces8<NP>(da_load8<NP>(p.q, b * p.q_b + i * p.q_n + h * p.q_h + m * p.q_m + d, r < p.rows && d < p.D), w);
+      da_pieces8<NP>(da_load8_if<NP>(p.q, b * p.q_b + i * p.q_n + h * p.q_h + m * p.q_m + d, r < p.rows && d < p.D), w);
       da_sign(w, p);
 #pragma unroll
       for (int k = 0; k < NR; ++k) qf[c][k] = as_bf16x8(w[k]);
@@ -441,8 +440,8 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_FWD_WAVES<NP
   DaFetchRows<NP, DP, NT> fk;
   DaFetchBlocks<NP, DP, NT> fv;
   const int64_t k_at = b * p.k_b + hk * p.k_h, v_at = b * p.v_b + hk * p.v_h;
-  fk.bind(p.k_n, p.k_m, p.D, true, tid);
-  fv.bind(p.v_n, 0, p.D, false, tid);
+  fk.bind(p.k_m, p.D, true, tid);
+  fv.bind(0, p.D, false, tid);
   fk.zero_padding(Ks);
   fv.template zero_padding<false, true>(nullptr, Vt);
   fk.zero_padding(Ks + BUF);
@@ -638,7 +637,7 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_DQ_WAVES<NP,
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = da_wave_id(), tid = threadIdx.x;
   const int pair = wave >> 1, odd = wave & 1;
   const int b = blockIdx.x / p.Hkv, hk = blockIdx.x % p.Hkv;
-  const int tile = da_tile(p.causal, true, 0);
+  const int tile = da_tile(p.causal, true);
   const int row0 = (tile * PAIRS + pair) * DA_T;
   const int len = da_len(p, b);
   const int lim_lo = da_limit(p, da_div_g(p, row0), len), lim_hi = da_limit(p, da_div_g(p, row0 + DA_T - 1), len);
@@ -662,7 +661,7 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_DQ_WAVES<NP,
       for (int c = 0; c < KC; ++c) {
         const int d = 16 * c + 8 * half;
         uint4 w[NR];
-        da_pieces8<NP>(da_load8<NP>(p.q, b * p.q_b + i * p.q_n + h * p.q_h + m * p.q_m + d, valid && d < p.D), w);
+        da_pieces8<NP>(da_load8_if<NP>(p.q, b * p.q_b + i * p.q_n + h * p.q_h + m * p.q_m + d, valid && d < p.D), w);
         da_sign(w, p);
 #pragma unroll
         for (int k = 0; k < NR; ++k) qf[m][c][k] = as_bf16x8(w[k]);
@@ -671,7 +670,7 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_DQ_WAVES<NP,
     for (int c = 0; c < VC; ++c) {
       const int d = 16 * c + 8 * half;
       uint4 w[NR];
-      da_pieces8<NP>(da_load8<NP>(p.dout, (((int64_t)b * p.Nq + i) * p.H + h) * 2 * p.D + d, valid && d < 2 * p.D), w);
+      da_pieces8<NP>(da_load8_if<NP>(p.dout, (((int64_t)b * p.Nq + i) * p.H + h) * 2 * p.D + d, valid && d < 2 * p.D), w);
 #pragma unroll
       for (int k = 0; k < NR; ++k) gf[c][k] = as_bf16x8(w[k]);
     }
@@ -691,8 +690,8 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_DQ_WAVES<NP,
   DaFetchBlocks<NP, DP, NT> fk;
   DaFetchRows<NP, DP, NT> fv;
   const int64_t k_at = b * p.k_b + hk * p.k_h, v_at = b * p.v_b + hk * p.v_h;
-  fk.bind(p.k_n, p.k_m, p.D, true, tid % NT);
-  fv.bind(p.v_n, 0, p.D, false, tid % NT);
+  fk.bind(p.k_m, p.D, true, tid % NT);
+  fv.bind(0, p.D, false, tid % NT);
   fk.template zero_padding<true, true>(Kp, Tp);
   fv.zero_padding(Vp);
   if (last > 0) {
@@ -865,7 +864,7 @@ __global__ __launch_bounds__(64 * NW) HITADV_WAVES_PER_SIMD((DA_DKV_WAVES<NP, DP
   int *lims = (int *)(st + 7 * DA_T);
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = da_wave_id(), tid = threadIdx.x;
   const int b = blockIdx.x / p.Hkv, hk = blockIdx.x % p.Hkv;
-  const int first = da_tile(p.causal, false, DP == 64 ? 0 : 512) * NW * DA_T, key0 = first + wave * DA_T, key = key0 + col;
+  const int first = da_tile(p.causal, false) * NW * DA_T, key0 = first + wave * DA_T, key = key0 + col;
   const int len = da_len(p, b);
   const int64_t n = (int64_t)p.B * p.H * p.Nq;
 
@@ -876,7 +875,7 @@ __global__ __launch_bounds__(64 * NW) HITADV_WAVES_PER_SIMD((DA_DKV_WAVES<NP, DP
     for (int c = 0; c < KC; ++c) {
       const int d = 16 * c + 8 * half;
       uint4 w[NR];
-      da_pieces8<NP>(da_load8<NP>(p.k, b * p.k_b + key * p.k_n + hk * p.k_h + m * p.k_m + d, key < len && d < p.D), w);
+      da_pieces8<NP>(da_load8_if<NP>(p.k, b * p.k_b + key * p.k_n + hk * p.k_h + m * p.k_m + d, key < len && d < p.D), w);
       da_sign(w, p);
 #pragma unroll
       for (int k = 0; k < NR; ++k) kf[m][c][k] = as_bf16x8(w[k]);
@@ -885,7 +884,7 @@ __global__ __launch_bounds__(64 * NW) HITADV_WAVES_PER_SIMD((DA_DKV_WAVES<NP, DP
   for (int c = 0; c < (DK ? VC : 0); ++c) {
     const int d = 16 * c + 8 * half;
     uint4 w[NR];
-    da_pieces8<NP>(da_load8<NP>(p.v, b * p.v_b + key * p.v_n + hk * p.v_h + d, key < len && d < 2 * p.D), w);
+    da_pieces8<NP>(da_load8_if<NP>(p.v, b * p.v_b + key * p.v_n + hk * p.v_h + d, key < len && d < 2 * p.D), w);
 #pragma unroll
     for (int k = 0; k < NR; ++k) vf[c][k] = as_bf16x8(w[k]);
   }
@@ -903,8 +902,8 @@ __global__ __launch_bounds__(64 * NW) HITADV_WAVES_PER_SIMD((DA_DKV_WAVES<NP, DP
   DaFetchBlocks<NP, DP, 64 * NW> fq, fg;
   const int64_t g_n = (int64_t)p.H * 2 * p.D;
   const int64_t q_at = b * p.q_b + hk * p.G * p.q_h, g_at = ((int64_t)b * p.Nq * p.H + hk * p.G) * 2 * p.D;
-  fq.bind(p.q_n, p.q_m, p.D, true, tid);
-  fg.bind(g_n, 0, p.D, false, tid);
+  fq.bind(p.q_m, p.D, true, tid);
+  fg.bind(0, p.D, false, tid);
   fq.template zero_padding<true, DK>(Qs, Qt);
   fg.template zero_padding<DK, DV>(Gs, Gt);
   // the rows' own values, fetched ahead like the tiles: thread (w = tid / 32, row): w = 0, 1 a map's maximum and log2 sum, 2 both r, 3 -lam and
@@ -912,10 +911,7 @@ __global__ __launch_bounds__(64 * NW) HITADV_WAVES_PER_SIMD((DA_DKV_WAVES<NP, DP
   float ahead[2] = {0.f, 0.f};
   auto load_row = [&](int t) {
     if (tid >= 4 * DA_T) return;
-    const int w = tid >> 5, r = t + (tid & 31), i = da_div_g(p, r), h = hk * p.G + r - i * p.G;
-    ahead[0] = 0.f;
-    ahead[1] = w < 2 ? DA_INF : 0.f;  // a row that does not exist: probability 2^-inf
-    if (r >= p.rows) return;
+    const int w = tid >> 5, r = min(t + (tid & 31), p.rows - 1), i = da_div_g(p, r), h = hk * p.G + r - i * p.G;
     const int64_t srow = ((int64_t)b * p.H + h) * p.Nq + i;
     if (w < 2) {
       ahead[0] = p.stats[2 * w * n + srow];
@@ -928,9 +924,10 @@ __global__ __launch_bounds__(64 * NW) HITADV_WAVES_PER_SIMD((DA_DKV_WAVES<NP, DP
       ahead[1] = __int_as_float(da_limit(p, i, len));
     }
   };
-  auto put_row = [&]() {
+  auto put_row = [&](int t) {
     if (tid >= 4 * DA_T) return;
     const int w = tid >> 5, at = tid & 31;
+    if (t + at >= p.rows && w < 2) ahead[1] = DA_INF;  // a row that does not exist: probability 2^-inf
     if (w < 2) {
       st[2 * w * DA_T + at] = NP == 3 ? ahead[0] : ahead[0] + ahead[1];  // (as in diff_attn_dq_k)
       st[(2 * w + 1) * DA_T + at] = ahead[1];
@@ -952,7 +949,7 @@ __global__ __launch_bounds__(64 * NW) HITADV_WAVES_PER_SIMD((DA_DKV_WAVES<NP, DP
     __syncthreads();
     fq.template put<true, DK>(Qs, Qt);
     fg.template put<DK, DV>(Gs, Gt);
-    put_row();
+    put_row(t);
     __syncthreads();
     if (t + DA_T < p.rows) {
       load_row(t + DA_T);
