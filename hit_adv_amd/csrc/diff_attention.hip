@@ -272,11 +272,13 @@ template <int NP> constexpr int DA_ES = NP == 3 ? 4 : 2;  // bytes of an element
 // byte offset of a column of the padded [2][DP] (maps) or [2 DP] columns; false: padding
 template <int NP, int DP> __device__ __forceinline__ bool da_bind(int col, int64_t m, int D, bool maps, uint32_t &off) {
   const int map = maps && col >= DP ? 1 : 0, d = col - map * DP;
-  off = (uint32_t)(map * (int)m + d) * DA_ES<NP>;
-  return d < (maps ? D : 2 * D);
+  const bool there = d < (maps ? D : 2 * D);
+  off = there ? (uint32_t)(map * (int)m + d) * DA_ES<NP> : 0u;  // (padding is fetched from the row's first column and not stored)
+  return there;
 }
-// Rows that do not exist are fetched as the last one that does and zeroed when they are stored: a load behind a branch, its register zeroed
-// first, has the compiler wait for every load in flight (with that the backward kernels took 1.5x as long).
+// Rows that do not exist are fetched as the last one that does and zeroed when they are stored, and columns that do not exist are fetched
+// and dropped: a load behind a branch, its register zeroed first or kept from before, has the compiler wait for every load in flight (with
+// that the backward kernels took 1.5x as long).
 template <int NP, int DP, int NT> struct DaFetchRows {  // 16-byte (32-byte) pieces of 32 rows of k, v
   static constexpr int CH = 2 * DP / 8, STEP = NT / CH, C = STEP >= DA_T ? 1 : DA_T / STEP, ES = DA_ES<NP>;
   Raw8<NP> x[C];
@@ -291,7 +293,6 @@ template <int NP, int DP, int NT> struct DaFetchRows {  // 16-byte (32-byte) pie
   // rows t .. t + 31 of the rows at `base` (elements, wave-uniform); `end` > 0: the first row that does not exist
   __device__ __forceinline__ void load(const void *src, int64_t base, int64_t n, int t, int end) {
     left = end - t;
-    if (!there) return;
     const int first = min(t, end - 1);
     const char *at = (const char *)src + (base + first * n) * ES;
 #pragma unroll
@@ -336,23 +337,29 @@ template <int NP, int DP, int NT> struct DaFetchBlocks {
     for (int i = 0; i < 4; ++i) o[i] = (uint32_t)(min(row + i, end - 1 - first) * (int)n) * ES;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      if (!there[c]) continue;
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[c][i] = da_load4<NP>(at + (o[i] + off[c]));
     }
   }
   // packed query rows: row r is query r / G, head r % G
   __device__ __forceinline__ void load_packed(const void *src, int64_t base, int64_t n, int64_t h, const DaP &p, int t) {
-    if (p.G == 1) return load(src, base, n, t, p.rows);
     left = p.rows - t;
+    const char *at = (const char *)src + base * ES;
+    int64_t o[4];
+    if (p.G == 1) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = min(t + row + i, p.rows - 1), q = da_div_g(p, r);
-      const char *at = (const char *)src + (base + q * n + (r - q * p.G) * h) * ES;
+      for (int i = 0; i < 4; ++i) o[i] = min(t + row + i, p.rows - 1) * n;
+    } else {
 #pragma unroll
-      for (int c = 0; c < C; ++c)
-        if (there[c]) x[c][i] = da_load4<NP>(at + off[c]);
+      for (int i = 0; i < 4; ++i) {
+        const int r = min(t + row + i, p.rows - 1), q = da_div_g(p, r);
+        o[i] = q * n + (r - q * p.G) * h;
+      }
     }
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[c][i] = da_load4<NP>(at + (o[i] * ES + off[c]));
   }
   template <bool ROWS, bool COLS> __device__ __forceinline__ void put(uint16_t *rows, uint16_t *cols) {
 #pragma unroll
@@ -747,7 +754,7 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_DQ_WAVES<NP,
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         if (SECOND && NP == 1) read_kt(m);
-        if (AHEAD > 1) __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_sched_barrier(0);  // (three pieces: without it four registers too many)
         float pr[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -906,37 +913,30 @@ __global__ __launch_bounds__(64 * NW) HITADV_WAVES_PER_SIMD((DA_DKV_WAVES<NP, DP
   fg.bind(0, p.D, false, tid);
   fq.template zero_padding<true, DK>(Qs, Qt);
   fg.template zero_padding<DK, DV>(Gs, Gt);
-  // the rows' own values, fetched ahead like the tiles: thread (w = tid / 32, row): w = 0, 1 a map's maximum and log2 sum, 2 both r, 3 -lam and
-  // the first key that the row does not see
+  // the rows' own values, fetched ahead like the tiles: thread (w = tid / 32, row): w = 0, 1 a map's maximum and log2 sum, 2 both r, 3 lam
   float ahead[2] = {0.f, 0.f};
   auto load_row = [&](int t) {
     if (tid >= 4 * DA_T) return;
     const int w = tid >> 5, r = min(t + (tid & 31), p.rows - 1), i = da_div_g(p, r), h = hk * p.G + r - i * p.G;
     const int64_t srow = ((int64_t)b * p.H + h) * p.Nq + i;
-    if (w < 2) {
-      ahead[0] = p.stats[2 * w * n + srow];
-      ahead[1] = p.stats[(2 * w + 1) * n + srow];
-    } else if (w == 2) {
-      ahead[0] = p.r[srow];
-      ahead[1] = p.r[n + srow];
-    } else {
-      ahead[0] = -da_lam(p, h);
-      ahead[1] = __int_as_float(da_limit(p, i, len));
-    }
+    const float *one = w < 2 ? p.stats + 2 * w * n + srow : w == 2 ? p.r + srow : p.lam + (p.lam_n == 1 ? 0 : h);
+    const float *two = w < 3 ? one + n : one;
+    ahead[0] = *one;
+    ahead[1] = *two;
   };
   auto put_row = [&](int t) {
     if (tid >= 4 * DA_T) return;
     const int w = tid >> 5, at = tid & 31;
-    if (t + at >= p.rows && w < 2) ahead[1] = DA_INF;  // a row that does not exist: probability 2^-inf
     if (w < 2) {
-      st[2 * w * DA_T + at] = NP == 3 ? ahead[0] : ahead[0] + ahead[1];  // (as in diff_attn_dq_k)
-      st[(2 * w + 1) * DA_T + at] = ahead[1];
+      const float ll = t + at < p.rows ? ahead[1] : DA_INF;  // a row that does not exist: probability 2^-inf
+      st[2 * w * DA_T + at] = NP == 3 ? ahead[0] : ahead[0] + ll;  // (as in diff_attn_dq_k)
+      st[(2 * w + 1) * DA_T + at] = ll;
     } else if (w == 2) {
       st[4 * DA_T + at] = ahead[0];
       st[5 * DA_T + at] = ahead[1];
     } else {
-      st[6 * DA_T + at] = ahead[0];
-      lims[at] = __float_as_int(ahead[1]);
+      st[6 * DA_T + at] = -ahead[0];
+      lims[at] = da_limit(p, da_div_g(p, t + at), len);  // the first key that the row does not see
     }
   };
   if (begin < p.rows) {
@@ -951,11 +951,9 @@ __global__ __launch_bounds__(64 * NW) HITADV_WAVES_PER_SIMD((DA_DKV_WAVES<NP, DP
     fg.template put<DK, DV>(Gs, Gt);
     put_row(t);
     __syncthreads();
-    if (t + DA_T < p.rows) {
-      load_row(t + DA_T);
-      fq.load_packed(p.q, q_at, p.q_n, p.q_h, p, t + DA_T);
-      fg.load_packed(p.dout, g_at, g_n, 2 * p.D, p, t + DA_T);
-    }
+    load_row(t + DA_T);  // (behind the last tile: its last row once more, not used)
+    fq.load_packed(p.q, q_at, p.q_n, p.q_h, p, t + DA_T);
+    fg.load_packed(p.dout, g_at, g_n, 2 * p.D, p, t + DA_T);
     constexpr bool FENCED = NP != 3 && DP == 64;      // (as in diff_attn_dq_k)
     constexpr bool SPOT = (NP == 3) == (DP == 64);    // read where they are used: no registers left, or two waves to a SIMD
     bf16x8 ga[VC][NR], qa[2][KC][NR];
