@@ -272,13 +272,11 @@ template <int NP> constexpr int DA_ES = NP == 3 ? 4 : 2;  // bytes of an element
 // byte offset of a column of the padded [2][DP] (maps) or [2 DP] columns; false: padding
 template <int NP, int DP> __device__ __forceinline__ bool da_bind(int col, int64_t m, int D, bool maps, uint32_t &off) {
   const int map = maps && col >= DP ? 1 : 0, d = col - map * DP;
-  const bool there = d < (maps ? D : 2 * D);
-  off = there ? (uint32_t)(map * (int)m + d) * DA_ES<NP> : 0u;  // (padding is fetched from the row's first column and not stored)
-  return there;
+  off = (uint32_t)(map * (int)m + d) * DA_ES<NP>;
+  return d < (maps ? D : 2 * D);
 }
-// Rows that do not exist are fetched as the last one that does and zeroed when they are stored, and columns that do not exist are fetched
-// and dropped: a load behind a branch, its register zeroed first or kept from before, has the compiler wait for every load in flight (with
-// that the backward kernels took 1.5x as long).
+// Rows that do not exist are fetched as the last one that does and zeroed when they are stored: a load behind a branch, its register zeroed
+// first, has the compiler wait for every load in flight (with that the backward kernels took 1.5x as long).
 template <int NP, int DP, int NT> struct DaFetchRows {  // 16-byte (32-byte) pieces of 32 rows of k, v
   static constexpr int CH = 2 * DP / 8, STEP = NT / CH, C = STEP >= DA_T ? 1 : DA_T / STEP, ES = DA_ES<NP>;
   Raw8<NP> x[C];
@@ -293,6 +291,7 @@ template <int NP, int DP, int NT> struct DaFetchRows {  // 16-byte (32-byte) pie
   // rows t .. t + 31 of the rows at `base` (elements, wave-uniform); `end` > 0: the first row that does not exist
   __device__ __forceinline__ void load(const void *src, int64_t base, int64_t n, int t, int end) {
     left = end - t;
+    if (!there) return;
     const int first = min(t, end - 1);
     const char *at = (const char *)src + (base + first * n) * ES;
 #pragma unroll
@@ -337,11 +336,13 @@ template <int NP, int DP, int NT> struct DaFetchBlocks {
     for (int i = 0; i < 4; ++i) o[i] = (uint32_t)(min(row + i, end - 1 - first) * (int)n) * ES;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
+      if (!there[c]) continue;
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[c][i] = da_load4<NP>(at + (o[i] + off[c]));
     }
   }
-  // packed query rows: row r is query r / G, head r % G
+  // packed query rows: row r is query r / G, head r % G.  Two ways to a row's address meet before the loads, so none is behind a branch:
+  // a column that does not exist is fetched as the row's first and dropped.
   __device__ __forceinline__ void load_packed(const void *src, int64_t base, int64_t n, int64_t h, const DaP &p, int t) {
     left = p.rows - t;
     const char *at = (const char *)src + base * ES;
@@ -357,9 +358,11 @@ template <int NP, int DP, int NT> struct DaFetchBlocks {
       }
     }
 #pragma unroll
-    for (int c = 0; c < C; ++c)
+    for (int c = 0; c < C; ++c) {
+      const uint32_t oc = there[c] ? off[c] : 0u;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[c][i] = da_load4<NP>(at + (o[i] * ES + off[c]));
+      for (int i = 0; i < 4; ++i) x[c][i] = da_load4<NP>(at + (o[i] * ES + oc));
+    }
   }
   template <bool ROWS, bool COLS> __device__ __forceinline__ void put(uint16_t *rows, uint16_t *cols) {
 #pragma unroll
