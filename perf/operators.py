@@ -140,8 +140,7 @@ def _own(s):
         return {"out": out, "dq": dq, "dk": dk, "dv": dv, "dlam": dlam}
     if c["op"] == "norm":
         if c["mode"] == "quant":
-            q, scale, total = ops.rms_norm_quant(s["x"], s["weight"], eps=EPS, residual=s["residual"])
-            return {"q": q, "scale": scale, "sum": total} if c["residual"] else {"q": q, "scale": scale}
+            return dict(zip(("q", "scale", "sum"), ops.rms_norm_quant(s["x"], s["weight"], eps=EPS, residual=s["residual"])))
         if c["residual"]:
             y, total = ops.rms_norm(s["x"], s["weight"], eps=EPS, residual=s["residual"])
             if c["mode"] == "fwd":
