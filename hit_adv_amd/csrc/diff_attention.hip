@@ -8,9 +8,9 @@
 //
 // Arithmetic.  Everything runs on the 16-bit matrix cores with fp32 accumulators.  The products of two inputs (the scores, dO V^T) take
 // bf16 and fp16 inputs as they are: every product is exact.  fp32 inputs enter as three bf16 pieces whose sum is the value (each the
-// truncation of what is left) and six piece products.  The products with a map on one side (P V and those of the backward pass) are
-// always bf16 pieces, also where the inputs are fp16 (two pieces, exact): a bf16 piece has fp32's exponent, so neither a small
-// probability nor a large gradient leaves the range.  The map itself is two pieces (three in fp32) also where the inputs are bf16:
+// truncation of what is left) and six piece products.  The products with a map on one side are bf16 pieces, in the backward pass also where
+// the inputs are fp16 (two pieces, exact): a bf16 piece has fp32's exponent, so no gradient leaves the range.  (P V of fp16 inputs: see the
+// forward kernel.)  The map itself is two pieces (three in fp32) also where the inputs are bf16:
 // rounding P_1 and P_2 to one bf16 each before their difference is taken puts back the noise that the difference is there to cancel,
 // and one-piece dS and A = P_1 - lam P_2 put the gradients at 1.5x the error of their own last rounding (two: 1.0x).  Maxima, sums
 // and accumulators are fp32.  A value that is not finite makes the rows that see it NaN.
@@ -167,6 +167,24 @@ template <int NPP> __device__ __forceinline__ void da_operand(const float *x, bf
     out[0] = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
     if constexpr (NPP == 2) out[1] = as_bf16x8(make_uint4(l[0], l[1], l[2], l[3]));
   }
+}
+
+// the same as two fp16 pieces (22 bits)
+__device__ __forceinline__ void da_operand_f16(const float *x, bf16x8 (&out)[2]) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  uint32_t w[4], l[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f16x2 h, r;
+    h.x = (_Float16)x[2 * i];
+    h.y = (_Float16)x[2 * i + 1];
+    r.x = (_Float16)(x[2 * i] - (float)h.x);
+    r.y = (_Float16)(x[2 * i + 1] - (float)h.y);
+    w[i] = __builtin_bit_cast(uint32_t, h);
+    l[i] = __builtin_bit_cast(uint32_t, r);
+  }
+  out[0] = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
+  out[1] = as_bf16x8(make_uint4(l[0], l[1], l[2], l[3]));
 }
 
 // c += a b over the pieces that count: weights 2^-8(i + j) with i + j < max(NA, NB)
@@ -408,6 +426,12 @@ __device__ __forceinline__ int da_wave_id() { return __builtin_amdgcn_readfirstl
 // its waves the first map, the other the second: half the accumulators each (two or three waves per SIMD, where one wave with both
 // maps fills the registers), and the difference is taken once, at the end, through LDS.  The next tile's elements are on their way in
 // registers while this one's are multiplied; two buffers, one barrier a tile.
+template <int NP> constexpr float DA_LIFT = NP == 2 ? 7.f : 0.f;
+// the stored statistics: without the lift, so that the logarithm keeps its bits
+template <int NP> __device__ __forceinline__ void da_store_stats(float *at, int64_t n, float mx, float sum) {
+  at[0] = sum == 0.f ? 0.f : mx + DA_LIFT<NP>;
+  at[n] = sum == 0.f ? DA_INF : log2f(NP == 2 ? sum * 0.0078125f : sum);  // an empty row: every probability 2^-inf = 0
+}
 template <int NP, int DP, int PAIRS> constexpr int DA_FWD_WAVES = NP == 3 && DP == 64 && PAIRS == 1 ? 1 : 2;  // waves per SIMD
 template <int NP, int DP, int PAIRS, bool SPLIT>
 __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_FWD_WAVES<NP, DP, PAIRS>)) void diff_attn_fwd_k(DaP p) {
@@ -415,7 +439,13 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_FWD_WAVES<NP
   constexpr int NR = DA_NR<NP>, NT = 128 * PAIRS;
   constexpr int NPP = NP == 3 ? 3 : 2;  // pieces of a probability
   constexpr int KC = DP / 16, VB = 2 * DP / 32;
-  constexpr int BUF = Tile::ROWS + Tile::COLS;
+  constexpr bool AHEAD = NP != 3;
+  // fp16 values stay as they are, and so a probability is two fp16 pieces: carried 2^7 times as large (the maximum that is kept, and the sum,
+  // follow), it lies below 2^15 and is off by at most 2^-22 of itself or 2^-32 of the running maximum
+  constexpr int NV = NP == 2 ? 1 : NP;
+  constexpr float LIFT = DA_LIFT<NP>;
+  using VTile = DaTile<NV, DP>;
+  constexpr int BUF = Tile::ROWS + VTile::COLS;
   extern __shared__ __attribute__((aligned(16))) uint16_t da_lds[];
   uint16_t *Ks = da_lds, *Vt = da_lds + Tile::ROWS;
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = da_wave_id(), m = wave & 1, tid = threadIdx.x;
@@ -448,7 +478,7 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_FWD_WAVES<NP
   float mx = -DA_INF, sum = 0.f;
 
   DaFetchRows<NP, DP, NT> fk;
-  DaFetchBlocks<NP, DP, NT> fv;
+  DaFetchBlocks<NV, DP, NT> fv;
   const int64_t k_at = b * p.k_b + hk * p.k_h, v_at = b * p.v_b + hk * p.v_h;
   fk.bind(p.k_m, p.D, true, tid);
   fv.bind(0, p.D, false, tid);
@@ -472,11 +502,19 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_FWD_WAVES<NP
     }
     if (t < lim_hi) {
       f32x16 s = da_zero16();
+      bf16x8 kf[KC][NR], vf[2][VB][NV];
+      auto read_v = [&](int c) {
 #pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        bf16x8 a[NR];
-        Tile::frag_row(Ks, col, m * DP + 16 * c + 8 * half, a);
-        s = da_mfma_in<NP, false>(a, qf[c], s);
+        for (int v = 0; v < VB; ++v) VTile::frag_col(Vt, 32 * v + col, c, half, vf[c][v]);
+      };
+#pragma unroll
+      for (int c = 0; c < KC; ++c) Tile::frag_row(Ks, col, m * DP + 16 * c + 8 * half, kf[c]);
+      if (AHEAD) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int c = 0; c < KC; ++c) s = da_mfma_in<NP, false>(kf[c], qf[c], s);
+      if (AHEAD) {
+        read_v(0);
+        __builtin_amdgcn_sched_barrier(0);
       }
       float pr[16];
       if (t + DA_T > lim_lo) {
@@ -487,7 +525,7 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_FWD_WAVES<NP
       float top = s[0];
 #pragma unroll
       for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
-      top = fmaxf(top, __shfl_xor(top, 32, HITADV_WAVE)) * p.scale2;
+      top = __builtin_fmaf(fmaxf(top, __shfl_xor(top, 32, HITADV_WAVE)), p.scale2, -LIFT);
       if (__ballot(top > mx + DA_SLACK) != 0ull) {  // (-inf + slack = -inf: the first visible key raises it)
         const float nm = fmaxf(mx, top);
         const float f = nm == -DA_INF ? 1.f : exp2_flush(mx - nm);
@@ -507,12 +545,17 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_FWD_WAVES<NP
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         bf16x8 bo[NPP];
-        da_operand<NPP>(&pr[8 * c], bo);
+        if (!AHEAD) read_v(c);
+        if (AHEAD && c == 0) {
+          read_v(1);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (NP == 2) da_operand_f16(&pr[8 * c], bo);
+        else da_operand<NPP>(&pr[8 * c], bo);
 #pragma unroll
         for (int v = 0; v < VB; ++v) {
-          bf16x8 a[NP];
-          Tile::frag_col(Vt, 32 * v + col, c, half, a);
-          o[v] = da_mfma<NP, NPP>(a, bo, o[v]);
+          if constexpr (NP == 2) o[v] = da_mfma_in<NP, false>(vf[c][v], {bo[0]}, da_mfma_in<NP, false>(vf[c][v], {bo[1]}, o[v]));
+          else o[v] = da_mfma<NP, NPP>(vf[c][v], bo, o[v]);
         }
       }
     }
@@ -544,8 +587,7 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_FWD_WAVES<NP
   }
   if (p.stats && valid && half == 0) {
     const int64_t n = (int64_t)p.B * p.H * p.Nq, row = ((int64_t)b * p.H + h) * p.Nq + i;
-    p.stats[(2 * m) * n + row] = sum == 0.f ? 0.f : mx;
-    p.stats[(2 * m + 1) * n + row] = sum == 0.f ? DA_INF : log2f(sum);  // an empty row: every probability 2^-inf = 0
+    da_store_stats<NP>(p.stats + (2 * m) * n + row, n, mx, sum);
   }
   const float w = sum == 0.f ? 0.f : (m && valid ? -da_lam(p, h) : 1.f) / sum;
   // the second map's part of a value block of 32 columns at a time, in the tiles' place (the last barrier is behind their readers)
@@ -596,8 +638,7 @@ __global__ __launch_bounds__(256) void diff_attn_join_k(DaP p) {
       total[wave] = sum == 0.f ? 0.f : (wave ? -da_lam(p, h) : 1.f) / sum;
       if (p.stats) {
         const int64_t n = (int64_t)p.B * p.H * p.Nq, srow = ((int64_t)b * p.H + h) * p.Nq + i;
-        p.stats[(2 * wave) * n + srow] = sum == 0.f ? 0.f : mx;
-        p.stats[(2 * wave + 1) * n + srow] = sum == 0.f ? DA_INF : log2f(sum);
+        da_store_stats<NP>(p.stats + (2 * wave) * n + srow, n, mx, sum);
       }
     }
   }
@@ -1154,7 +1195,7 @@ static DaPlan da_plan(int B, int Nq, int Nk, int H, int Hkv) {
 }
 
 template <int NP, int DP, int PAIRS> static int da_launch_fwd_pairs(const DaP &p, const DaPlan &pl, hipStream_t s) {
-  const int tiles = 4 * (DaTile<NP, DP>::ROWS + DaTile<NP, DP>::COLS), parts = PAIRS * 4096;  // bytes
+  const int tiles = 4 * (DaTile<NP, DP>::ROWS + DaTile<NP == 2 ? 1 : NP, DP>::COLS), parts = PAIRS * 4096;  // bytes
   const int lds = tiles > parts ? tiles : parts;
   const dim3 grid(p.B * p.Hkv, pl.tiles, pl.splits);
   if (pl.splits > 1) {

@@ -236,6 +236,34 @@ def test_diff_attention_extreme_scores_and_scales():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("at", [0, 1500, 4095])
+def test_diff_attention_many_small_probabilities_beside_a_large_one(t, at):
+    """4095 keys with 2^-18 of the largest one's probability carry the whole output (the large one's value is 0), and the large one comes
+    first, in the middle or last; few rows (the keys are split) and many (they are not)."""
+    q, k, v, lam, _ = make(t, 1, 64, 4096, 2, 1, 8, seed=17)
+    q, k = torch.zeros_like(q), torch.zeros_like(k)
+    q[..., 0, 0] = 1.  # (the second map is uniform)
+    k[..., 0, 0] = -12.5
+    k[:, at, :, 0, 0] = 0.
+    v = v.abs()
+    v[:, at] = 0.
+    for Nq in (1, 64):
+        r = attention_reference(q[:, :Nq], k, v, lam * 1e-3, scale=1.)
+        assert float(r.out.min()) > 2.0 ** -8  # (about 0.012)
+        check(ops.diff_attention(q[:, :Nq], k, v, lam * 1e-3, scale=1.), r.out, attention_bounds(t, r, False)["out"] - smallest(t), "%d rows" % Nq)
+
+
+@pytest.mark.gpu
+def test_diff_attention_subnormal_values():
+    """A column that holds one subnormal value everywhere comes out as that value: the mean is off by far less than half of fp16's last step."""
+    q, k, v, _, _ = make(F16, 1, 40, 300, 2, 1, 24, seed=18)
+    v = torch.arange(1, 49, device="cuda").to(F32).mul(2.0 ** -24).to(F16).expand_as(v).contiguous()
+    for Nq in (1, 40):
+        assert torch.equal(ops.diff_attention(q[:, :Nq], k, v, torch.zeros(1, device="cuda")), v[:, :1].expand(1, Nq, 2, 48))
+
+
+@pytest.mark.gpu
 def test_diff_attention_empty_axes():
     for B, Nq, Nk in ((0, 3, 4), (2, 0, 4), (2, 3, 0)):
         q, k, v, lam, g = make(F32, B, Nq, Nk, 2, 1, 8)
