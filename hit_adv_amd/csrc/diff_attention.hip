@@ -425,7 +425,12 @@ __device__ __forceinline__ int da_wave_id() { return __builtin_amdgcn_readfirstl
 // One workgroup: PAIRS pairs of waves over the keys [split chunk, ...) of one (cloud, key / value head); a pair has 32 packed rows, one of
 // its waves the first map, the other the second: half the accumulators each (two or three waves per SIMD, where one wave with both
 // maps fills the registers), and the difference is taken once, at the end, through LDS.  The next tile's elements are on their way in
-// registers while this one's are multiplied; two buffers, one barrier a tile.
+// registers while this one's are multiplied; two buffers, one barrier a tile.  LDS operands are read a phase ahead of their products.
+// Bound by instruction issue: on this chip a SIMD's matrix and vector instructions do not overlap, and a pair of keys costs a map's share of
+// 3 matrix instructions a 16-column block plus two exponentials, two splits and a maximum.  Measured: 2 clouds x 8 heads x 4096 x 4096, D 64,
+// bfloat16: 370 us (137 GFLOP of the formula: 371 TFLOP/s; 556 with the second piece's products), causal 203; 8 clouds x 8 heads (2 shared) x
+// 1000, D 48, fp16: 95 us with three fifths of the keys; 32 x 4 x 256 x 256, D 32, fp32: 27 us (six products for one); 16 tokens x 16 heads
+// over 8192 keys of 4 heads, split: 38 us = 4.4 TB/s of cache, and 6 us for the join.
 template <int NP> constexpr float DA_LIFT = NP == 2 ? 7.f : 0.f;
 // the stored statistics: without the lift, so that the logarithm keeps its bits
 template <int NP> __device__ __forceinline__ void da_store_stats(float *at, int64_t n, float mx, float sum) {
@@ -613,7 +618,8 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_FWD_WAVES<NP
   }
 }
 
-// joins the splits of a row: waves 0 and 1 weigh a map's splits each, then a thread has a (map, value column), eight splits in flight
+// joins the splits of a row: waves 0 and 1 weigh a map's splits each, then a thread has a (map, value column), eight splits in flight (one at
+// a time: 18.8 us against 6.0 for 256 rows of 32 splits, 2 x 128 columns)
 constexpr int DA_MAX_SPLITS = 1024;
 template <int NP>
 __global__ __launch_bounds__(256) void diff_attn_join_k(DaP p) {
@@ -668,13 +674,69 @@ __global__ __launch_bounds__(256) void diff_attn_join_k(DaP p) {
   }
 }
 
+// The same for few splits of many rows, where a workgroup a row is mostly its own launch: a thread has four columns of a row and both maps, four
+// splits in flight, and weighs the splits for itself.  16384 rows of 3 splits 11 us against 29 with a workgroup each; 256 rows of 16 splits
+// 11.8 us against 4.9, so up to 8.
+constexpr int DA_FEW_SPLITS = 8;
+template <int NP>
+__global__ __launch_bounds__(256) void diff_attn_join_few_k(DaP p) {
+  const int w = p.D / 2, at4 = blockIdx.x * 256 + threadIdx.x, r = at4 / w, c = 4 * (at4 - r * w), bh = blockIdx.y;
+  if (r >= p.rows) return;
+  const int b = bh / p.Hkv, hk = bh % p.Hkv, i = da_div_g(p, r), h = hk * p.G + r - i * p.G;
+  const int64_t step = (int64_t)p.B * p.Hkv * p.rows, row = (int64_t)bh * p.rows + r;
+  const float4 *ml = (const float4 *)p.part_ml + row;  // maximum and sum of map 1, of map 2
+  const float *po = p.part_o + 4 * row * p.D + c;
+  float mx[2] = {-DA_INF, -DA_INF}, sum[2] = {0.f, 0.f}, o[2][4] = {};
+  for (int s = 0; s < p.splits; ++s) {
+    const float4 x = ml[s * step];
+    mx[0] = fmaxf(mx[0], x.x);
+    mx[1] = fmaxf(mx[1], x.z);
+  }
+  const float base0 = mx[0] == -DA_INF ? 0.f : mx[0], base1 = mx[1] == -DA_INF ? 0.f : mx[1];
+  for (int s0 = 0; s0 < p.splits; s0 += 4) {
+    float4 x[4], y[4][2];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int s = min(s0 + u, p.splits - 1);
+      x[u] = ml[s * step];
+      y[u][0] = *(const float4 *)(po + s * step * 4 * p.D);
+      y[u][1] = *(const float4 *)(po + s * step * 4 * p.D + 2 * p.D);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (s0 + u >= p.splits) break;
+      const float f[2] = {exp2_flush(x[u].x - base0), exp2_flush(x[u].z - base1)};  // a split that saw nothing: 2^-inf = 0
+      sum[0] += x[u].y * f[0];
+      sum[1] += x[u].w * f[1];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        o[m][0] += y[u][m].x * f[m];
+        o[m][1] += y[u][m].y * f[m];
+        o[m][2] += y[u][m].z * f[m];
+        o[m][3] += y[u][m].w * f[m];
+      }
+    }
+  }
+  const float t0 = sum[0] == 0.f ? 0.f : 1.f / sum[0], t1 = sum[1] == 0.f ? 0.f : -da_lam(p, h) / sum[1];
+  da_store4<NP>(p.out, (((int64_t)b * p.Nq + i) * p.H + h) * 2 * p.D + c, o[0][0] * t0 + o[1][0] * t1, o[0][1] * t0 + o[1][1] * t1,
+                o[0][2] * t0 + o[1][2] * t1, o[0][3] * t0 + o[1][3] * t1);
+  if (p.stats && c == 0) {
+    const int64_t n = (int64_t)p.B * p.H * p.Nq, srow = ((int64_t)b * p.H + h) * p.Nq + i;
+    da_store_stats<NP>(p.stats + srow, n, mx[0], sum[0]);
+    da_store_stats<NP>(p.stats + 2 * n + srow, n, mx[1], sum[1]);
+  }
+}
+
 // ---------------------------------------------------------------------------------------------------------------- backward
 // dP = dO V^T;  r_m = sum_j P_m dP;  dS_1 = P_1 (dP - r_1), dS_2 = -lam P_2 (dP - r_2).  The r are sums over the very P and dP that the
 // second pass multiplies (not dO . out: out is rounded, and where a row sees one key dS has to vanish exactly).
 //
 // dQ: the forward kernel's layout, two passes over the keys: first r, then dQ_m^T = K_m^T dS_m^T.
 // A pair of waves shares 32 packed rows and takes the even and the odd tiles of 32 keys; the two meet in LDS (r behind the first pass, dQ at
-// the end): half the longest row's way through the keys, and twice the waves where clouds are few or short.
+// the end): half the longest row's way through the keys, and twice the waves where clouds are few or short.  Bound by instruction issue:
+// 24 D matrix flop a pair of keys where the formula has 12 (the scores and dP twice, dS as two pieces).  2 x 8 x 4096 x 4096, D 64, bfloat16:
+// 565 us, causal 313 (660 TFLOP/s executed); the one-pass form with r from dO . out loses the exact zero of a row with one key.  32 x 4 x
+// 256, D 32, fp32: 46 us.
 template <int NP, int DP> constexpr int DA_DQ_WAVES = NP == 3 && DP == 64 ? 1 : 2;  // waves per SIMD
 template <int NP, int DP, int PAIRS>
 __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_DQ_WAVES<NP, DP>)) void diff_attn_dq_k(DaP p) {
@@ -901,7 +963,9 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_DQ_WAVES<NP,
 // dK and dV: a wave owns 32 keys (the lane's column) and walks over the packed rows of all G heads, so that the sum over the heads that
 // share a key needs no atomics: dV^T += dO^T A, dK_m^T += Q_m^T dS_m, A = P_1 - lam P_2.  One launch for both, except for fp32 at DP = 64,
 // where three pieces of K and V and both accumulators are more than 512 registers: dV and dK in a launch each (the scores twice, a quarter
-// more products).
+// more products).  Bound by instruction issue and, with one wave a SIMD (the accumulators: 192 registers at DP = 64), by what of a barrier
+// and of LDS latency a wave sees alone.  2 x 8 x 4096 x 4096, D 64, bfloat16: 725 us, causal 399 (517 TFLOP/s executed); 32 x 4 x 256, D 32,
+// fp32: 48 us.
 template <int NP, int DP> constexpr int DA_DKV_WAVES = NP != 3 && DP == 32 ? 2 : 1;  // waves per SIMD
 template <int NP, int DP, int NW, bool DV, bool DK>
 __global__ __launch_bounds__(64 * NW) HITADV_WAVES_PER_SIMD((DA_DKV_WAVES<NP, DP>)) void diff_attn_dkv_k(DaP p) {
@@ -1146,7 +1210,7 @@ __global__ __launch_bounds__(64 * NW) HITADV_WAVES_PER_SIMD((DA_DKV_WAVES<NP, DP
 }
 
 // dlam[h] = -sum over clouds and queries of r_2 (one value for all heads: over the heads too); one workgroup per output, fixed order,
-// sums in double (a long sum of values of both signs)
+// sums in double (a long sum of values of both signs); latency of one pass: 5 us for 32 x 256 rows
 __global__ __launch_bounds__(1024) void diff_attn_dlam_k(const float *__restrict__ r2, int B, int H, int Nq, int lam_n, float *__restrict__ dlam) {
   __shared__ double part[16];
   double s = 0.0;
@@ -1176,13 +1240,19 @@ constexpr int64_t DA_STRIDE = 1 << 24;
 struct DaPlan {
   int pairs, tiles, splits, chunk;
 };
-// Few rows: one pair of waves, the keys split over enough workgroups to fill the chip; else four pairs share a tile of keys.
+// Up to 32 rows: one pair of waves (16 tokens x 16 heads over 8192 keys of 4: one pair 57 us, two 64, four 97).  Else four pairs share the keys'
+// tiles (2 x 8 x 4096 causal: one 322 us, two 246, four 213; 32 x 4 x 256 in fp32: 44, 28, 25), but two where few short rows leave the chip
+// empty (16 x 4 x 128: two 12.0 us, four 13.6; 2 x 4 x 100 rows over 1000 keys 15.0, 17.3).
+// Below 2048 waves the keys are split so that the chip fills (the tokens over 8192 keys: one part 308 us, 16 parts 48, 32 parts 57; 4 x 4096 rows
+// causal: one 138, three 74 + 11 for the join), parts of 256 keys at least (5 tokens over 3000 keys: 256 keys a part 15.2 us, 512 24.2), of 512
+// with four pairs, where the join of many rows costs what the parts save (8 x 4 x 512 rows over 512 keys: one part 28 us, two 28 and the join).
 static DaPlan da_plan(int B, int Nq, int Nk, int H, int Hkv) {
   DaPlan pl;
   const int64_t rows = (int64_t)Nq * (H / Hkv), bh = (int64_t)B * Hkv;
-  pl.pairs = rows <= DA_T ? 1 : bh * ((rows + 4 * DA_T - 1) / (4 * DA_T)) < 512 ? 2 : 4;
+  pl.pairs = rows <= DA_T ? 1 : rows <= 8 * DA_T && bh * ((rows + 4 * DA_T - 1) / (4 * DA_T)) < 256 ? 2 : 4;
   pl.tiles = (int)((rows + DA_T * pl.pairs - 1) / (DA_T * pl.pairs));
-  const int64_t waves = bh * pl.tiles * pl.pairs * 2, want = (4096 + waves - 1) / waves, most = (Nk + 255) / 256;
+  const int64_t waves = bh * pl.tiles * pl.pairs * 2, want = ((pl.pairs == 1 ? 2048 : 3072) + waves - 1) / waves;
+  const int64_t most = pl.pairs == 4 ? (Nk + 511) / 512 : (Nk + 255) / 256;
   int64_t s = waves >= 2048 ? 1 : want < most ? want : most;
   if (s < 1) s = 1;
   if (s > DA_MAX_SPLITS) s = DA_MAX_SPLITS;
@@ -1202,7 +1272,8 @@ template <int NP, int DP, int PAIRS> static int da_launch_fwd_pairs(const DaP &p
     HITADV_RAISE_LDS((diff_attn_fwd_k<NP, DP, PAIRS, true>), lds);
     diff_attn_fwd_k<NP, DP, PAIRS, true><<<grid, 128 * PAIRS, lds, s>>>(p);
     HITADV_LAUNCH_CHECK();
-    diff_attn_join_k<NP><<<dim3(p.rows, p.B * p.Hkv), 256, 0, s>>>(p);
+    if (pl.splits <= DA_FEW_SPLITS) diff_attn_join_few_k<NP><<<dim3((p.rows * (p.D / 2) + 255) / 256, p.B * p.Hkv), 256, 0, s>>>(p);
+    else diff_attn_join_k<NP><<<dim3(p.rows, p.B * p.Hkv), 256, 0, s>>>(p);
   } else {
     HITADV_RAISE_LDS((diff_attn_fwd_k<NP, DP, PAIRS, false>), lds);
     diff_attn_fwd_k<NP, DP, PAIRS, false><<<grid, 128 * PAIRS, lds, s>>>(p);

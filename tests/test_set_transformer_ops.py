@@ -156,6 +156,20 @@ def test_diff_attention_and_its_gradients(t, case):
         check(got, getattr(r, name), b[name], name)
 
 
+MANY_ROWS_SPLIT = [  # few parts of the keys, joined for many rows at once
+    (1, 70, 1100, 4, 2, 40, True, (1037,), None),
+    (2, 300, 1500, 2, 2, 64, False, (1500, 0), 1),
+    (1, 33, 600, 3, 3, 8, True, None, None),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("case", MANY_ROWS_SPLIT, ids=lambda c: "x".join(str(v) for v in c[:6]))
+def test_diff_attention_many_rows_over_split_keys(t, case):
+    test_diff_attention_and_its_gradients(t, case)
+
+
 @pytest.mark.gpu
 def test_diff_attention_gradients_against_differences():
     """Directional derivatives of sum(out g) by central differences of the 64-bit definition (independent of the backward formulas above)."""
