@@ -13,7 +13,7 @@
 // forward kernel.)  The map itself is two pieces (three in fp32) also where the inputs are bf16:
 // rounding P_1 and P_2 to one bf16 each before their difference is taken puts back the noise that the difference is there to cancel,
 // and one-piece dS and A = P_1 - lam P_2 put the gradients at 1.5x the error of their own last rounding (two: 1.0x).  Maxima, sums
-// and accumulators are fp32.  A value that is not finite makes the rows that see it NaN.
+// and accumulators are fp32.  A value that is not finite leaves no finite row that sees it.
 //
 // Layout.  All products are computed transposed so that no map ever leaves the registers: S^T = K Q^T has the query in the lane (column
 // lane & 31) and 16 keys in its registers, which is -- with the keys of a 16-chunk in the order 4h..4h+3, 8+4h..8+4h+3 for lane half h --
@@ -429,8 +429,8 @@ __device__ __forceinline__ int da_wave_id() { return __builtin_amdgcn_readfirstl
 // Bound by instruction issue: on this chip a SIMD's matrix and vector instructions do not overlap, and a pair of keys costs a map's share of
 // 3 matrix instructions a 16-column block plus two exponentials, two splits and a maximum.  Measured: 2 clouds x 8 heads x 4096 x 4096, D 64,
 // bfloat16: 370 us (137 GFLOP of the formula: 371 TFLOP/s; 556 with the second piece's products), causal 203; 8 clouds x 8 heads (2 shared) x
-// 1000, D 48, fp16: 95 us with three fifths of the keys; 32 x 4 x 256 x 256, D 32, fp32: 27 us (six products for one); 16 tokens x 16 heads
-// over 8192 keys of 4 heads, split: 38 us = 4.4 TB/s of cache, and 6 us for the join.
+// 1000, D 48, fp16: 95 us with three fifths of the keys; 32 x 4 x 256 x 256, D 32, fp32: 24 us (six products for one); 16 tokens x 16 heads
+// over 8192 keys of 4 heads, in 16 parts: 43 us = 6.2 TB/s of cache, and 4.4 us for the join.
 template <int NP> constexpr float DA_LIFT = NP == 2 ? 7.f : 0.f;
 // the stored statistics: without the lift, so that the logarithm keeps its bits
 template <int NP> __device__ __forceinline__ void da_store_stats(float *at, int64_t n, float mx, float sum) {
@@ -1251,7 +1251,7 @@ static DaPlan da_plan(int B, int Nq, int Nk, int H, int Hkv) {
   const int64_t rows = (int64_t)Nq * (H / Hkv), bh = (int64_t)B * Hkv;
   pl.pairs = rows <= DA_T ? 1 : rows <= 8 * DA_T && bh * ((rows + 4 * DA_T - 1) / (4 * DA_T)) < 256 ? 2 : 4;
   pl.tiles = (int)((rows + DA_T * pl.pairs - 1) / (DA_T * pl.pairs));
-  const int64_t waves = bh * pl.tiles * pl.pairs * 2, want = ((pl.pairs == 1 ? 2048 : 3072) + waves - 1) / waves;
+  const int64_t waves = bh * pl.tiles * pl.pairs * 2, want = ((pl.pairs == 1 ? 2048 : 3000) + waves - 1) / waves;
   const int64_t most = pl.pairs == 4 ? (Nk + 511) / 512 : (Nk + 255) / 256;
   int64_t s = waves >= 2048 ? 1 : want < most ? want : most;
   if (s < 1) s = 1;

@@ -682,7 +682,7 @@ int hitadv_row_sqnorm(const float *X, int64_t rows, int D, float *xx, void *stre
  *   (clamped to 0 .. Nk; what lies behind it is not used, whatever it holds); causal: also only at j <= i + Nk - Nq.
  *   out [B,Nq,H,2D] dtype, contiguous, 16-byte aligned; a row that sees no key is 0.
  *   stats: NULL, or [4,B,H,Nq] fp32 for the backward pass (maximum and log2 of the sum of either map's row).
- *   scratch: hitadv_diff_attention_scratch_floats(...) floats, 16-byte aligned (0: NULL is fine): few rows over many keys are split.
+ *   scratch: hitadv_diff_attention_scratch_floats(...) floats, 16-byte aligned (0: NULL is fine): where rows are too few to fill the chip the keys are split.
  * backward: dout [B,Nq,H,2D] contiguous; r [2,B,H,Nq] fp32 scratch; dq, dk, dv contiguous in the shapes of q, k, v (dk, dv summed over a
  *   group's heads; 0 behind the lengths; both or neither may be NULL); dlam [lam_n] fp32, or NULL if not wanted.  Every sum in a fixed order: no atomics.
  * D a multiple of 8 up to 64, H a multiple of Hkv; hitadv_diff_attention_supported says whether the sizes are taken (rows Nq G and Nk up
