@@ -10,7 +10,7 @@
 // meet in LDS, those of the grid in a second small kernel, both in a fixed order (no atomics).  Sums are fp32.
 //
 // Measured, 16384 rows of 4096 bfloat16: forward with residual 92 us = 5.8 TB/s, 8-bit output with residual 98 us = 4.8 TB/s, backward 113 us
-// = 4.8 TB/s and its second kernel 5 us (a copy of 2 GiB: 4.9 TB/s).  8192 rows of 256 fp32: forward 5.8, backward 6.5 + 4.8 us.
+// = 4.8 TB/s and its second kernel 12 us (a copy of 2 GiB: 4.9 TB/s).  8192 rows of 256 fp32: forward 5.8, backward 6.5 + 4.8 us.
 #include "elements.hpp"
 #include "hitadv.h"
 
