@@ -124,6 +124,12 @@ template <int N> __device__ __forceinline__ void da_sign(uint4 (&w)[N], const Da
   for (int k = 0; k < N; ++k)
     w[k] = make_uint4((w[k].x & p.s_and) ^ p.s_xor, (w[k].y & p.s_and) ^ p.s_xor, (w[k].z & p.s_and) ^ p.s_xor, (w[k].w & p.s_and) ^ p.s_xor);
 }
+// dP's operand, its sign turned in every other tile of keys
+template <int N> __device__ __forceinline__ void da_turn(uint4 (&w)[N], bool neg) {
+  const uint32_t x = neg ? 0x80008000u : 0u;
+#pragma unroll
+  for (int k = 0; k < N; ++k) w[k] = make_uint4(w[k].x ^ x, w[k].y ^ x, w[k].z ^ x, w[k].w ^ x);
+}
 // the pieces of four rows of four values, [row][column][piece]
 template <int NP> __device__ __forceinline__ void da_pieces4x4(const Raw4<NP> (&r)[4], uint32_t (&p)[4][4][NP]) {
 #pragma unroll
@@ -760,8 +766,12 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_DQ_WAVES<NP,
   const int ph = wave / PAIRS;  // the parity that the wave stages
   uint16_t *Kp = da_lds + ph * SET, *Vp = Kp + Tile::ROWS, *Tp = Vp + Tile::ROWS;
 
+  // every other tile of keys takes dP with its sign turned: the matrix instruction truncates downwards, and the offsets cancel in r (with one
+  // sign dlam of 7 x 2 heads x 1987 rows in bf16 is 1.8e-6 off)
+  const bool neg = odd != 0;
+  const float sgn = neg ? -1.f : 1.f;
   bf16x8 qf[2][KC][NR], gf[VC][NR];
-  float mx[2], ll[2], rs[2] = {0.f, 0.f};
+  float mx[2], ll[2], rs[2] = {0.f, 0.f}, back[2] = {1.f, 1.f};
   int lim;
   {
     const int r = row0 + col, i = da_div_g(p, r), h = hk * p.G + r - i * p.G;
@@ -784,6 +794,7 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_DQ_WAVES<NP,
       const int d = 16 * c + 8 * half;
       uint4 w[NR];
       da_pieces8<NP>(da_load8_if<NP>(p.dout, (((int64_t)b * p.Nq + i) * p.H + h) * 2 * p.D + d, valid && d < 2 * p.D), w);
+      da_turn(w, neg);
 #pragma unroll
       for (int k = 0; k < NR; ++k) gf[c][k] = as_bf16x8(w[k]);
     }
@@ -791,7 +802,13 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_DQ_WAVES<NP,
     for (int m = 0; m < 2; ++m) {
       mx[m] = valid ? p.stats[(2 * m) * n + srow] : 0.f;
       ll[m] = valid ? p.stats[(2 * m + 1) * n + srow] : DA_INF;
-      if (NP != 3) mx[m] += ll[m];  // one subtraction less; fp32 keeps the two apart: their sum's last bit is a probability's error
+      if (NP != 3) {
+        // one subtraction less (fp32 keeps the two apart).  What the sum rounds off is the row's factor 2^-off, which r gets back: dlam adds r over
+        // all rows
+        const float c = mx[m] + ll[m], y = c - mx[m], off = (mx[m] - (c - y)) + (ll[m] - y);
+        back[m] = ll[m] == DA_INF ? 1.f : 1.f - 0.69314718f * off;
+        mx[m] = c;
+      }
     }
   }
   f32x16 acc[2][DB];
@@ -855,7 +872,7 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_DQ_WAVES<NP,
 #pragma unroll
         for (int e = 0; e < 16; ++e) dp[e] += small[e];
       }
-      if (!SECOND && t == 0 && half == 0) red[(pair * 3 + 2) * 32 + col] = dp[0];  // key 0
+      if (!SECOND && t == 0 && half == 0) red[(pair * 3 + 2) * 32 + col] = sgn * dp[0];  // key 0
       const bool edge = t + DA_T > lim_lo;
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
@@ -908,13 +925,14 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_DQ_WAVES<NP,
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     rs[m] += __shfl_xor(rs[m], 32, HITADV_WAVE);
-    if (half == 0) red[((odd * PAIRS + pair) * 3 + m) * 32 + col] = rs[m];
+    if (half == 0) red[((odd * PAIRS + pair) * 3 + m) * 32 + col] = sgn * rs[m];
   }
   __syncthreads();
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    rs[m] = red[(pair * 3 + m) * 32 + col] + red[((PAIRS + pair) * 3 + m) * 32 + col];
+    rs[m] = (red[(pair * 3 + m) * 32 + col] + red[((PAIRS + pair) * 3 + m) * 32 + col]) * back[m];
     if (lim == 1) rs[m] = red[(pair * 3 + 2) * 32 + col];  // a row with one key: its probability is 1, dP - r exactly 0
+    rs[m] *= sgn;
   }
   sweep(std::true_type());
   // the odd wave's dQ, a block of 32 columns at a time, in the tiles' place
@@ -934,7 +952,7 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_DQ_WAVES<NP,
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float4 y = part[64 * e];
-          acc[m][v][4 * e] += y.x, acc[m][v][4 * e + 1] += y.y, acc[m][v][4 * e + 2] += y.z, acc[m][v][4 * e + 3] += y.w;
+          acc[m][v][4 * e] -= y.x, acc[m][v][4 * e + 1] -= y.y, acc[m][v][4 * e + 2] -= y.z, acc[m][v][4 * e + 3] -= y.w;  // (turned)
         }
       }
     }
@@ -943,13 +961,13 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_DQ_WAVES<NP,
   if (r >= p.rows) return;
   if (ln < 32) {
     const int64_t srow = ((int64_t)b * p.H + h) * p.Nq + i;
-    p.r[srow] = rs[0];
-    p.r[n + srow] = rs[1];
+    p.r[srow] = sgn * rs[0];
+    p.r[n + srow] = sgn * rs[1];
   }
   const int64_t at = (((int64_t)b * p.Nq + i) * p.H + h) * 2 * p.D;
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    const float w = m == 0 ? p.scale : -da_lam(p, h) * p.scale;
+    const float w = sgn * (m == 0 ? p.scale : -da_lam(p, h) * p.scale);
 #pragma unroll
     for (int v = 0; v < DB; ++v)
 #pragma unroll
@@ -983,6 +1001,8 @@ __global__ __launch_bounds__(64 * NW) HITADV_WAVES_PER_SIMD((DA_DKV_WAVES<NP, DP
   const int len = da_len(p, b);
   const int64_t n = (int64_t)p.B * p.H * p.Nq;
 
+  const bool neg = (key0 / DA_T & 1) != 0;  // (as in diff_attn_dq_k)
+  const float sgn = neg ? -1.f : 1.f;
   bf16x8 kf[2][KC][NR], vf[VC][NR];
 #pragma unroll
   for (int m = 0; m < 2; ++m)
@@ -1000,6 +1020,7 @@ __global__ __launch_bounds__(64 * NW) HITADV_WAVES_PER_SIMD((DA_DKV_WAVES<NP, DP
     const int d = 16 * c + 8 * half;
     uint4 w[NR];
     da_pieces8<NP>(da_load8_if<NP>(p.v, b * p.v_b + key * p.v_n + hk * p.v_h + d, key < len && d < 2 * p.D), w);
+    da_turn(w, neg);
 #pragma unroll
     for (int k = 0; k < NR; ++k) vf[c][k] = as_bf16x8(w[k]);
   }
@@ -1162,7 +1183,8 @@ __global__ __launch_bounds__(64 * NW) HITADV_WAVES_PER_SIMD((DA_DKV_WAVES<NP, DP
         for (int j = 0; j < 4; ++j) A[4 * q + j] = m ? A[4 * q + j] + x[j] : x[j];
         if (DK) {
           const f32x16 &d = dp;
-          x[0] *= d[4 * q] - rr[q].x, x[1] *= d[4 * q + 1] - rr[q].y, x[2] *= d[4 * q + 2] - rr[q].z, x[3] *= d[4 * q + 3] - rr[q].w;
+          x[0] *= __builtin_fmaf(sgn, d[4 * q], -rr[q].x), x[1] *= __builtin_fmaf(sgn, d[4 * q + 1], -rr[q].y);
+          x[2] *= __builtin_fmaf(sgn, d[4 * q + 2], -rr[q].z), x[3] *= __builtin_fmaf(sgn, d[4 * q + 3], -rr[q].w);
         }
       }
 #pragma unroll
