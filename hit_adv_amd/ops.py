@@ -1169,7 +1169,13 @@ def _call_on(t, name, *args):
 
 
 def _at(t):
+    """The address of ``t``, which the caller holds until the launch: a copy made inside the call's own argument list is given up at once, and the
+    next allocation may get its memory before the kernel has read it."""
     return 0 if t is None else t.data_ptr()
+
+
+def _contiguous(t):
+    return None if t is None else t.contiguous()
 
 
 def _typed(t, name, like=None, dtypes=_DTYPE_CODE):
@@ -1240,7 +1246,7 @@ class DiffAttention(torch.autograd.Function):
         need = ctx.needs_input_grad
         if ctx.empty:
             return tuple(torch.zeros_like(t) if need[i] else None for i, t in enumerate((q, k, v, lam))) + (None,) * 4
-        g = _aligned(g)
+        g, lam = _aligned(g), lam.contiguous()
         r = torch.empty(2, B, H, Nq, device=q.device)
         dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
         dk = dv = dlam = None
@@ -1248,7 +1254,7 @@ class DiffAttention(torch.autograd.Function):
             dk, dv = torch.empty(k.shape, device=q.device, dtype=q.dtype), torch.empty(v.shape, device=q.device, dtype=q.dtype)
         if need[3]:
             dlam = torch.empty(lam.shape, device=q.device)
-        _call_on(q, "hitadv_diff_attention_bwd", _DTYPE_CODE[q.dtype], _at(q), _at(k), _at(v), _at(lam.contiguous()), lam.numel(), _at(lengths),
+        _call_on(q, "hitadv_diff_attention_bwd", _DTYPE_CODE[q.dtype], _at(q), _at(k), _at(v), _at(lam), lam.numel(), _at(lengths),
                  ctx.strides, _at(g), _at(stats), B, Nq, Nk, H, Hkv, D, int(ctx.causal), ctx.scale, _at(r), _at(dq), _at(dk), _at(dv),
                  _at(dlam))
         return dq, dk, dv, dlam, None, None, None, None
@@ -1298,7 +1304,7 @@ RMS_NORM_MAX_COLS = 16384
 class RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, eps, residual, keep):
-        x, weight = x.contiguous(), weight.contiguous()
+        x, weight, residual = x.contiguous(), weight.contiguous(), _contiguous(residual)
         C = x.shape[-1]
         rows = x.numel() // C
         y = torch.empty_like(x)
@@ -1306,7 +1312,7 @@ class RmsNorm(torch.autograd.Function):
         rstd = torch.empty(rows, device=x.device) if keep else None
         if rows:
             _call_on(x, "hitadv_rms_norm_fwd", _DTYPE_CODE[x.dtype], _DTYPE_CODE[weight.dtype], _at(x),
-                     _at(residual.contiguous() if residual is not None else None), _at(weight), rows, C, eps, _at(y), _at(total), _at(rstd))
+                     _at(residual), _at(weight), rows, C, eps, _at(y), _at(total), _at(rstd))
         if keep:
             ctx.set_materialize_grads(False)
             ctx.save_for_backward(x if residual is None else total, weight, rstd)
@@ -1319,6 +1325,7 @@ class RmsNorm(torch.autograd.Function):
         need = ctx.needs_input_grad
         if dy is None:
             return dsum if need[0] else None, None, None, dsum if need[3] else None, None
+        dy, dsum = dy.contiguous(), _contiguous(dsum)
         C = s.shape[-1]
         rows = s.numel() // C
         dx = torch.empty_like(s)
@@ -1327,8 +1334,8 @@ class RmsNorm(torch.autograd.Function):
             dw = torch.empty_like(weight)
             scratch = torch.empty(_lib.load().hitadv_rms_norm_bwd_scratch_floats(rows, C), device=s.device)
         if rows:
-            _call_on(s, "hitadv_rms_norm_bwd", _DTYPE_CODE[s.dtype], _DTYPE_CODE[weight.dtype], _at(s), _at(weight), _at(rstd), _at(dy.contiguous()),
-                     _at(dsum.contiguous() if dsum is not None else None), rows, C, _at(dx), _at(scratch), _at(dw))
+            _call_on(s, "hitadv_rms_norm_bwd", _DTYPE_CODE[s.dtype], _DTYPE_CODE[weight.dtype], _at(s), _at(weight), _at(rstd), _at(dy),
+                     _at(dsum), rows, C, _at(dx), _at(scratch), _at(dw))
         elif dw is not None:
             dw.zero_()
         return dx if need[0] else None, dw, None, dx if need[3] else None, None
@@ -1366,7 +1373,7 @@ def rms_norm_quant(x, weight, eps=1e-6, residual=None):
     _rms_args("rms_norm_quant", x, weight, residual)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
         raise RuntimeError("rms_norm_quant has no backward pass: call it under torch.no_grad(), or rms_norm")
-    x, weight = x.contiguous(), weight.contiguous()
+    x, weight, residual = x.contiguous(), weight.contiguous(), _contiguous(residual)
     C = x.shape[-1]
     rows = x.numel() // C
     q = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
@@ -1374,8 +1381,7 @@ def rms_norm_quant(x, weight, eps=1e-6, residual=None):
     total = torch.empty_like(x) if residual is not None else None
     if rows:
         _call_on(x, "hitadv_rms_norm_e4m3", _DTYPE_CODE[x.dtype], _DTYPE_CODE[weight.dtype], _at(x),
-                 _at(residual.contiguous() if residual is not None else None), _at(weight), rows, C, float(eps), _at(q), _at(scale),
-                 _at(total))
+                 _at(residual), _at(weight), rows, C, float(eps), _at(q), _at(scale), _at(total))
     return (q, scale) if residual is None else (q, scale, total)
 
 

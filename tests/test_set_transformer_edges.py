@@ -1,0 +1,156 @@
+"""ops.diff_attention, rms_norm, rms_norm_quant and dropout at calls where a wrapper, rather than a kernel, can go wrong.  The CPU tests run the
+package's own functions on the kernels' source on the wave emulator: every launch is checked for what its addresses belong to."""
+import ctypes
+import os
+import sys
+import weakref
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, os.path.join(ROOT, "tests", "native"))
+import emu_build  # noqa: E402
+from hit_adv_amd import _lib, ops  # noqa: E402
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+emulator = pytest.mark.skipif(not os.path.exists(emu_build.CLANGXX), reason="no host clang++")
+
+
+@pytest.fixture(scope="module")
+def emulated(tmp_path_factory):
+    """Functions of the emulated kernel files, built when first asked for."""
+    d, built = str(tmp_path_factory.mktemp("emu")), {}
+
+    def function(name):
+        stem = "diff_attention" if "attention" in name else "rms_norm" if "rms" in name else "dropout"
+        if stem not in built:
+            built[stem] = ctypes.CDLL(emu_build.build(stem, d))
+        f = getattr(built[stem], name)
+        f.argtypes, f.restype = _lib.PROTOTYPES[name], _lib._RESTYPE.get(name, ctypes.c_int)
+        return f
+    return function
+
+
+class Launches:
+    """In ops' place between the wrappers and the library: CPU tensors are taken, and at each launch the tensors whose addresses it got
+    have to be there still (what nobody holds, the allocator may hand out again before the launch)."""
+
+    def __init__(self, emulated, monkeypatch):
+        self.taken, self.names, self.run, self.emulated = [], [], True, emulated
+        monkeypatch.setattr(ops, "_typed", self.typed)
+        monkeypatch.setattr(ops, "_at", self.at)
+        monkeypatch.setattr(ops, "_call_on", self.launch)
+
+    def typed(self, t, name, like=None, dtypes=ops._DTYPE_CODE):
+        assert torch.is_tensor(t) and t.dtype in dtypes, name
+        return t
+
+    def at(self, t):
+        if t is None:
+            return 0
+        self.taken.append((weakref.ref(t), t.dtype, tuple(t.shape)))
+        return t.data_ptr()
+
+    def launch(self, t, name, *args):
+        gone = [(dtype, shape) for r, dtype, shape in self.taken if r() is None]
+        types = {dtype for _, dtype, _ in self.taken}
+        self.taken = []
+        self.names.append(name)
+        assert not gone, "%s: tensors given up before the launch: %s" % (name, gone)
+        self.types(t, name, types)
+        if self.run:
+            assert self.emulated(name)(*args, None) == 0
+
+    def types(self, t, name, types):
+        pass
+
+
+@pytest.fixture
+def launches(emulated, monkeypatch):
+    return Launches(emulated, monkeypatch)
+
+
+def strided(t):
+    """The same values, last axis not contiguous."""
+    return t.transpose(0, 1).contiguous().transpose(0, 1)
+
+
+# ---------------------------------------------------------------------------------------------------------------- gradients' layouts
+def norm_gradients(device, layout_y, layout_s, rows=37, cols=100):
+    g = torch.Generator().manual_seed(3)
+    n = lambda *s: torch.randn(*s, generator=g).to(device)  # noqa: E731
+    x, residual, w = n(rows, cols).requires_grad_(), n(rows, cols).requires_grad_(), n(cols).requires_grad_()
+    gy, gs = n(rows, cols), n(rows, cols)
+    y, s = ops.rms_norm(x, w, residual=residual)
+    return torch.autograd.grad((y, s), (x, residual, w), (layout_y(gy), layout_s(gs)))
+
+
+def same(t):
+    return t
+
+
+LAYOUTS = [(strided, same), (same, strided), (strided, strided)]
+
+
+def norm_sums(device, plain, rows=37, cols=100):
+    """Gradients of y.sum() + 2 s.sum(): autograd hands both to the norm expanded from one value."""
+    g = torch.Generator().manual_seed(4)
+    n = lambda *s: torch.randn(*s, generator=g).to(device)  # noqa: E731
+    x, residual, w = n(rows, cols).requires_grad_(), n(rows, cols).requires_grad_(), n(cols).requires_grad_()
+    y, s = ops.rms_norm(x, w, residual=residual)
+    if plain:
+        return torch.autograd.grad((y, s), (x, residual, w), (torch.ones_like(y), torch.full_like(s, 2.)))
+    return torch.autograd.grad(y.sum() + 2 * s.sum(), (x, residual, w))
+
+
+@emulator
+@pytest.mark.parametrize("layout", LAYOUTS, ids=["y", "sum", "both"])
+def test_norm_gradients_of_any_layout(launches, layout):
+    for a, b in zip(norm_gradients("cpu", *layout), norm_gradients("cpu", same, same)):
+        assert torch.equal(a, b)
+
+
+@emulator
+def test_norm_gradients_of_sums(launches):
+    for a, b in zip(norm_sums("cpu", False), norm_sums("cpu", True)):
+        assert torch.equal(a, b)
+
+
+def test_every_launch_holds_the_copies_it_reads(launches):
+    """Inputs of every operator in a layout that has to be copied first, forward and backward (nothing is launched)."""
+    launches.run = False
+    g = torch.Generator().manual_seed(5)
+    n = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    x, r, w = strided(n(6, 40)).requires_grad_(), strided(n(6, 40)).requires_grad_(), n(40, 2)[:, 0].requires_grad_()
+    y, s = ops.rms_norm(x, w, residual=r)
+    torch.autograd.grad((y, s), (x, r, w), (strided(n(6, 40)), n(1).expand(6, 40)))
+    y = ops.rms_norm(x, w)
+    torch.autograd.grad(y, (x, w), strided(n(6, 40)))
+    with torch.no_grad():
+        ops.rms_norm_quant(x, w, residual=r)
+        ops.rms_norm_quant(x, w)
+    rng = torch.tensor([[1, 2], [3, 4]])[:, 0]
+    torch.autograd.grad(ops.dropout(x, 0.5, rng, residual=r), (x, r), strided(n(6, 40)))
+    q, k, v = (n(2, 5, *tail, 17)[..., :16].requires_grad_() for tail in ((4, 2), (2, 2), (2, 2)))
+    v = n(2, 5, 2, 33)[..., :32].requires_grad_()
+    lam = n(4, 3)[:, 1].requires_grad_()
+    lengths = torch.tensor([[5, 0], [3, 0]])[:, 0]
+    for kl in (lengths, lengths.int()[:], torch.tensor([[5, 0], [3, 0]], dtype=torch.int32)[:, 0]):
+        out = ops.diff_attention(q, k, v, lam, key_lengths=kl)
+        torch.autograd.grad(out, (q, k, v, lam), n(1).expand(out.shape))
+    assert len(launches.names) == 2 + 2 + 2 + 2 + 3 * 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols", [(37, 100), (300, 1000)])
+@pytest.mark.parametrize("layout", LAYOUTS, ids=["y", "sum", "both"])
+def test_norm_gradients_of_any_layout_on_the_gpu(layout, rows, cols):
+    for a, b in zip(norm_gradients("cuda", *layout, rows, cols), norm_gradients("cuda", same, same, rows, cols)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_norm_gradients_of_sums_on_the_gpu():
+    for a, b in zip(norm_sums("cuda", False), norm_sums("cuda", True)):
+        assert torch.equal(a, b)
