@@ -1226,9 +1226,9 @@ class DiffAttention(torch.autograd.Function):
             v, vs = _strided(v)
             ctx.strides = (ctypes.c_int64 * 11)(*qs, *ks, *vs)
             if keep:
-                stats = torch.empty(4, B, H, Nq, device=q.device)
+                stats = torch.empty(4, B, H, Nq, device=q.device, dtype=torch.float32)
             n = _lib.load().hitadv_diff_attention_scratch_floats(B, Nq, Nk, H, Hkv, D)
-            scratch = torch.empty(n, device=q.device) if n else None
+            scratch = torch.empty(n, device=q.device, dtype=torch.float32) if n else None
             lam32 = lam.contiguous()
             _call_on(q, "hitadv_diff_attention_fwd", _DTYPE_CODE[q.dtype], _at(q), _at(k), _at(v), _at(lam32), lam.numel(), _at(lengths), ctx.strides,
                      B, Nq, Nk, H, Hkv, D, int(causal), scale, _at(out), _at(stats), _at(scratch))
@@ -1247,13 +1247,13 @@ class DiffAttention(torch.autograd.Function):
         if ctx.empty:
             return tuple(torch.zeros_like(t) if need[i] else None for i, t in enumerate((q, k, v, lam))) + (None,) * 4
         g, lam = _aligned(g), lam.contiguous()
-        r = torch.empty(2, B, H, Nq, device=q.device)
+        r = torch.empty(2, B, H, Nq, device=q.device, dtype=torch.float32)
         dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
         dk = dv = dlam = None
         if need[1] or need[2]:
             dk, dv = torch.empty(k.shape, device=q.device, dtype=q.dtype), torch.empty(v.shape, device=q.device, dtype=q.dtype)
         if need[3]:
-            dlam = torch.empty(lam.shape, device=q.device)
+            dlam = torch.empty(lam.shape, device=q.device, dtype=lam.dtype)
         _call_on(q, "hitadv_diff_attention_bwd", _DTYPE_CODE[q.dtype], _at(q), _at(k), _at(v), _at(lam), lam.numel(), _at(lengths),
                  ctx.strides, _at(g), _at(stats), B, Nq, Nk, H, Hkv, D, int(ctx.causal), ctx.scale, _at(r), _at(dq), _at(dk), _at(dv),
                  _at(dlam))
@@ -1309,7 +1309,7 @@ class RmsNorm(torch.autograd.Function):
         rows = x.numel() // C
         y = torch.empty_like(x)
         total = torch.empty_like(x) if residual is not None else None
-        rstd = torch.empty(rows, device=x.device) if keep else None
+        rstd = torch.empty(rows, device=x.device, dtype=torch.float32) if keep else None
         if rows:
             _call_on(x, "hitadv_rms_norm_fwd", _DTYPE_CODE[x.dtype], _DTYPE_CODE[weight.dtype], _at(x),
                      _at(residual), _at(weight), rows, C, eps, _at(y), _at(total), _at(rstd))
@@ -1332,7 +1332,7 @@ class RmsNorm(torch.autograd.Function):
         dw = scratch = None
         if need[1]:
             dw = torch.empty_like(weight)
-            scratch = torch.empty(_lib.load().hitadv_rms_norm_bwd_scratch_floats(rows, C), device=s.device)
+            scratch = torch.empty(_lib.load().hitadv_rms_norm_bwd_scratch_floats(rows, C), device=s.device, dtype=torch.float32)
         if rows:
             _call_on(s, "hitadv_rms_norm_bwd", _DTYPE_CODE[s.dtype], _DTYPE_CODE[weight.dtype], _at(s), _at(weight), _at(rstd), _at(dy),
                      _at(dsum), rows, C, _at(dx), _at(scratch), _at(dw))
@@ -1377,7 +1377,7 @@ def rms_norm_quant(x, weight, eps=1e-6, residual=None):
     C = x.shape[-1]
     rows = x.numel() // C
     q = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
-    scale = torch.empty(x.shape[:-1], device=x.device)
+    scale = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
     total = torch.empty_like(x) if residual is not None else None
     if rows:
         _call_on(x, "hitadv_rms_norm_e4m3", _DTYPE_CODE[x.dtype], _DTYPE_CODE[weight.dtype], _at(x),

@@ -154,3 +154,63 @@ def test_norm_gradients_of_any_layout_on_the_gpu(layout, rows, cols):
 def test_norm_gradients_of_sums_on_the_gpu():
     for a, b in zip(norm_sums("cuda", False), norm_sums("cuda", True)):
         assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------------------------------------------------------- torch's default type
+class _DefaultType:
+    def __init__(self, t):
+        self.t = t
+
+    def __enter__(self):
+        self.before = torch.get_default_dtype()
+        torch.set_default_dtype(self.t)
+
+    def __exit__(self, *_):
+        torch.set_default_dtype(self.before)
+
+
+def every_operator(device, t):
+    """Outputs and gradients of each operator in type t (attention: keys split and not)."""
+    g = torch.Generator().manual_seed(6)
+    n = lambda *s: torch.randn(*s, generator=g, dtype=F32).to(t).to(device)  # noqa: E731
+    x, r, w = n(9, 72).requires_grad_(), n(9, 72).requires_grad_(), n(72).float().requires_grad_()
+    y, s = ops.rms_norm(x, w, residual=r)
+    res = [y, s, *torch.autograd.grad((y, s), (x, r, w), (n(9, 72), n(9, 72)))]
+    with torch.no_grad():
+        res += ops.rms_norm_quant(x, w, residual=r)
+    y = ops.dropout(x, 0.5, torch.tensor([1, 2], device=device), residual=r)
+    res += [y, *torch.autograd.grad(y, (x, r), n(9, 72))]
+    for Nq, Nk in ((7, 40), (2, 600)):
+        q, k, v = n(2, Nq, 2, 2, 16).requires_grad_(), n(2, Nk, 1, 2, 16).requires_grad_(), n(2, Nk, 1, 32).requires_grad_()
+        lam = torch.tensor([0.25, 0.5], dtype=F32, device=device, requires_grad=True)
+        out = ops.diff_attention(q, k, v, lam, causal=True)
+        res += [out, *torch.autograd.grad(out, (q, k, v, lam), n(2, Nq, 2, 32))]
+    return res
+
+
+@emulator
+@pytest.mark.parametrize("t,default", [(F32, torch.float64), (F32, BF16), (BF16, F16), (F16, BF16)])  # (a buffer of t itself could not be told)
+def test_buffers_do_not_follow_the_default_type(launches, t, default):
+    """A program that works with torch.set_default_dtype(bfloat16) gets the same bits: the kernels' own buffers are fp32 whatever it says (half as
+    large, a launch would write behind them: the sizes are checked before it)."""
+    want = every_operator("cpu", t)
+
+    def types(tensor, name, seen):
+        assert seen <= {t, F32, torch.int32, torch.int64, torch.float8_e4m3fn}, "%s: %s" % (name, seen)
+    launches.types = types
+    with _DefaultType(default):
+        got = every_operator("cpu", t)
+    assert launches.names[:len(launches.names) // 2] == launches.names[len(launches.names) // 2:]
+    for a, b in zip(got, want):
+        assert a.dtype == b.dtype and torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("default", [torch.float64, BF16, F16])
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+def test_buffers_do_not_follow_the_default_type_on_the_gpu(t, default):
+    want = every_operator("cuda", t)
+    with _DefaultType(default):
+        got = every_operator("cuda", t)
+    for a, b in zip(got, want):
+        assert a.dtype == b.dtype and torch.equal(a.view(torch.uint8), b.view(torch.uint8))
