@@ -13,7 +13,9 @@
 // forward kernel.)  The map itself is two pieces (three in fp32) also where the inputs are bf16:
 // rounding P_1 and P_2 to one bf16 each before their difference is taken puts back the noise that the difference is there to cancel,
 // and one-piece dS and A = P_1 - lam P_2 put the gradients at 1.5x the error of their own last rounding (two: 1.0x).  Maxima, sums
-// and accumulators are fp32.  A value that is not finite leaves no finite row that sees it.
+// and accumulators are fp32.  A row is empty if its limit says so, not if its sum is 0: where every visible score is -inf (an infinite query or
+// key, a product beyond fp32) softmax is 0 / 0 and the row NaN.  One score of -inf is a probability of 0 in 16-bit types; the pieces of an
+// infinity in fp32 are NaN.  Any other visible value that is not finite makes the row not finite.
 //
 // Layout.  All products are computed transposed so that no map ever leaves the registers: S^T = K Q^T has the query in the lane (column
 // lane & 31) and 16 keys in its registers, which is -- with the keys of a 16-chunk in the order 4h..4h+3, 8+4h..8+4h+3 for lane half h --
@@ -439,9 +441,9 @@ __device__ __forceinline__ int da_wave_id() { return __builtin_amdgcn_readfirstl
 // over 8192 keys of 4 heads, in 16 parts: 43 us = 6.2 TB/s of cache, and 4.4 us for the join.
 template <int NP> constexpr float DA_LIFT = NP == 2 ? 7.f : 0.f;
 // the stored statistics: without the lift, so that the logarithm keeps its bits
-template <int NP> __device__ __forceinline__ void da_store_stats(float *at, int64_t n, float mx, float sum) {
-  at[0] = sum == 0.f ? 0.f : mx + DA_LIFT<NP>;
-  at[n] = sum == 0.f ? DA_INF : log2f(NP == 2 ? sum * 0.0078125f : sum);  // an empty row: every probability 2^-inf = 0
+template <int NP> __device__ __forceinline__ void da_store_stats(float *at, int64_t n, float mx, float sum, bool empty) {
+  at[0] = empty ? 0.f : mx + DA_LIFT<NP>;
+  at[n] = empty ? DA_INF : log2f(NP == 2 ? sum * 0.0078125f : sum);  // an empty row: every probability 2^-inf = 0
 }
 template <int NP, int DP, int PAIRS> constexpr int DA_FWD_WAVES = NP == 3 && DP == 64 && PAIRS == 1 ? 1 : 2;  // waves per SIMD
 template <int NP, int DP, int PAIRS, bool SPLIT>
@@ -598,9 +600,9 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_FWD_WAVES<NP
   }
   if (p.stats && valid && half == 0) {
     const int64_t n = (int64_t)p.B * p.H * p.Nq, row = ((int64_t)b * p.H + h) * p.Nq + i;
-    da_store_stats<NP>(p.stats + (2 * m) * n + row, n, mx, sum);
+    da_store_stats<NP>(p.stats + (2 * m) * n + row, n, mx, sum, lim == 0);
   }
-  const float w = sum == 0.f ? 0.f : (m && valid ? -da_lam(p, h) : 1.f) / sum;
+  const float w = lim == 0 ? 0.f : (m && valid ? -da_lam(p, h) : 1.f) / sum;
   // the second map's part of a value block of 32 columns at a time, in the tiles' place (the last barrier is behind their readers)
   float4 *part = (float4 *)da_lds + (wave >> 1) * 256 + lane;
   const int64_t at = (((int64_t)b * p.Nq + i) * p.H + h) * 2 * p.D;
@@ -647,10 +649,11 @@ __global__ __launch_bounds__(256) void diff_attn_join_k(DaP p) {
     }
     sum = wave_sum(sum);
     if (lane == 0) {
-      total[wave] = sum == 0.f ? 0.f : (wave ? -da_lam(p, h) : 1.f) / sum;
+      const bool empty = da_limit(p, i, da_len(p, b)) == 0;
+      total[wave] = empty ? 0.f : (wave ? -da_lam(p, h) : 1.f) / sum;
       if (p.stats) {
         const int64_t n = (int64_t)p.B * p.H * p.Nq, srow = ((int64_t)b * p.H + h) * p.Nq + i;
-        da_store_stats<NP>(p.stats + (2 * wave) * n + srow, n, mx, sum);
+        da_store_stats<NP>(p.stats + (2 * wave) * n + srow, n, mx, sum, empty);
       }
     }
   }
@@ -723,13 +726,14 @@ __global__ __launch_bounds__(256) void diff_attn_join_few_k(DaP p) {
       }
     }
   }
-  const float t0 = sum[0] == 0.f ? 0.f : 1.f / sum[0], t1 = sum[1] == 0.f ? 0.f : -da_lam(p, h) / sum[1];
+  const bool empty = da_limit(p, i, da_len(p, b)) == 0;
+  const float t0 = empty ? 0.f : 1.f / sum[0], t1 = empty ? 0.f : -da_lam(p, h) / sum[1];
   da_store4<NP>(p.out, (((int64_t)b * p.Nq + i) * p.H + h) * 2 * p.D + c, o[0][0] * t0 + o[1][0] * t1, o[0][1] * t0 + o[1][1] * t1,
                 o[0][2] * t0 + o[1][2] * t1, o[0][3] * t0 + o[1][3] * t1);
   if (p.stats && c == 0) {
     const int64_t n = (int64_t)p.B * p.H * p.Nq, srow = ((int64_t)b * p.H + h) * p.Nq + i;
-    da_store_stats<NP>(p.stats + srow, n, mx[0], sum[0]);
-    da_store_stats<NP>(p.stats + 2 * n + srow, n, mx[1], sum[1]);
+    da_store_stats<NP>(p.stats + srow, n, mx[0], sum[0], empty);
+    da_store_stats<NP>(p.stats + 2 * n + srow, n, mx[1], sum[1], empty);
   }
 }
 

@@ -680,7 +680,7 @@ int hitadv_row_sqnorm(const float *X, int64_t rows, int D, float *xx, void *stre
  *   queries, keys and maps below 2^24;
  *   lam fp32 [H], or one value for all heads (lam_n = H or 1); lengths int32 [B] or NULL (device): key j is visible below lengths[b]
  *   (clamped to 0 .. Nk; what lies behind it is not used, whatever it holds); causal: also only at j <= i + Nk - Nq.
- *   out [B,Nq,H,2D] dtype, contiguous, 16-byte aligned; a row that sees no key is 0.
+ *   out [B,Nq,H,2D] dtype, contiguous, 16-byte aligned; a row that sees no key is 0 (one whose visible scores are all -inf is NaN).
  *   stats: NULL, or [4,B,H,Nq] fp32 for the backward pass (maximum and log2 of the sum of either map's row).
  *   scratch: hitadv_diff_attention_scratch_floats(...) floats, 16-byte aligned (0: NULL is fine): where rows are too few to fill the chip the keys are split.
  * backward: dout [B,Nq,H,2D] contiguous; r [2,B,H,Nq] fp32 scratch; dq, dk, dv contiguous in the shapes of q, k, v (dk, dv summed over a

@@ -214,3 +214,97 @@ def test_buffers_do_not_follow_the_default_type_on_the_gpu(t, default):
         got = every_operator("cuda", t)
     for a, b in zip(got, want):
         assert a.dtype == b.dtype and torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+# ---------------------------------------------------------------------------------------------------------------- infinite scores
+INFINITE = [  # rows x keys: one part of the keys, few parts, more than eight
+    (40, 70), (40, 700), (3, 2700)]
+
+
+def infinite_row(device, t, Nq, Nk):
+    """Two heads, causal; in map 1 every score of row 2 of head 1 is -inf (an infinite query against negative keys)."""
+    g = torch.Generator().manual_seed(7)
+    n = lambda *s: torch.randn(*s, generator=g).to(t).to(device)  # noqa: E731
+    q, k, v, go = n(1, Nq, 2, 2, 16), n(1, Nk, 2, 2, 16), n(1, Nk, 2, 32), n(1, Nq, 2, 32)
+    q[..., 0, 0], k[..., 0, 0] = 1., -k[..., 0, 0].abs() - 0.5
+    lam = torch.tensor([0.25, 0.5], dtype=F32, device=device)
+
+    def run(q):
+        leaves = [x.clone().requires_grad_() for x in (q, k, v, lam)]
+        out = ops.diff_attention(*leaves, causal=True)
+        with torch.no_grad():
+            same = ops.diff_attention(*leaves, causal=True)
+        return out, same, torch.autograd.grad(out, leaves, go)
+    bad = q.clone()
+    bad[0, 2, 1, 0, 0] = float("inf")
+    return run(q), run(bad)
+
+
+def check_infinite_row(device, t, Nq, Nk):
+    """softmax of a row of -inf is NaN: the row, and what map 1 of its query, its keys and their values get of it; nothing else is touched."""
+    (out, same, grads), (bad, bad_same, bad_grads) = infinite_row(device, t, Nq, Nk)
+    assert torch.equal(out, same) and bool(out.isfinite().all())
+    keep = torch.ones_like(out, dtype=torch.bool)
+    keep[0, 2, 1] = False
+    for x in (bad, bad_same):
+        assert bool(x[0, 2, 1].isnan().all()) and torch.equal(x[keep], out[keep])
+    dq, dk, dv, dlam = bad_grads
+    seen = Nk - Nq + 3  # row 2's keys; (r = NaN reaches map 1 of the keys behind them)
+    assert bool(dq[0, 2, 1, 0].isnan().all()) and bool(dk[0, :seen, 1, 0].isnan().all()) and bool(dv[0, :seen, 1].isnan().all())
+    keep = torch.ones_like(dq, dtype=torch.bool)
+    keep[0, 2, 1, 0] = False
+    assert torch.equal(dq[keep], grads[0][keep]) and torch.equal(dlam, grads[3])
+    assert torch.equal(dk[:, :, 0], grads[1][:, :, 0]) and torch.equal(dk[:, :, 1, 1], grads[1][:, :, 1, 1])
+    assert torch.equal(dv[:, :, 0], grads[2][:, :, 0]) and torch.equal(dv[:, seen:], grads[2][:, seen:])
+
+
+@emulator
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+def test_a_row_of_infinite_scores_is_nan(launches, t):
+    check_infinite_row("cpu", t, *INFINITE[0])
+    with torch.no_grad():  # the joins: forward
+        for size in INFINITE[1:]:
+            q, k, v = (torch.ones(1, size[i > 0], 1, *((2, 8) if i < 2 else (16,))).to(t) for i in range(3))
+            q[0, 1] = float("inf")
+            out = ops.diff_attention(q, -k, v, torch.tensor(0.5))
+            assert bool(out[0, 1].isnan().all()) and torch.equal(out[0, 0], out[0, 2]) and bool(out[0, 0].isfinite().all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("size", INFINITE, ids=str)
+def test_a_row_of_infinite_scores_is_nan_on_the_gpu(t, size):
+    check_infinite_row("cuda", t, *size)
+
+
+def one_infinite_key(device, t, Nq, Nk):
+    g = torch.Generator().manual_seed(8)
+    n = lambda *s: torch.randn(*s, generator=g).to(t).to(device)  # noqa: E731
+    q, k, v = n(1, Nq, 2, 2, 16), n(1, Nk, 2, 2, 16), n(1, Nk, 2, 32)
+    q[..., 0, 0] = 1.
+    lam = torch.tensor([0.25, 0.5], dtype=F32, device=device)
+    outs = []
+    for value in (-1e4, -float("inf")):  # (a score of -2500: its probability is 0 in fp32)
+        k[0, 5, :, 0, 0] = value
+        outs.append(ops.diff_attention(q, k, v, lam))
+    return outs
+
+
+def check_one_infinite_key(device, t, Nq, Nk):
+    """A key with a score of -inf has probability 0 in 16-bit types; fp32's pieces of an infinity are NaN, and so is the row."""
+    far, infinite = one_infinite_key(device, t, Nq, Nk)
+    assert bool(far.isfinite().all())
+    assert bool(infinite.isnan().all()) if t is F32 else torch.equal(far, infinite)
+
+
+@emulator
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+def test_one_infinite_score(launches, t):
+    check_one_infinite_key("cpu", t, *INFINITE[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("size", INFINITE, ids=str)
+def test_one_infinite_score_on_the_gpu(t, size):
+    check_one_infinite_key("cuda", t, *size)
