@@ -1,7 +1,7 @@
 // Root-mean-square norm of rows, with the residual's addition in front and an 8-bit output with a scale per row behind.
 //
 //     s = x + residual (rounded to the element type: it is an output)      r = 1 / sqrt(mean(s^2) + eps)      y = s r w
-//     8 bits: scale = max |y| / 448 (1 for a row of zeros), q = e4m3(y / scale)
+//     8 bits: scale = max |y| / 448 (1 for a row of zeros; NaN, infinite as the maximum is), q = e4m3(y / scale)
 //     backward, g = dy w:  ds = dsum + r (g - s r^2 mean(g s)),   dw = sum over rows of dy s r
 //
 // All of it is bound by bytes: a row is read once, held in registers as fp32 and written once.  A row belongs to a team of lanes as wide
@@ -27,13 +27,19 @@ struct RnP {
   float eps, inv_cols;
 };
 
-// sum / maximum over a team of lanes; `red`: LDS of one float per wave (teams wider than a wave)
+// the larger of two values >= +0, NaN if one is (compared as integers, where NaN lies above infinity)
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+  return __uint_as_float(x > y ? x : y);
+}
+
+// sum / maximum (of values >= +0, NaN kept) over a team of lanes; `red`: LDS of one float per wave (teams wider than a wave)
 template <int TEAM, bool MAX> __device__ __forceinline__ float team_reduce(float v, float *red) {
   constexpr int W = TEAM < 64 ? TEAM : 64;
 #pragma unroll
   for (int m = W / 2; m >= 1; m >>= 1) {
     const float o = __shfl_xor(v, m, HITADV_WAVE);
-    v = MAX ? fmaxf(v, o) : v + o;
+    v = MAX ? max_or_nan(v, o) : v + o;
   }
   if constexpr (TEAM > 64) {
     __syncthreads();  // the last reduction's readers are done
@@ -41,7 +47,7 @@ template <int TEAM, bool MAX> __device__ __forceinline__ float team_reduce(float
     __syncthreads();
     v = red[0];
 #pragma unroll
-    for (int i = 1; i < TEAM / 64; ++i) v = MAX ? fmaxf(v, red[i]) : v + red[i];
+    for (int i = 1; i < TEAM / 64; ++i) v = MAX ? max_or_nan(v, red[i]) : v + red[i];
   }
   return v;
 }
@@ -125,13 +131,13 @@ __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void rms_norm_k(RnP p) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       f[k][j] = (f[k][j] * r) * w[j];
-      if (MODE == 1) top = fmaxf(top, fabsf(f[k][j]));
+      if (MODE == 1) top = max_or_nan(top, fabsf(f[k][j]));
     }
     if (MODE == 0) elem_store_vec<T>(p.y, at + c, n, f[k]);
   }
   if constexpr (MODE == 1) {
     top = team_reduce<TEAM, true>(top, red);
-    const float scale = top > 0.f ? top / E4M3_MAX : 1.f;
+    const float scale = top == 0.f ? 1.f : top / E4M3_MAX;
     if (lane == 0) p.scale[row] = scale;
 #pragma unroll
     for (int k = 0; k < KI; ++k) {

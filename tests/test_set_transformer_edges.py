@@ -308,3 +308,39 @@ def test_one_infinite_score(launches, t):
 @pytest.mark.parametrize("size", INFINITE, ids=str)
 def test_one_infinite_score_on_the_gpu(t, size):
     check_one_infinite_key("cuda", t, *size)
+
+
+# ---------------------------------------------------------------------------------------------------------------- 8-bit rows
+def check_special_quant_rows(device, t, cols):
+    """scale = max |y| / 448 also where that is not finite: NaN for a row with a NaN (or an infinity in x: its r is 0), inf for an infinite weight."""
+    x = torch.ones(4, cols, dtype=t)
+    x[0, cols // 2], x[1, 0], x[2, cols - 1] = float("nan"), float("inf"), -float("inf")
+    w = torch.ones(cols)
+    q, scale = ops.rms_norm_quant(x.to(device), w.to(device))
+    q, scale = q.float().cpu(), scale.cpu()
+    assert bool(scale[:3].isnan().all()) and bool(q[:3].isnan().all())
+    assert bool(scale[3].isfinite()) and bool((q[3] == 448).all())
+    w[3] = -float("inf")
+    q, scale = ops.rms_norm_quant(x[3:].to(device), w.to(device))
+    q = q[0].float().cpu()
+    assert float(scale[0]) == float("inf") and bool(q[3].isnan()) and not q[:3].any() and not q[4:].any()
+    w[3] = float("nan")
+    q, scale = ops.rms_norm_quant(x[3:].to(device), w.to(device))
+    assert bool(scale.isnan().all()) and bool(q.float().isnan().all())
+
+
+SPECIAL_COLS = [5, 64, 500, 3000, 9000]  # each width of a row's team
+
+
+@emulator
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+def test_quant_rows_that_are_not_finite(launches, t):
+    for cols in SPECIAL_COLS[:4]:
+        check_special_quant_rows("cpu", t, cols)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("cols", SPECIAL_COLS)
+def test_quant_rows_that_are_not_finite_on_the_gpu(t, cols):
+    check_special_quant_rows("cuda", t, cols)
