@@ -1,7 +1,7 @@
 // Root-mean-square norm of rows, with the residual's addition in front and an 8-bit output with a scale per row behind.
 //
 //     s = x + residual (rounded to the element type: it is an output)      r = 1 / sqrt(mean(s^2) + eps)      y = s r w
-//     8 bits: scale = max |y| / 448 (1 for a row of zeros; NaN, infinite as the maximum is), q = e4m3(y / scale)
+//     8 bits: scale = max |y| / 448 (1 where that is 0; NaN, infinite as the maximum is), q = e4m3(y / scale)
 //     backward, g = dy w:  ds = dsum + r (g - s r^2 mean(g s)),   dw = sum over rows of dy s r
 //
 // All of it is bound by bytes: a row is read once, held in registers as fp32 and written once.  A row belongs to a team of lanes as wide
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void rms_norm_k(RnP p) {
   }
   if constexpr (MODE == 1) {
     top = team_reduce<TEAM, true>(top, red);
-    const float scale = top == 0.f ? 1.f : top / E4M3_MAX;
+    const float share = top / E4M3_MAX, scale = share == 0.f ? 1.f : share;  // (0 also where max |y| is below 448 2^-150)
     if (lane == 0) p.scale[row] = scale;
 #pragma unroll
     for (int k = 0; k < KI; ++k) {

@@ -1370,7 +1370,7 @@ def rms_norm(x, weight, eps=1e-6, residual=None):
 
 def rms_norm_quant(x, weight, eps=1e-6, residual=None):
     """``rms_norm`` with an 8-bit output and a scale per row: -> (q float8_e4m3fn, scale fp32 [...]) with y ~ q scale, scale = max |y| / 448
-    (1 for a row of zeros; a row with a NaN has the scale NaN and NaN throughout), and s behind them if there is a residual.  For serving: no
+    (1 where that is 0 in fp32; a row with a NaN has the scale NaN and NaN throughout), and s behind them if there is a residual.  For serving: no
     gradient."""
     _rms_args("rms_norm_quant", x, weight, residual)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):

@@ -699,7 +699,7 @@ int hitadv_diff_attention_bwd(int dtype, const void *q, const void *k, const voi
 /* Root-mean-square norm of contiguous rows [rows,cols], 1 <= cols <= 16384: s = x + residual rounded to dtype (residual NULL: s = x),
  * r = 1 / sqrt(mean(s^2) + eps), y = s r w.  w [cols] is fp32 or dtype (wtype).
  *   fwd    y [rows,cols]; sum [rows,cols] = s if there is a residual; rstd [rows] = r, or NULL
- *   e4m3   q [rows,cols] = e4m3(y / scale), scale [rows] = max |y| / 448 (1 for a row of zeros)
+ *   e4m3   q [rows,cols] = e4m3(y / scale), scale [rows] = max |y| / 448 (1 where that is 0; NaN if a y is)
  *   bwd    dx = r (g - s r^2 mean(g s)) + dsum, g = dy w (dsum NULL: without it; dx is the gradient of x and of the residual);
  *          dw [cols] in wtype = sum over the rows of dy s r, or NULL; scratch: hitadv_rms_norm_bwd_scratch_floats if dw is wanted */
 int hitadv_rms_norm_fwd(int dtype, int wtype, const void *x, const void *residual, const void *w, int64_t rows, int cols, float eps,

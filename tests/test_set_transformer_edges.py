@@ -344,3 +344,27 @@ def test_quant_rows_that_are_not_finite(launches, t):
 @pytest.mark.parametrize("cols", SPECIAL_COLS)
 def test_quant_rows_that_are_not_finite_on_the_gpu(t, cols):
     check_special_quant_rows("cuda", t, cols)
+
+
+def check_tiny_quant_rows(device, cols):
+    """Rows whose max |y| / 448 is below the smallest fp32 number are zeros with the scale 1 (0 / 0 would make them NaN, and what is not 0 would be 448)."""
+    x = torch.zeros(2, cols)
+    x[0, 1::2] = 1e-44
+    x[1] = 1.
+    w = torch.full((cols,), 1e-3)
+    q, scale = ops.rms_norm_quant(x.to(device), w.to(device))
+    q, scale = q.float().cpu(), scale.cpu()
+    assert float(scale[0]) == 1. and not q[0].any()
+    assert float(scale[1]) < 1e-3 and bool((q[1] == 448).all())
+
+
+@emulator
+def test_quant_rows_below_the_smallest_scale(launches):
+    for cols in SPECIAL_COLS[:4]:
+        check_tiny_quant_rows("cpu", cols)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", SPECIAL_COLS)
+def test_quant_rows_below_the_smallest_scale_on_the_gpu(cols):
+    check_tiny_quant_rows("cuda", cols)
