@@ -100,8 +100,8 @@ __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void rms_norm_k(RnP p) {
   constexpr int V = ELEM_VEC<T>, NT = TEAM > 256 ? TEAM : 256, PER = NT / TEAM;
   __shared__ float red[TEAM > 64 ? TEAM / 64 : 1];
   const int lane = threadIdx.x % TEAM;
-  const int64_t row = (int64_t)blockIdx.x * PER + threadIdx.x / TEAM;
-  if (TEAM <= 64 && row >= p.rows) return;  // (a workgroup-wide team has the row of its block)
+  const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * PER + threadIdx.x / TEAM;
+  if (row >= p.rows) return;  // (a team of several waves is the whole workgroup)
   const int64_t at = row * p.cols;
   float f[KI][V];
   float ss = 0.f;
@@ -268,6 +268,9 @@ __global__ __launch_bounds__(256) void rms_norm_dw_k(const float *__restrict__ p
 }
 
 constexpr int RN_MAX_COLS = 16384;
+// workgroups in a grid's first dimension: 2^31 threads at most.  A dimension takes 2^32 - 1; a launch with more came back without an
+// error and with wrong rows (2^28 + 5 rows of 8 columns).
+constexpr int64_t RN_GRID_X = 1 << 21;
 
 // workgroups of the backward kernel: enough to fill the chip, few enough that the shares of dw stay a small part of the bytes (16384 x 4096
 // bfloat16, with the second kernel: 512 at most 126 us, 1024 97, 2048 114)
@@ -280,12 +283,13 @@ static int rn_bwd_blocks(int64_t rows, int cols) {
 template <int T, int TEAM, int KI> static int rn_launch(const RnP &p, int mode, hipStream_t s) {
   constexpr int PER = (TEAM > 256 ? TEAM : 256) / TEAM, NT = TEAM > 256 ? TEAM : 256;
   const int64_t blocks = (p.rows + PER - 1) / PER;
+  const dim3 grid((unsigned)(blocks < RN_GRID_X ? blocks : RN_GRID_X), (unsigned)((blocks + RN_GRID_X - 1) / RN_GRID_X));
   if (mode == 0) {
-    if (p.residual) rms_norm_k<T, TEAM, KI, 0, true><<<dim3((unsigned)blocks), NT, 0, s>>>(p);
-    else rms_norm_k<T, TEAM, KI, 0, false><<<dim3((unsigned)blocks), NT, 0, s>>>(p);
+    if (p.residual) rms_norm_k<T, TEAM, KI, 0, true><<<grid, NT, 0, s>>>(p);
+    else rms_norm_k<T, TEAM, KI, 0, false><<<grid, NT, 0, s>>>(p);
   } else if (mode == 1) {
-    if (p.residual) rms_norm_k<T, TEAM, KI, 1, true><<<dim3((unsigned)blocks), NT, 0, s>>>(p);
-    else rms_norm_k<T, TEAM, KI, 1, false><<<dim3((unsigned)blocks), NT, 0, s>>>(p);
+    if (p.residual) rms_norm_k<T, TEAM, KI, 1, true><<<grid, NT, 0, s>>>(p);
+    else rms_norm_k<T, TEAM, KI, 1, false><<<grid, NT, 0, s>>>(p);
   } else {
     const unsigned g = (unsigned)rn_bwd_blocks(p.rows, p.cols);
     if (p.dw_part) {

@@ -368,3 +368,27 @@ def test_quant_rows_below_the_smallest_scale(launches):
 @pytest.mark.parametrize("cols", SPECIAL_COLS)
 def test_quant_rows_below_the_smallest_scale_on_the_gpu(cols):
     check_tiny_quant_rows("cuda", cols)
+
+
+# ---------------------------------------------------------------------------------------------------------------- many rows
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols", [(2 ** 28 + 5, 8), (2 ** 26 + 1, 130), (2 ** 24 + 3, 1026)])
+def test_norm_of_more_rows_than_a_grid_dimension_takes(rows, cols):
+    """2^32 threads are a dimension's limit: 2^28 rows with 16 lanes each, 2^26 with 64, 2^24 with 256.  The rows are those of smaller calls."""
+    x = torch.empty(rows, cols, device="cuda", dtype=BF16).normal_(generator=torch.Generator("cuda").manual_seed(1))
+    w = torch.rand(cols, generator=torch.Generator().manual_seed(2)).cuda()
+    cuts = [*range(0, rows, rows // 5), rows]
+    y = ops.rms_norm(x, w)
+    for a, b in zip(cuts, cuts[1:]):
+        assert torch.equal(y[a:b], ops.rms_norm(x[a:b], w))
+    del y
+    q, scale = ops.rms_norm_quant(x, w)
+    for a, b in zip(cuts, cuts[1:]):
+        qs, ss = ops.rms_norm_quant(x[a:b], w)
+        assert torch.equal(q[a:b].view(torch.uint8), qs.view(torch.uint8)) and torch.equal(scale[a:b], ss)
+    del q, scale, qs, ss
+    if cols == 8:
+        dx, = torch.autograd.grad(ops.rms_norm(x.requires_grad_(), w), x, x.detach())
+        for a, b in zip(cuts, cuts[1:]):
+            part = x.detach()[a:b].requires_grad_()
+            assert torch.equal(dx[a:b], torch.autograd.grad(ops.rms_norm(part, w), part, part.detach())[0])
