@@ -1349,8 +1349,8 @@ static bool da_shape_ok(int dtype, int64_t B, int64_t Nq, int64_t Nk, int64_t H,
   if (dtype < 0 || dtype > 2 || B < 1 || Nq < 1 || Nk < 1 || H < 1 || Hkv < 1 || H % Hkv || D < 8 || D > 64 || D % 8) return false;
   const int64_t G = H / Hkv, rows = Nq * G;
   // rows and keys are 32-bit indexes (with room for a tile beyond the end), the division by G is exact below 2^32 / G, and the grid's
-  // second and third extents are 16-bit
-  return rows <= 2000000 && (rows + 256) * G < (1ll << 32) && Nk <= 2000000 && B * Hkv < (1ll << 31) && B * Hkv <= 65535 &&
+  // second and third extents are 16-bit; dlam's kernel has a workgroup of 1024 a head (2^32 threads are too many for a dimension)
+  return rows <= 2000000 && (rows + 256) * G < (1ll << 32) && Nk <= 2000000 && B * Hkv < (1ll << 31) && B * Hkv <= 65535 && H < (1 << 22) &&
          B * H * Nq < (1ll << 40);
 }
 static void da_fill(DaP &p, int B, int Nq, int Nk, int H, int Hkv, int D, int lam_n, int causal, float scale, const int64_t *st) {

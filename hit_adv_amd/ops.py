@@ -1292,7 +1292,7 @@ def diff_attention(q, k, v, lam, scale=None, causal=False, key_lengths=None):
             raise ValueError("diff_attention: key_lengths is [B=%d], got %s" % (B, tuple(key_lengths.shape)))
         key_lengths = key_lengths.clamp(0, Nk).to(torch.int32) if key_lengths.dtype == torch.int64 else key_lengths.contiguous()
     if B and Nq and Nk and not _lib.load().hitadv_diff_attention_supported(_DTYPE_CODE[q.dtype], B, Nq, Nk, H, Hkv, D):
-        raise ValueError("diff_attention: D=%d must be a multiple of 8 up to 64, Nq * H / Hkv and Nk at most 2,000,000 and B * Hkv at most 65535 "
+        raise ValueError("diff_attention: D=%d must be a multiple of 8 up to 64, Nq * H / Hkv and Nk at most 2,000,000, B * Hkv at most 65535 and H below 2^22 "
                          "(q %s, k %s)" % (D, tuple(q.shape), tuple(k.shape)))
     scale = float(D) ** -0.5 if scale is None else float(scale)
     keep = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or lam.requires_grad)

@@ -686,7 +686,7 @@ int hitadv_row_sqnorm(const float *X, int64_t rows, int D, float *xx, void *stre
  * backward: dout [B,Nq,H,2D] contiguous; r [2,B,H,Nq] fp32 scratch; dq, dk, dv contiguous in the shapes of q, k, v (dk, dv summed over a
  *   group's heads; 0 behind the lengths; both or neither may be NULL); dlam [lam_n] fp32, or NULL if not wanted.  Every sum in a fixed order: no atomics.
  * D a multiple of 8 up to 64, H a multiple of Hkv; hitadv_diff_attention_supported says whether the sizes are taken (rows Nq G and Nk up
- * to 2,000,000, B Hkv up to 65535). */
+ * to 2,000,000, B Hkv up to 65535, H below 2^22). */
 int hitadv_diff_attention_supported(int dtype, int64_t B, int64_t Nq, int64_t Nk, int64_t H, int64_t Hkv, int64_t D);
 int64_t hitadv_diff_attention_scratch_floats(int B, int Nq, int Nk, int H, int Hkv, int D);
 int hitadv_diff_attention_fwd(int dtype, const void *q, const void *k, const void *v, const float *lam, int lam_n, const int32_t *lengths,

@@ -392,3 +392,11 @@ def test_norm_of_more_rows_than_a_grid_dimension_takes(rows, cols):
         for a, b in zip(cuts, cuts[1:]):
             part = x.detach()[a:b].requires_grad_()
             assert torch.equal(dx[a:b], torch.autograd.grad(ops.rms_norm(part, w), part, part.detach())[0])
+
+
+def test_attention_refuses_more_heads_than_the_weights_gradient_has_workgroups_for():
+    """dlam's kernel has 1024 threads a head, and a grid dimension ends below 2^32."""
+    supported = _lib.load().hitadv_diff_attention_supported
+    assert supported(1, 1, 1, 1, 2 ** 22 - 2 ** 7, 2 ** 15 - 1, 8) == 1
+    for heads in (2 ** 22, 2 ** 22 + 2 ** 15, 2 ** 24):
+        assert supported(1, 1, 1, 1, heads, 2 ** 15, 8) == 0
