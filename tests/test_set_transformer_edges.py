@@ -10,8 +10,10 @@ import torch
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, os.path.join(ROOT, "tests", "native"))
+sys.path.insert(0, os.path.join(ROOT, "tests"))
 import emu_build  # noqa: E402
 from hit_adv_amd import _lib, ops  # noqa: E402
+from test_set_transformer_ops import attention_bounds, attention_reference, check, make  # noqa: E402
 
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 emulator = pytest.mark.skipif(not os.path.exists(emu_build.CLANGXX), reason="no host clang++")
@@ -392,6 +394,9 @@ def test_norm_of_more_rows_than_a_grid_dimension_takes(rows, cols):
         for a, b in zip(cuts, cuts[1:]):
             part = x.detach()[a:b].requires_grad_()
             assert torch.equal(dx[a:b], torch.autograd.grad(ops.rms_norm(part, w), part, part.detach())[0])
+        del dx, part
+    del x
+    torch.cuda.empty_cache()  # (up to 90 GB)
 
 
 def test_attention_refuses_more_heads_than_the_weights_gradient_has_workgroups_for():
@@ -400,3 +405,72 @@ def test_attention_refuses_more_heads_than_the_weights_gradient_has_workgroups_f
     assert supported(1, 1, 1, 1, 2 ** 22 - 2 ** 7, 2 ** 15 - 1, 8) == 1
     for heads in (2 ** 22, 2 ** 22 + 2 ** 15, 2 ** 24):
         assert supported(1, 1, 1, 1, heads, 2 ** 15, 8) == 0
+
+
+# ---------------------------------------------------------------------------------------------------------------- scales
+def underflow(r, Hkv):
+    """What numbers below u = 2^-126, which the exponential and the matrix instruction drop, take from the sums in front of their factor ``scale``:
+    a probability (u times what it is multiplied with), the three pieces of A or dS (3 u times the other operand) and the up to six
+    products of a term with their sums (6 u)."""
+    u = 2.0 ** -126
+    B, Nq, H, _, D = r.q.shape
+    e = lambda s, *t: torch.einsum(s, *(x.abs() for x in t))  # noqa: E731
+    w = (r.dP[:, :, None] - r.r[..., None]).abs() * r.sign.abs() + 3
+    a = (4 + r.l.abs()).expand(B, H, Nq, r.Nk)
+    heads = lambda t: t.view(B, r.Nk, Hkv, H // Hkv, *t.shape[3:]).sum(3)  # noqa: E731
+    return {"out": u * (e("bhij,bjhd->bihd", a, r.vv) + 6 * r.Nk), "dv": u * heads(e("bhij,bihd->bjhd", a, r.g) + 6 * Nq),
+            "dq": abs(r.scale) * u * (e("bhmij,bjhmd->bihmd", w, r.kk) + 6 * r.Nk),
+            "dk": abs(r.scale) * u * heads(e("bhmij,bihmd->bjhmd", w, r.q) + 6 * Nq), "dlam": u * (r.dP.abs() + 6).sum((0, 2, 3))}
+
+
+def check_scaled_gradients(device, t, scale, causal, size=(1, 40, 70, 2, 1, 16)):
+    """Output and gradients at scores of 1e4, of 0 and with a negative scale.  The bounds hold a probability's error for the scores' size: at 1e4 the
+    fp32 numbers that stand for a score, a row's maximum and its logarithm have steps of 2^-10.  What underflows is added: a probability of 2^-120
+    in front of a scale of 300 makes a gradient that is not small beside fp32's smallest numbers."""
+    q, k, v, lam, g = make(t, *size, seed=21, device=device)
+    r = attention_reference(q, k, v, lam, causal, scale=scale, dout=g)
+    b, u = attention_bounds(t, r, True), underflow(r, size[4])
+    b = {name: b[name] + u[name] for name in b}
+    leaves = [x.requires_grad_() for x in (q, k, v, lam)]
+    out = ops.diff_attention(*leaves, scale=scale, causal=causal)
+    check(out, r.out, b["out"], "out")
+    grads = torch.autograd.grad(out, leaves, g)
+    for name, got in zip(("dq", "dk", "dv", "dlam"), grads):
+        check(got, getattr(r, name), b[name], name)
+    if scale == 0.:
+        assert not grads[0].any() and not grads[1].any()
+    return out, grads
+
+
+SCALES = [0., 300., -2., -300., 2. ** -20]
+
+
+@emulator
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+def test_gradients_at_extreme_scales(launches, t):
+    for scale in (0., 300., -2.):
+        check_scaled_gradients("cpu", t, scale, True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("scale", SCALES)
+@pytest.mark.parametrize("size", [(1, 40, 70, 2, 1, 16), (2, 33, 700, 4, 2, 64)], ids=str)
+def test_gradients_at_extreme_scales_on_the_gpu(t, scale, size):
+    for causal in (False, True):
+        check_scaled_gradients("cuda", t, scale, causal, size)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+def test_a_negative_scale_is_a_negative_query(t):
+    """The sign is taken into the operand: the same bits as the query's own sign, dq turned.  (dK = scale dS^T Q sums products of the other sign, and the
+    matrix instruction truncates downwards: its last bits differ, and the test above holds it to its bound.)"""
+    q, k, v, lam, g = make(t, 2, 50, 90, 4, 2, 32, seed=22)
+
+    def run(q, scale):
+        leaves = [x.detach().clone().requires_grad_() for x in (q, k, v, lam)]
+        out = ops.diff_attention(*leaves, scale=scale, causal=True)
+        return (out, *torch.autograd.grad(out, leaves, g))
+    (o, dq, _, dv, dl), (o2, dq2, _, dv2, dl2) = run(q, -0.25), run(-q, 0.25)
+    assert torch.equal(o, o2) and torch.equal(dq, -dq2) and torch.equal(dv, dv2) and torch.equal(dl, dl2)
