@@ -390,10 +390,16 @@ template <int NP, int DP, int NT> struct DaFetchBlocks {
       for (int i = 0; i < 4; ++i) x[c][i] = da_load4<NP>(at + (o[i] * ES + oc));
     }
   }
-  template <bool ROWS, bool COLS> __device__ __forceinline__ void put(uint16_t *rows, uint16_t *cols) {
+  // `none` > 0: so many rows of the tile see no key, and what they hold is dropped
+  template <bool ROWS, bool COLS> __device__ __forceinline__ void put(uint16_t *rows, uint16_t *cols, int none = 0) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       if (!there[c]) continue;
+      if (none > 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (row + i < none) x[c][i] = da_zero<Raw4<NP>>();
+      }
       if (left < DA_T) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -797,7 +803,7 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_DQ_WAVES<NP,
     for (int c = 0; c < VC; ++c) {
       const int d = 16 * c + 8 * half;
       uint4 w[NR];
-      da_pieces8<NP>(da_load8_if<NP>(p.dout, (((int64_t)b * p.Nq + i) * p.H + h) * 2 * p.D + d, valid && d < 2 * p.D), w);
+      da_pieces8<NP>(da_load8_if<NP>(p.dout, (((int64_t)b * p.Nq + i) * p.H + h) * 2 * p.D + d, valid && lim > 0 && d < 2 * p.D), w);
       da_turn(w, neg);
 #pragma unroll
       for (int k = 0; k < NR; ++k) gf[c][k] = as_bf16x8(w[k]);
@@ -1039,6 +1045,8 @@ __global__ __launch_bounds__(64 * NW) HITADV_WAVES_PER_SIMD((DA_DKV_WAVES<NP, DP
   // causal: query i sees key j when i >= j - (Nk - Nq): rows before that of the workgroup's first key have nothing here
   int begin = p.causal ? max(0, first - (p.Nk - p.Nq)) : 0;
   begin = first >= len ? p.rows : (int)min((int64_t)p.rows, (int64_t)begin * p.G) / DA_T * DA_T;
+  // rows that see no key at all share a tile with the first that do: 0 times what they hold need not be 0
+  const int none = p.causal ? max(0, p.Nq - p.Nk) * p.G : 0;
   DaFetchBlocks<NP, DP, 64 * NW> fq, fg;
   const int64_t g_n = (int64_t)p.H * 2 * p.D;
   const int64_t q_at = b * p.q_b + hk * p.G * p.q_h, g_at = ((int64_t)b * p.Nq * p.H + hk * p.G) * 2 * p.D;
@@ -1080,8 +1088,8 @@ __global__ __launch_bounds__(64 * NW) HITADV_WAVES_PER_SIMD((DA_DKV_WAVES<NP, DP
 #pragma unroll 1
   for (int t = begin; t < p.rows; t += DA_T) {
     __syncthreads();
-    fq.template put<true, DK>(Qs, Qt);
-    fg.template put<DK, DV>(Gs, Gt);
+    fq.template put<true, DK>(Qs, Qt, none - t);
+    fg.template put<DK, DV>(Gs, Gt, none - t);
     put_row(t);
     __syncthreads();
     load_row(t + DA_T);  // (behind the last tile: its last row once more, not used)

@@ -1267,7 +1267,7 @@ def diff_attention(q, k, v, lam, scale=None, causal=False, key_lengths=None):
     head h // (H // Hkv)), D a multiple of 8 up to 64; lam fp32, [H] or one value for all heads -> [B,Nq,H,2D] of that type.  ``scale``
     defaults to D ** -0.5.  ``causal``: query i sees the keys j <= i + Nk - Nq, so that a few new queries stand at the end of a cache.
     ``key_lengths`` [B] int: only the keys below it (clamped to 0 .. Nk) exist; what lies behind it may hold anything.  A row that sees no key
-    is 0 and has no gradient.  Values that are visible to some row should be finite: a row that sees one that is not is not finite itself (NaN too
+    is 0 and has no gradient, whatever it and its incoming gradient hold.  Values that are visible to some row should be finite: a row that sees one that is not is not finite itself (NaN too
     where all its scores are -inf; but one key with a score of -inf has probability 0 in 16-bit types, as in the formula), and so may be rows, and
     gradients of keys, of the same tile from which only ``causal`` hides it.  Views whose last axis is contiguous and whose rows start at multiples of 16
     bytes (a slice of a cache) are read where they are, others are copied.  Same bits on every run; no second derivative."""

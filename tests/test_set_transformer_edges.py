@@ -474,3 +474,41 @@ def test_a_negative_scale_is_a_negative_query(t):
         return (out, *torch.autograd.grad(out, leaves, g))
     (o, dq, _, dv, dl), (o2, dq2, _, dv2, dl2) = run(q, -0.25), run(-q, 0.25)
     assert torch.equal(o, o2) and torch.equal(dq, -dq2) and torch.equal(dv, dv2) and torch.equal(dl, dl2)
+
+
+# ---------------------------------------------------------------------------------------------------------------- rows that see nothing
+def check_empty_rows_give_nothing(device, t, B, Nq, Nk, H, Hkv, D, lengths=None):
+    """Queries in front of the first key (causal, more queries than keys) and all queries of an empty sequence: whatever they and their incoming
+    gradients hold -- NaN, infinities -- stays out of every other row's output and of all gradients."""
+    q, k, v, lam, g = make(t, B, Nq, Nk, H, Hkv, D, seed=31, device=device)
+    kl = torch.tensor(lengths, dtype=torch.int32, device=device) if lengths else None
+    seen = torch.full((B, Nq), Nk) if kl is None else kl.cpu().long()[:, None].expand(B, Nq)
+    empty = (torch.minimum(seen, torch.arange(Nq) + Nk - Nq + 1) <= 0).to(device)
+    assert bool(empty.any()) and not bool(empty.all())
+
+    def run(fill_q, fill_g):
+        leaves = [x.clone().requires_grad_() for x in (q.masked_fill(empty[:, :, None, None, None], fill_q), k, v, lam)]
+        out = ops.diff_attention(*leaves, causal=True, key_lengths=kl)
+        return (out, *torch.autograd.grad(out, leaves, g.masked_fill(empty[:, :, None, None], fill_g)))
+    want = run(0., 0.)
+    assert not want[0][empty].any() and not want[1][empty].any()
+    for fill_q, fill_g in ((0., float("nan")), (float("nan"), 0.), (float("inf"), -float("inf"))):
+        for a, b, name in zip(run(fill_q, fill_g), want, ("out", "dq", "dk", "dv", "dlam")):
+            assert torch.equal(a, b), (name, fill_q, fill_g)
+
+
+EMPTY = [(1, 50, 20, 2, 2, 16), (2, 77, 45, 3, 1, 40), (1, 200, 70, 2, 1, 64), (2, 40, 33, 4, 2, 32, (33, 0))]
+
+
+@emulator
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+def test_rows_that_see_nothing_give_nothing(launches, t):
+    for case in (EMPTY[0], EMPTY[1]):
+        check_empty_rows_give_nothing("cpu", t, *case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("case", EMPTY, ids=str)
+def test_rows_that_see_nothing_give_nothing_on_the_gpu(t, case):
+    check_empty_rows_give_nothing("cuda", t, *case)
