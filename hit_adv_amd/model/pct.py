@@ -190,7 +190,7 @@ class DA_Layer(nn.Module):
             return x + F.dropout(y, self.p)
         rng = self.rng.clone()  # the backward pass needs this call's offset
         self.rng[1] += 1
-        return ops.dropout(y, self.p, rng, residual=x)
+        return ops.dropout(y.to(x.dtype), self.p, rng, residual=x)  # (under autocast y is 16-bit, and x + y above is of x's type)
 
     def forward(self, x):
         return self.forward_pm(x.permute(0, 2, 1)).permute(0, 2, 1)

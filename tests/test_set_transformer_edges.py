@@ -512,3 +512,63 @@ def test_rows_that_see_nothing_give_nothing(launches, t):
 @pytest.mark.parametrize("case", EMPTY, ids=str)
 def test_rows_that_see_nothing_give_nothing_on_the_gpu(t, case):
     check_empty_rows_give_nothing("cuda", t, *case)
+
+
+# ---------------------------------------------------------------------------------------------------------------- the layer
+@pytest.mark.gpu
+@pytest.mark.parametrize("p", [0., 0.5])
+def test_da_layer_under_autocast(p):
+    """In training as in evaluation the projections' 16-bit output joins the residual in the residual's type."""
+    from hit_adv_amd.model.pct import DA_Layer
+    torch.manual_seed(0)
+    m = DA_Layer(128, dropout=p).cuda()
+    x = torch.randn(2, 128, 40, device="cuda")
+    outs = {}
+    for mode in (False, True):
+        m.train(mode)
+        with torch.autocast("cuda", dtype=BF16):
+            y = m(x.requires_grad_())
+        assert y.dtype == F32 and y.shape == x.shape
+        g, = torch.autograd.grad(y, x, torch.ones_like(y))
+        assert bool(g.isfinite().all())
+        outs[mode] = y.detach()
+    if p == 0.:
+        assert torch.equal(outs[False], outs[True])
+    else:  # an element is dropped, or twice what evaluation adds
+        d, e = outs[True] - x.detach(), outs[False] - x.detach()
+        # either sum is rounded once: 2^-24 of values below 2^3, twice where doubled
+        assert bool(((d == 0) | ((d - 2 * e).abs() <= 3 * 2.0 ** -21)).all()) and 0.4 < float((d == 0).float().mean()) < 0.6
+
+
+@pytest.mark.gpu
+def test_da_layer_captured_draws_new_masks():
+    """A captured training step: every replay takes the next offset, and gives the eager layer's bits at that offset."""
+    from hit_adv_amd.model.pct import DA_Layer
+    torch.manual_seed(0)
+    m = DA_Layer(64, dropout=0.5).cuda().train()
+    x, g = torch.randn(2, 64, 40, device="cuda"), torch.randn(2, 64, 40, device="cuda")
+    leaf = x.clone().requires_grad_()
+
+    def step():
+        y = m(leaf)
+        return y.detach(), *torch.autograd.grad(y, [leaf, m.out.weight], g)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    last = None
+    for _ in range(4):
+        offset = int(m.rng[1])
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in held]
+        assert int(m.rng[1]) == offset + 1 and (last is None or not torch.equal(got[0], last))
+        last = got[0]
+        m.rng[1] = offset
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b)
