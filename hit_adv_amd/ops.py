@@ -1212,6 +1212,13 @@ def _strided(t):
 
 class DiffAttention(torch.autograd.Function):
     @staticmethod
+    def strides(q, k, v):
+        q, qs = _strided(q)
+        k, ks = _strided(k)
+        v, vs = _strided(v)
+        return q, k, v, (ctypes.c_int64 * 11)(*qs, *ks, *vs)
+
+    @staticmethod
     def forward(ctx, q, k, v, lam, scale, causal, lengths, keep):
         B, Nq, H, _, D = q.shape
         Nk, Hkv = k.shape[1], k.shape[2]
@@ -1221,10 +1228,8 @@ class DiffAttention(torch.autograd.Function):
         if ctx.empty:
             out.zero_()
         else:
-            q, qs = _strided(q)
-            k, ks = _strided(k)
-            v, vs = _strided(v)
-            ctx.strides = (ctypes.c_int64 * 11)(*qs, *ks, *vs)
+            q, k, v, ctx.strides = DiffAttention.strides(q, k, v)
+            ctx.layout = q.stride(), k.stride(), v.stride()
             if keep:
                 stats = torch.empty(4, B, H, Nq, device=q.device, dtype=torch.float32)
             n = _lib.load().hitadv_diff_attention_scratch_floats(B, Nq, Nk, H, Hkv, D)
@@ -1246,7 +1251,10 @@ class DiffAttention(torch.autograd.Function):
         need = ctx.needs_input_grad
         if ctx.empty:
             return tuple(torch.zeros_like(t) if need[i] else None for i, t in enumerate((q, k, v, lam))) + (None,) * 4
-        g, lam = _aligned(g), lam.contiguous()
+        if ctx.layout != (q.stride(), k.stride(), v.stride()) or (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
+            q, k, v, ctx.strides = DiffAttention.strides(q, k, v)  # saved-tensor hooks give back the values, in a layout of their own
+            ctx.layout = q.stride(), k.stride(), v.stride()
+        g, lam, lengths, stats = _aligned(g), lam.contiguous(), _contiguous(lengths), stats.contiguous()
         r = torch.empty(2, B, H, Nq, device=q.device, dtype=torch.float32)
         dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
         dk = dv = dlam = None
@@ -1322,7 +1330,7 @@ class RmsNorm(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dsum=None):
-        s, weight, rstd = ctx.saved_tensors
+        s, weight, rstd = (t.contiguous() for t in ctx.saved_tensors)  # (saved-tensor hooks may give back another layout)
         need = ctx.needs_input_grad
         if dy is None:
             return dsum if need[0] else None, None, None, dsum if need[3] else None, None
@@ -1405,7 +1413,7 @@ class Dropout(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        rng, = ctx.saved_tensors
+        rng = ctx.saved_tensors[0].contiguous()
         need = ctx.needs_input_grad
         return _dropout_raw(g.contiguous(), None, ctx.p, rng) if need[0] else None, None, None, g if need[3] else None
 

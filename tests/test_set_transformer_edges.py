@@ -57,9 +57,12 @@ class Launches:
     def launch(self, t, name, *args):
         gone = [(dtype, shape) for r, dtype, shape in self.taken if r() is None]
         types = {dtype for _, dtype, _ in self.taken}
-        self.taken = []
+        held, self.taken = [r() for r, _, _ in self.taken], []
         self.names.append(name)
         assert not gone, "%s: tensors given up before the launch: %s" % (name, gone)
+        if "attention" in name:  # q, k, v: the strides that go with the addresses
+            want = [(n, st) for x in held[:3] for n, st in zip(x.shape[:-1], x.stride())]
+            assert all(got == st or n == 1 for got, (n, st) in zip(args[7], want)), "%s: strides %s of tensors with %s" % (name, list(args[7]), want)
         self.types(t, name, types)
         if self.run:
             assert self.emulated(name)(*args, None) == 0
@@ -156,6 +159,46 @@ def test_norm_gradients_of_any_layout_on_the_gpu(layout, rows, cols):
 def test_norm_gradients_of_sums_on_the_gpu():
     for a, b in zip(norm_sums("cuda", False), norm_sums("cuda", True)):
         assert torch.equal(a, b)
+
+
+def fused_gradients(device, hooks):
+    """Gradients of attention over slices of one projection and a norm, what is saved for them going through ``hooks``."""
+    g = torch.Generator().manual_seed(11)
+    n = lambda *s: torch.randn(*s, generator=g).to(device)  # noqa: E731
+    h, lam, w = n(2, 40, 3, 128).requires_grad_(), torch.tensor([0.25, 0.5], device=device, requires_grad=True), n(64).requires_grad_()
+    lengths = torch.tensor([40, 21], dtype=torch.int32, device=device)
+    with hooks:
+        q, k, v = h.unbind(2)
+        out = ops.diff_attention(q.view(2, 40, 2, 2, 32), k.view(2, 40, 2, 2, 32), v.view(2, 40, 2, 64), lam, key_lengths=lengths)
+        y, s = ops.rms_norm(out, w, residual=out.detach())
+        z = ops.dropout(y, 0.5, torch.tensor([1, 2], device=device))
+    return torch.autograd.grad((z, s), (h, lam, w), (n(2, 40, 2, 64), n(2, 40, 2, 64)))
+
+
+def turned(t):
+    return t.t().contiguous().t() if t.dim() == 2 else t.transpose(0, -1).contiguous().transpose(0, -1) if t.dim() > 2 else t
+
+
+HOOKS = {"contiguous": (lambda t: t.clone(memory_format=torch.contiguous_format), lambda t: t),
+         "turned": (turned, lambda t: t),
+         "misaligned": (lambda t: t.detach(), lambda t: torch.cat([t.reshape(-1)[:1], t.reshape(-1)])[1:].view(t.shape))}
+
+
+@emulator
+@pytest.mark.parametrize("hooks", sorted(HOOKS))
+def test_saved_tensors_may_come_back_in_another_layout(launches, hooks):
+    """Saved-tensor hooks (activations moved to the host and back) return the values, not the strides."""
+    want = fused_gradients("cpu", torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t))
+    for a, b in zip(fused_gradients("cpu", torch.autograd.graph.saved_tensors_hooks(*HOOKS[hooks])), want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_saved_tensors_may_come_back_in_another_layout_on_the_gpu():
+    want = fused_gradients("cuda", torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t))
+    for hooks in [torch.autograd.graph.saved_tensors_hooks(*HOOKS[n]) for n in sorted(HOOKS)] + [torch.autograd.graph.save_on_cpu()]:
+        for a, b in zip(fused_gradients("cuda", hooks), want):
+            assert torch.equal(a, b)
 
 
 # ---------------------------------------------------------------------------------------------------------------- torch's default type
