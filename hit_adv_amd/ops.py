@@ -1174,10 +1174,6 @@ def _at(t):
     return 0 if t is None else t.data_ptr()
 
 
-def _contiguous(t):
-    return None if t is None else t.contiguous()
-
-
 def _typed(t, name, like=None, dtypes=_DTYPE_CODE):
     """A GPU tensor of one of ``dtypes`` on the device of ``like``, as it is (no cast: the type says how outputs are rounded)."""
     if not torch.is_tensor(t):
@@ -1229,8 +1225,8 @@ class DiffAttention(torch.autograd.Function):
             out.zero_()
         else:
             q, k, v, ctx.strides = DiffAttention.strides(q, k, v)
-            ctx.layout = q.stride(), k.stride(), v.stride()
             if keep:
+                ctx.layout = q.stride(), k.stride(), v.stride()
                 stats = torch.empty(4, B, H, Nq, device=q.device, dtype=torch.float32)
             n = _lib.load().hitadv_diff_attention_scratch_floats(B, Nq, Nk, H, Hkv, D)
             scratch = torch.empty(n, device=q.device, dtype=torch.float32) if n else None
@@ -1254,7 +1250,9 @@ class DiffAttention(torch.autograd.Function):
         if ctx.layout != (q.stride(), k.stride(), v.stride()) or (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
             q, k, v, ctx.strides = DiffAttention.strides(q, k, v)  # saved-tensor hooks give back the values, in a layout of their own
             ctx.layout = q.stride(), k.stride(), v.stride()
-        g, lam, lengths, stats = _aligned(g), lam.contiguous(), _contiguous(lengths), stats.contiguous()
+        g, lam, stats = _aligned(g), lam.contiguous(), stats.contiguous()
+        if lengths is not None:
+            lengths = lengths.contiguous()
         r = torch.empty(2, B, H, Nq, device=q.device, dtype=torch.float32)
         dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
         dk = dv = dlam = None
@@ -1313,11 +1311,12 @@ RMS_NORM_MAX_COLS = 16384
 class RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, eps, residual, keep):
-        x, weight, residual = x.contiguous(), weight.contiguous(), _contiguous(residual)
+        x, weight, total = x.contiguous(), weight.contiguous(), None
+        if residual is not None:
+            residual, total = residual.contiguous(), torch.empty_like(x)
         C = x.shape[-1]
         rows = x.numel() // C
         y = torch.empty_like(x)
-        total = torch.empty_like(x) if residual is not None else None
         rstd = torch.empty(rows, device=x.device, dtype=torch.float32) if keep else None
         if rows:
             _call_on(x, "hitadv_rms_norm_fwd", _DTYPE_CODE[x.dtype], _DTYPE_CODE[weight.dtype], _at(x),
@@ -1330,11 +1329,13 @@ class RmsNorm(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dsum=None):
-        s, weight, rstd = (t.contiguous() for t in ctx.saved_tensors)  # (saved-tensor hooks may give back another layout)
+        s, weight, rstd = ctx.saved_tensors
         need = ctx.needs_input_grad
         if dy is None:
             return dsum if need[0] else None, None, None, dsum if need[3] else None, None
-        dy, dsum = dy.contiguous(), _contiguous(dsum)
+        s, weight, rstd, dy = s.contiguous(), weight.contiguous(), rstd.contiguous(), dy.contiguous()  # (saved-tensor hooks have layouts of their own)
+        if dsum is not None:
+            dsum = dsum.contiguous()
         C = s.shape[-1]
         rows = s.numel() // C
         dx = torch.empty_like(s)
@@ -1383,12 +1384,13 @@ def rms_norm_quant(x, weight, eps=1e-6, residual=None):
     _rms_args("rms_norm_quant", x, weight, residual)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
         raise RuntimeError("rms_norm_quant has no backward pass: call it under torch.no_grad(), or rms_norm")
-    x, weight, residual = x.contiguous(), weight.contiguous(), _contiguous(residual)
+    x, weight, total = x.contiguous(), weight.contiguous(), None
+    if residual is not None:
+        residual, total = residual.contiguous(), torch.empty_like(x)
     C = x.shape[-1]
     rows = x.numel() // C
     q = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
     scale = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
-    total = torch.empty_like(x) if residual is not None else None
     if rows:
         _call_on(x, "hitadv_rms_norm_e4m3", _DTYPE_CODE[x.dtype], _DTYPE_CODE[weight.dtype], _at(x),
                  _at(residual), _at(weight), rows, C, float(eps), _at(q), _at(scale), _at(total))
