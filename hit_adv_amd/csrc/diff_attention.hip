@@ -440,11 +440,13 @@ __device__ __forceinline__ int da_wave_id() { return __builtin_amdgcn_readfirstl
 // its waves the first map, the other the second: half the accumulators each (two or three waves per SIMD, where one wave with both
 // maps fills the registers), and the difference is taken once, at the end, through LDS.  The next tile's elements are on their way in
 // registers while this one's are multiplied; two buffers, one barrier a tile.  LDS operands are read a phase ahead of their products.
-// Bound by instruction issue: on this chip a SIMD's matrix and vector instructions do not overlap, and a pair of keys costs a map's share of
-// 3 matrix instructions a 16-column block plus two exponentials, two splits and a maximum.  Measured: 2 clouds x 8 heads x 4096 x 4096, D 64,
-// bfloat16: 370 us (137 GFLOP of the formula: 371 TFLOP/s; 556 with the second piece's products), causal 203; 8 clouds x 8 heads (2 shared) x
-// 1000, D 48, fp16: 95 us with three fifths of the keys; 32 x 4 x 256 x 256, D 32, fp32: 24 us (six products for one); 16 tokens x 16 heads
-// over 8192 keys of 4 heads, in 16 parts: 43 us = 6.2 TB/s of cache, and 4.4 us for the join.
+// Bound by the matrix instructions, most of which are V times either map in two pieces: a pair of keys costs 4 D flop for the scores and
+// 2 maps x 2 pieces x 4 D for the values = 20 D (fp32: six products for one, 72 D) where the formula has 8 D, the difference taken first.  Taking
+// it first needs both maps in one wave, whose accumulators then fill the registers.  Two exponentials, splits and a maximum come on top: a
+// SIMD's matrix and vector instructions do not overlap here.  Measured: 2 clouds x 8 heads x 4096 x 4096, D 64, bfloat16: 351 - 371 us (137 GFLOP
+// of the formula: 370 - 391 TFLOP/s; 926 - 979 executed, where a large library product reaches 1094), causal 196 - 205; 8 clouds x 8 heads (2
+// shared) x 1000, D 48, fp16: 96 us with three fifths of the keys; 32 x 4 x 256 x 256, D 32, fp32: 23 - 25 us; 16 tokens x 16 heads over 8192 keys
+// of 4 heads, in 16 parts: 43 us = 6.2 TB/s of cache, and 4.8 us for the join.
 template <int NP> constexpr float DA_LIFT = NP == 2 ? 7.f : 0.f;
 // the stored statistics: without the lift, so that the logarithm keeps its bits
 template <int NP> __device__ __forceinline__ void da_store_stats(float *at, int64_t n, float mx, float sum, bool empty) {
@@ -690,8 +692,8 @@ __global__ __launch_bounds__(256) void diff_attn_join_k(DaP p) {
 }
 
 // The same for few splits of many rows, where a workgroup a row is mostly its own launch: a thread has four columns of a row and both maps, four
-// splits in flight, and weighs the splits for itself.  16384 rows of 3 splits 11 us against 29 with a workgroup each; 256 rows of 16 splits
-// 11.8 us against 4.9, so up to 8.
+// splits in flight, and weighs the splits for itself.  16384 rows of 3 splits 10.6 us against 27.7 with a workgroup each; 256 rows of 16 splits
+// 12.6 us against 5.4, so up to 8.
 constexpr int DA_FEW_SPLITS = 8;
 template <int NP>
 __global__ __launch_bounds__(256) void diff_attn_join_few_k(DaP p) {
@@ -751,8 +753,8 @@ __global__ __launch_bounds__(256) void diff_attn_join_few_k(DaP p) {
 // A pair of waves shares 32 packed rows and takes the even and the odd tiles of 32 keys; the two meet in LDS (r behind the first pass, dQ at
 // the end): half the longest row's way through the keys, and twice the waves where clouds are few or short.  Bound by instruction issue:
 // 24 D matrix flop a pair of keys where the formula has 12 (the scores and dP twice, dS as two pieces).  2 x 8 x 4096 x 4096, D 64, bfloat16:
-// 565 us, causal 313 (660 TFLOP/s executed); the one-pass form with r from dO . out loses the exact zero of a row with one key.  32 x 4 x
-// 256, D 32, fp32: 46 us.
+// 526 - 567 us, causal 298 - 311 (660 - 690 TFLOP/s executed); 32 x 4 x 256, D 32, fp32: 44 us.  A one-pass form (a third of the products less)
+// needs r before the sweep, as dO . O_m of the unrounded sums O_m of either map: 4 D fp32 values a row written and read once more.
 template <int NP, int DP> constexpr int DA_DQ_WAVES = NP == 3 && DP == 64 ? 1 : 2;  // waves per SIMD
 template <int NP, int DP, int PAIRS>
 __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_DQ_WAVES<NP, DP>)) void diff_attn_dq_k(DaP p) {
@@ -992,8 +994,8 @@ __global__ __launch_bounds__(128 * PAIRS) HITADV_WAVES_PER_SIMD((DA_DQ_WAVES<NP,
 // share a key needs no atomics: dV^T += dO^T A, dK_m^T += Q_m^T dS_m, A = P_1 - lam P_2.  One launch for both, except for fp32 at DP = 64,
 // where three pieces of K and V and both accumulators are more than 512 registers: dV and dK in a launch each (the scores twice, a quarter
 // more products).  Bound by instruction issue and, with one wave a SIMD (the accumulators: 192 registers at DP = 64), by what of a barrier
-// and of LDS latency a wave sees alone.  2 x 8 x 4096 x 4096, D 64, bfloat16: 725 us, causal 399 (517 TFLOP/s executed); 32 x 4 x 256, D 32,
-// fp32: 48 us.
+// and of LDS latency a wave sees alone.  2 x 8 x 4096 x 4096, D 64, bfloat16: 687 - 742 us, causal 390 - 406 (508 - 529 TFLOP/s executed);
+// 32 x 4 x 256, D 32, fp32: 48 us.
 template <int NP, int DP> constexpr int DA_DKV_WAVES = NP != 3 && DP == 32 ? 2 : 1;  // waves per SIMD
 template <int NP, int DP, int NW, bool DV, bool DK>
 __global__ __launch_bounds__(64 * NW) HITADV_WAVES_PER_SIMD((DA_DKV_WAVES<NP, DP>)) void diff_attn_dkv_k(DaP p) {
@@ -1274,12 +1276,13 @@ constexpr int64_t DA_STRIDE = 1 << 24;
 struct DaPlan {
   int pairs, tiles, splits, chunk;
 };
-// Up to 32 rows: one pair of waves (16 tokens x 16 heads over 8192 keys of 4: one pair 57 us, two 64, four 97).  Else four pairs share the keys'
-// tiles (2 x 8 x 4096 causal: one 322 us, two 246, four 213; 32 x 4 x 256 in fp32: 44, 28, 25), but two where few short rows leave the chip
-// empty (16 x 4 x 128: two 12.0 us, four 13.6; 2 x 4 x 100 rows over 1000 keys 15.0, 17.3).
-// Below 2048 waves the keys are split so that the chip fills (the tokens over 8192 keys: one part 308 us, 16 parts 48, 32 parts 57; 4 x 4096 rows
-// causal: one 138, three 74 + 11 for the join), parts of 256 keys at least (5 tokens over 3000 keys: 256 keys a part 15.2 us, 512 24.2), of 512
-// with four pairs, where the join of many rows costs what the parts save (8 x 4 x 512 rows over 512 keys: one part 28 us, two 28 and the join).
+// Up to 32 rows: one pair of waves (16 tokens x 16 heads over 8192 keys of 4: one pair 44 us, two 70, four 117).  Else four pairs share the keys'
+// tiles (2 x 8 x 4096 causal: one 305 us, two 227, four 196; 32 x 4 x 256 in fp32: 42, 25, 23), but two where few short rows leave the chip
+// empty (16 x 4 x 128: two 11.2 us, four 12.5; 2 x 4 x 100 rows over 1000 keys with the join: 18.6, 29.4).
+// Below 2048 waves the keys are split so that the chip fills (the tokens over 8192 keys with the join: one part 297 us, 16 parts 49, 32 parts
+// 62; 4 x 4096 rows causal: one 152, three 68 + 11 for the join), parts of 256 keys at least (5 tokens over 3000 keys: 256 keys a part 18.6 us,
+// 512 28.8), of 512 with four pairs, where the join of many rows costs what the parts save (8 x 4 x 512 rows over 512 keys: one part 26 us, two 25
+// and 8 for the join).
 static DaPlan da_plan(int B, int Nq, int Nk, int H, int Hkv) {
   DaPlan pl;
   const int64_t rows = (int64_t)Nq * (H / Hkv), bh = (int64_t)B * Hkv;

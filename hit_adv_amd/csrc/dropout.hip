@@ -5,7 +5,7 @@
 //
 // Philox4x32-10 is the generator of Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as easy as 1, 2, 3" (SC 2011): ten rounds
 // of two 32 x 32 -> 64 bit products.  Bound by bytes and by those products (quarter rate: 20 per four elements) about alike: 16384 x 4096
-// bfloat16 76 us with a residual = 5.3 TB/s, 50 us without = 5.4 TB/s (a copy of 2 GiB: 4.9 TB/s).
+// bfloat16 74 us with a residual = 5.4 TB/s, 50 us without = 5.4 TB/s (a copy of 2 GiB: 4.9 TB/s).
 #include "elements.hpp"
 #include "hitadv.h"
 

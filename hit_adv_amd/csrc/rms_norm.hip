@@ -9,8 +9,8 @@
 // flight per lane.  The backward kernel's teams walk over many rows and keep their share of dw in registers; the shares of a workgroup
 // meet in LDS, those of the grid in a second small kernel, both in a fixed order (no atomics).  Sums are fp32.
 //
-// Measured, 16384 rows of 4096 bfloat16: forward with residual 92 us = 5.8 TB/s, 8-bit output with residual 98 us = 4.8 TB/s, backward 113 us
-// = 4.8 TB/s and its second kernel 12 us (a copy of 2 GiB: 4.9 TB/s).  8192 rows of 256 fp32: forward 5.8, backward 6.5 + 4.8 us.
+// Measured, 16384 rows of 4096 bfloat16: forward with residual 94 us = 5.7 TB/s, 8-bit output with residual 98 - 107 us = 4.4 - 4.8 TB/s, backward
+// 115 us = 4.7 TB/s and its second kernel 12 us (a copy of 2 GiB: 4.9 TB/s).  8192 rows of 256 fp32: forward 5.1, backward 6.6 + 4.5 us.
 #include "elements.hpp"
 #include "hitadv.h"
 
@@ -273,7 +273,7 @@ constexpr int RN_MAX_COLS = 16384;
 constexpr int64_t RN_GRID_X = 1 << 21;
 
 // workgroups of the backward kernel: enough to fill the chip, few enough that the shares of dw stay a small part of the bytes (16384 x 4096
-// bfloat16, with the second kernel: 512 at most 126 us, 1024 97, 2048 114)
+// bfloat16, with the second kernel: 512 at most 126 us, 1024 96, 2048 112)
 static int rn_bwd_blocks(int64_t rows, int cols) {
   const int per = cols <= 128 ? 16 : cols <= 1024 ? 4 : 1;
   const int64_t b = (rows + per - 1) / per;
@@ -304,8 +304,8 @@ template <int T, int TEAM, int KI> static int rn_launch(const RnP &p, int mode, 
   return 0;
 }
 
-// the narrowest team whose registers hold the row (forward + backward, bfloat16: 262144 x 64 with 16 lanes 51 us, with 64 172; 65536 x 256 with
-// 64 lanes 52 us, with 256 168; 16384 x 1024 with 64 34 us, with 256 47; 16384 x 4096 with 256 141 us, with 1024 221)
+// the narrowest team whose registers hold the row (forward + backward, bfloat16: 262144 x 64 with 16 lanes 55 us, with 64 175; 65536 x 256 with
+// 64 lanes 55 us, with 256 170; 16384 x 1024 with 64 37 us, with 256 50; 16384 x 4096 with 256 150, with 1024 235)
 template <int T> static int rn_dispatch(const RnP &p, int mode, hipStream_t s) {
   constexpr int U = T == ELEM_F32 ? 2 : 1;  // fp32: half as many elements in an access, twice the accesses
   if (p.cols <= 128) return rn_launch<T, 16, U>(p, mode, s);
