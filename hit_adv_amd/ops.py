@@ -1273,10 +1273,11 @@ def diff_attention(q, k, v, lam, scale=None, causal=False, key_lengths=None):
     head h // (H // Hkv)), D a multiple of 8 up to 64; lam fp32, [H] or one value for all heads -> [B,Nq,H,2D] of that type.  ``scale``
     defaults to D ** -0.5.  ``causal``: query i sees the keys j <= i + Nk - Nq, so that a few new queries stand at the end of a cache.
     ``key_lengths`` [B] int: only the keys below it (clamped to 0 .. Nk) exist; what lies behind it may hold anything.  A row that sees no key
-    is 0 and has no gradient, whatever it and its incoming gradient hold.  Values that are visible to some row should be finite: a row that sees one that is not is not finite itself (NaN too
-    where all its scores are -inf; but one key with a score of -inf has probability 0 in 16-bit types, as in the formula), and so may be rows, and
-    gradients of keys, of the same tile from which only ``causal`` hides it.  Views whose last axis is contiguous and whose rows start at multiples of 16
-    bytes (a slice of a cache) are read where they are, others are copied.  Same bits on every run; no second derivative."""
+    is 0 and has no gradient, whatever it and its incoming gradient hold.  Values that are visible to some row should be finite: a row that sees
+    one that is not is not finite itself (NaN too where all its scores are -inf; but one key with a score of -inf has probability 0 in 16-bit
+    types, as in the formula), and so may be rows, and gradients of keys, of the same tile from which only ``causal`` hides it.  Views whose last
+    axis is contiguous and whose rows start at multiples of 16 bytes (a slice of a cache) are read where they are, others are copied.  Same bits
+    on every run; no second derivative."""
     _typed(q, "q")
     for t, name in ((k, "k"), (v, "v")):
         _typed(t, name, q)
@@ -1298,8 +1299,8 @@ def diff_attention(q, k, v, lam, scale=None, causal=False, key_lengths=None):
             raise ValueError("diff_attention: key_lengths is [B=%d], got %s" % (B, tuple(key_lengths.shape)))
         key_lengths = key_lengths.clamp(0, Nk).to(torch.int32) if key_lengths.dtype == torch.int64 else key_lengths.contiguous()
     if B and Nq and Nk and not _lib.load().hitadv_diff_attention_supported(_DTYPE_CODE[q.dtype], B, Nq, Nk, H, Hkv, D):
-        raise ValueError("diff_attention: D=%d must be a multiple of 8 up to 64, Nq * H / Hkv and Nk at most 2,000,000, B * Hkv at most 65535 and H below 2^22 "
-                         "(q %s, k %s)" % (D, tuple(q.shape), tuple(k.shape)))
+        raise ValueError("diff_attention: D=%d must be a multiple of 8 up to 64, Nq * H / Hkv and Nk at most 2,000,000, B * Hkv at most 65535 and "
+                         "H below 2^22 (q %s, k %s)" % (D, tuple(q.shape), tuple(k.shape)))
     scale = float(D) ** -0.5 if scale is None else float(scale)
     keep = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or lam.requires_grad)
     return DiffAttention.apply(q, k, v, lam, scale, bool(causal), key_lengths, keep)
